@@ -3,8 +3,8 @@ its plain form (elementary torch operations in 32 bits) or through the package's
 
 The cache holds, per page of 16 tokens and per head, 16 rows of 64 bytes of 4-bit codes followed by
 16 rows of four fp16 scales.  A group is 32 neighbouring elements of a head row; with
-``d = 32 g + 8 j + n`` the code of (token t, element d) is the nibble ``n & 1`` of byte
-``64 t + 16 (j ^ ((t >> 1) & 3)) + 4 g + n // 2`` and stands for ``scale[t, g] * (code - 8)``.
+``d = 32 g + 8 j + n`` the code of (token t, element d) is nibble ``n // 2 + 4 (n & 1)`` of the 32-bit
+word at byte ``64 t + 16 (j ^ ((t >> 1) & 3)) + 4 g`` and stands for ``scale[t, g] * (code - 8)``.
 """
 
 from __future__ import annotations
@@ -21,6 +21,7 @@ GROUP = 32             # elements that share a scale
 BLOCK = PS * D // 2 + PS * (D // GROUP) * 2   # bytes of one page of one head: 1152
 EPS = 1e-6
 LOG2E = 1.4426950408889634
+MOST_SCALE = 9352.0    # 7 times it is the largest multiple of 7 scale steps that fp16 holds
 
 
 # ---------------------------------------------------------------------------------------------
@@ -91,7 +92,7 @@ def _quantise(x):
     """fp16 ``[..., 128]`` -> codes 0..15 (uint8 ``[..., 128]``) and scales (fp16 ``[..., 4]``)."""
     g = x.float().unflatten(-1, (D // GROUP, GROUP))
     amax = g.abs().amax(-1)
-    scale = (amax / 7.0).half()
+    scale = (amax / 7.0).half().clamp(max=MOST_SCALE)
     s = scale.double().unsqueeze(-1)                      # 64 bits: values next to a border
     c = torch.floor(torch.where(s > 0, g.double() / s, 0.0) + 0.5).clamp(-8, 7)
     fine = torch.isfinite(amax)
@@ -108,9 +109,15 @@ def _pack_rows(codes, t):
     """Codes ``[n, rows, 128]`` of tokens at page positions ``t`` [n] -> bytes ``[n, rows, 64]``."""
     n, rows = codes.shape[:2]
     c = codes.view(n, rows, 4, 4, 8).transpose(2, 3)       # [n, rows, j, g, 8]
-    c = c[:, :, :, :, 0::2] | (c[:, :, :, :, 1::2] << 4)   # [n, rows, j, g, 4 bytes]
+    c = c.unflatten(-1, (4, 2)).transpose(-1, -2).flatten(-2)   # even elements, then odd ones
+    c = c[..., 0::2] | (c[..., 1::2] << 4)                 # [n, rows, j, g, 4 bytes]
     at = _byte_order(t).view(n, 1, 4, 1, 1).expand(n, rows, 4, 4, 4)
     return torch.gather(c, 2, at).reshape(n, rows, 64)
+
+
+def _nibbles(b):
+    """Bytes ``[..., 4]`` of words -> their eight codes in the order of the elements."""
+    return torch.stack((b & 15, b >> 4), -1).unflatten(-2, (2, 2)).flatten(-2).transpose(-1, -2).flatten(-2)
 
 
 def _unpack_blocks(blocks):
@@ -118,8 +125,7 @@ def _unpack_blocks(blocks):
     b = blocks[..., : PS * 64].unflatten(-1, (PS, 4, 4, 4))
     t = torch.arange(PS, device=blocks.device)
     b = b[..., t.unsqueeze(-1), _byte_order(t), :, :]      # [..., 16, j, g, 4 bytes]
-    c = torch.stack((b & 15, b >> 4), -1).flatten(-2)      # [..., 16, j, g, 8]
-    c = c.transpose(-3, -2).flatten(-2).float() - 8        # [..., 16, g, 32]
+    c = _nibbles(b).transpose(-3, -2).flatten(-2).float() - 8   # [..., 16, g, 32]
     s = blocks[..., PS * 64:].contiguous().view(torch.float16).unflatten(-1, (PS, 4)).float()
     return (c * s.unsqueeze(-1)).flatten(-2)
 
@@ -137,9 +143,9 @@ def _plain_gather(pool, slots):
     rows = pool[..., : PS * 64].unflatten(-1, (PS, 4, 4, 4))[page, :, t]            # [n, rows, 4, 4, 4]
     n, r = rows.shape[:2]
     rows = torch.gather(rows, 2, _byte_order(t).view(n, 1, 4, 1, 1).expand_as(rows))
-    c = torch.stack((rows & 15, rows >> 4), -1).flatten(-2).transpose(2, 3).reshape(n, r, 4, 32).float() - 8
+    c = _nibbles(rows).transpose(2, 3).reshape(n, r, 4, 32).float() - 8
     s = pool.view(torch.float16)[..., PS * 32:].unflatten(-1, (PS, 4))[page, :, t].float()
-    return (c * s.unsqueeze(-1)).flatten(-2).clamp(-65504, 65504).half()
+    return (c * s.unsqueeze(-1)).flatten(-2).half()
 
 
 def _plain_norm(x, weight):
@@ -365,12 +371,13 @@ def _exact_values(pool, slots):
     d = torch.arange(D, device=pool.device)
     g, j, n = d // 32, d % 32 // 8, d % 8
     page, t = slots.long().unsqueeze(-1) // PS, slots.long().unsqueeze(-1) % PS
-    byte = 64 * t + 16 * (j ^ (t // 2 % 4)) + 4 * g + n // 2                    # [n, 128]
+    nibble = n // 2 + 4 * (n % 2)
+    byte = 64 * t + 16 * (j ^ (t // 2 % 4)) + 4 * g + nibble // 2               # [n, 128]
     scale_at = PS * 64 + 8 * t + 2 * g
     flat = pool.view(-1)
     rows = torch.arange(pool.shape[1], device=pool.device).view(1, -1, 1)
     base = (page.unsqueeze(-1) * pool.shape[1] + rows) * BLOCK
-    code = (flat[base + byte.unsqueeze(1)].long() >> (4 * (n % 2))) & 15
+    code = (flat[base + byte.unsqueeze(1)].long() >> (4 * (nibble % 2))) & 15
     scale = pool.view(torch.float16).view(-1)[(base + scale_at.unsqueeze(1)) // 2]
     return (code - 8).double() * scale.double()
 
@@ -378,7 +385,7 @@ def _exact_values(pool, slots):
 def _exact_stored(x):
     """What the cache stands for after fp16 values ``x`` were appended: fp64, same shape."""
     g = x.double().view(*x.shape[:-1], D // GROUP, GROUP)
-    scale = (g.abs().max(-1).values / 7).half().double().unsqueeze(-1)
+    scale = (g.abs().max(-1).values / 7).half().double().clamp(max=MOST_SCALE).unsqueeze(-1)
     c = torch.where(scale == 0, torch.zeros_like(g), torch.floor(g / scale + 0.5)).clamp(-8, 7)
     return (c * scale).view(x.shape)
 
