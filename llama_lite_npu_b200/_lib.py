@@ -106,6 +106,40 @@ _SIGNATURES = {
          c_void_p, c_int64, c_int64,
          c_void_p, c_void_p],
     ),
+    # 4-bit paged cache (include/b200kv_kv4.h)
+    "b200kv_kv4_append": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_int64, c_int64, c_void_p,   # K, V, tokens, strides, slots
+         c_void_p, c_int64, c_int64, c_int, c_int,                  # pool, pages, page stride, heads, dim
+         c_void_p, c_void_p],
+    ),
+    "b200kv_kv4_qk_norm_rope_append": (
+        c_int,
+        [c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_int64,
+         c_void_p, c_void_p, c_float, c_void_p, c_void_p, c_int64, c_void_p,
+         c_void_p, c_int64, c_int64, c_int64, c_int, c_int, c_int, c_void_p, c_void_p],
+    ),
+    "b200kv_kv4_gather": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_int64, c_int, c_int, c_void_p, c_void_p],
+    ),
+    "b200kv_stream_capture_id": (c_int, [c_void_p, c_void_p]),
+    "b200kv_kv4_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "b200kv_kv4_paged_decode": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,    # q, pool
+         c_void_p, c_int64, c_int, c_int, c_int64, c_void_p,        # table, row ids
+         c_void_p, c_int, c_int, c_int, c_int, c_int, c_int,        # lengths, batch, heads, dims
+         c_float, c_int64, c_void_p, c_size_t, c_void_p, c_int64, c_int64,
+         c_int, c_void_p, c_void_p],
+    ),
+    "b200kv_kv4_paged_prefill": (
+        c_int,
+        [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
+         c_void_p, c_int64, c_int, c_int, c_int64, c_void_p, c_void_p,
+         c_void_p, c_void_p, c_int, c_int, c_int64, c_int64,
+         c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p],
+    ),
     # host-side prefix cache (include/b200kv_prefix_cache.h)
     "b200kv_prefix_cache_create": (c_void_p, [c_int, c_int64, c_int64]),
     "b200kv_prefix_cache_destroy": (None, [c_void_p]),

@@ -30,6 +30,8 @@ SOURCES = (
     "paged_prefill_sm100.cu",
     "prefix_cache.cpp",
     "host_step.cu",
+    "kv4_append.cu",
+    "kv4_decode.cu",
 )
 
 NVCC_FLAGS = (

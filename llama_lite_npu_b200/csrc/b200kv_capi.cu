@@ -5,6 +5,7 @@
 #include <cstring>
 
 #include "b200kv.h"
+#include "b200kv_kv4.h"
 #include "launch.h"
 
 namespace b200kv {
@@ -301,6 +302,165 @@ int b200kv_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, 
   a.out_stride_h = out_stride_h;
   a.status = status;
   return b200kv::paged_prefill(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_kv4_append(const void* k_values, const void* v_values, int64_t n_tokens, int64_t k_tok_stride,
+                      int64_t v_tok_stride, const int32_t* slots, void* pool, int64_t pool_pages,
+                      int64_t page_stride_bytes, int kv_heads, int head_dim, int32_t* status, void* stream) {
+  b200kv::Kv4AppendArgs a{};
+  a.k = k_values;
+  a.v = v_values;
+  a.k_tok_stride = k_tok_stride;
+  a.v_tok_stride = v_tok_stride;
+  a.slots = slots;
+  a.pool = pool;
+  a.pool_pages = pool_pages;
+  a.page_stride_bytes = page_stride_bytes;
+  a.n_tokens = n_tokens;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.status = status;
+  return b200kv::kv4_append(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_kv4_qk_norm_rope_append(const void* q, void* q_out, int64_t q_tok_stride, int64_t q_out_tok_stride,
+                                   const void* kv, int64_t kv_tok_stride, const void* q_weight,
+                                   const void* k_weight, float eps, const void* cos, const void* sin,
+                                   int64_t cs_tok_stride, const int32_t* slots, void* pool, int64_t pool_pages,
+                                   int64_t page_stride_bytes, int64_t n_tokens, int q_heads, int kv_heads,
+                                   int head_dim, int32_t* status, void* stream) {
+  if (n_tokens > 0 && (q == nullptr || kv == nullptr)) return B200KV_EINVAL;
+  if (kv_heads <= 0 || q_heads <= 0) return B200KV_EINVAL;
+  if (kv_heads > 1024) return B200KV_ETOOLARGE;
+  if (head_dim != 128) return B200KV_EUNSUPPORTED;
+  // one row per token holds K and V, so its stride has to hold both
+  if (n_tokens > 0 && kv_tok_stride < static_cast<int64_t>(2) * kv_heads * head_dim) return B200KV_EINVAL;
+  b200kv::Kv4AppendArgs a{};
+  a.k = kv;
+  a.v = kv ? static_cast<const char*>(kv) + static_cast<size_t>(kv_heads) * head_dim * 2 : nullptr;
+  a.k_tok_stride = kv_tok_stride;
+  a.v_tok_stride = kv_tok_stride;
+  a.slots = slots;
+  a.pool = pool;
+  a.pool_pages = pool_pages;
+  a.page_stride_bytes = page_stride_bytes;
+  a.n_tokens = n_tokens;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.status = status;
+  a.q = q;
+  a.q_out = q_out;
+  a.q_tok_stride = q_tok_stride;
+  a.q_out_tok_stride = q_out_tok_stride;
+  a.q_weight = q_weight;
+  a.k_weight = k_weight;
+  a.eps = eps;
+  a.cos = cos;
+  a.sin = sin;
+  a.cs_tok_stride = cs_tok_stride;
+  a.q_heads = q_heads;
+  return b200kv::kv4_append(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_kv4_gather(const void* pool, int64_t pool_pages, int64_t page_stride_bytes, const int32_t* slots,
+                      int64_t n, void* out, int64_t out_tok_stride, int kv_heads, int head_dim, int32_t* status,
+                      void* stream) {
+  return b200kv::kv4_gather(pool, pool_pages, page_stride_bytes, slots, n, out, out_tok_stride, kv_heads, head_dim,
+                            status, static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_stream_capture_id(void* stream, uint64_t* id) {
+  if (id == nullptr) return B200KV_EINVAL;
+  *id = 0;
+  cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+  unsigned long long cap = 0;
+  const cudaError_t e = cudaStreamGetCaptureInfo(static_cast<cudaStream_t>(stream), &st, &cap);
+  if (e != cudaSuccess) return b200kv::record_cuda_error(e);
+  if (st == cudaStreamCaptureStatusActive) *id = cap;
+  return B200KV_OK;
+}
+
+size_t b200kv_kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim) {
+  return b200kv::kv4_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim);
+}
+
+int b200kv_kv4_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* pool,
+                            int64_t pool_pages, int64_t page_stride_bytes, const int32_t* table,
+                            int64_t table_row_stride, int table_kind, int table_rows, int64_t table_cols,
+                            const int32_t* row_ids, const void* seq_lens, int seq_lens_i64, int batch,
+                            int q_heads, int kv_heads, int head_dim, int page_size, float scale,
+                            int64_t max_seq_len, void* workspace, size_t workspace_bytes, void* out,
+                            int64_t out_stride_b, int64_t out_stride_h, int flags, int32_t* status,
+                            void* stream) {
+  b200kv::Kv4DecodeArgs a{};
+  a.q = q;
+  a.q_stride_b = q_stride_b;
+  a.q_stride_h = q_stride_h;
+  a.pool = pool;
+  a.pool_pages = pool_pages;
+  a.page_stride_bytes = page_stride_bytes;
+  a.table = table;
+  a.table_row_stride = table_row_stride;
+  a.table_kind = table_kind;
+  a.table_rows = table_rows;
+  a.table_cols = table_cols;
+  a.row_ids = row_ids;
+  a.seq_lens = seq_lens;
+  a.seq_lens_i64 = seq_lens_i64;
+  a.batch = batch;
+  a.q_heads = q_heads;
+  a.kv_heads = kv_heads;
+  a.head_dim = head_dim;
+  a.page_size = page_size;
+  a.scale = scale;
+  a.max_seq_len = max_seq_len;
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
+  a.out = out;
+  a.out_stride_b = out_stride_b;
+  a.out_stride_h = out_stride_h;
+  a.flags = flags;
+  a.status = status;
+  return b200kv::kv4_paged_decode(a, static_cast<cudaStream_t>(stream));
+}
+
+int b200kv_kv4_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h, const void* pool,
+                             int64_t pool_pages, int64_t page_stride_bytes, const int32_t* table,
+                             int64_t table_row_stride, int table_kind, int table_rows, int64_t table_cols,
+                             const int32_t* req_ids, const int32_t* q_start, const void* ctx_lens,
+                             const void* q_lens, int lens_i64, int batch, int64_t total_q, int64_t max_q_len,
+                             int q_heads, int kv_heads, int head_dim, int page_size, float scale_log2, void* out,
+                             int64_t out_stride_t, int64_t out_stride_h, int32_t* status, void* stream) {
+  b200kv::Kv4PrefillArgs a{};
+  a.pool = pool;
+  a.pool_pages = pool_pages;
+  a.page_stride_bytes = page_stride_bytes;
+  a.args.q = q;
+  a.args.q_stride_t = q_stride_t;
+  a.args.q_stride_h = q_stride_h;
+  a.args.table = table;
+  a.args.table_row_stride = table_row_stride;
+  a.args.table_kind = table_kind;
+  a.args.table_rows = table_rows;
+  a.args.table_cols = table_cols;
+  a.args.req_ids = req_ids;
+  a.args.q_start = q_start;
+  a.args.ctx_lens = ctx_lens;
+  a.args.q_lens = q_lens;
+  a.args.lens_i64 = lens_i64;
+  a.args.batch = batch;
+  a.args.total_q = total_q;
+  a.args.max_q_len = max_q_len;
+  a.args.q_heads = q_heads;
+  a.args.kv_heads = kv_heads;
+  a.args.head_dim = head_dim;
+  a.args.page_size = page_size;
+  a.args.scale_log2 = scale_log2;
+  a.args.out = out;
+  a.args.out_stride_t = out_stride_t;
+  a.args.out_stride_h = out_stride_h;
+  a.args.status = status;
+  return b200kv::kv4_paged_prefill(a, static_cast<cudaStream_t>(stream));
 }
 
 int b200kv_selftest_bounded_wait(uint64_t limit_ns, int32_t* result, int32_t* status, void* stream) {

@@ -1,0 +1,417 @@
+// Writers of the 4-bit paged cache, and the read-back of its rows.
+//
+// Append: the K and V rows of a token, as they are or straight from the projections (per-head RMSNorm
+// and rotary embedding on the way, as in qk_prologue.cu), quantised in groups of 32 elements and
+// scattered by slot_mapping.  With x the fp16 values of a group:
+//   s = min(fp16(max |x| / 7), 9352),   code = clamp(floor(x / s + 1/2), -8, 7) + 8.
+// K is rounded to fp16 after the rotation, as the fp16 pool would hold it, so a cache filled through
+// this launch and one filled from an fp16 pool's rows hold the same codes.
+//
+// The codes have to be exactly those of the definition, although x / s is evaluated as x * (1 / s):
+// x and s have 11-bit significands, so x / s is either exactly a border k + 1/2 or at least 2^-13
+// away from it, and the product is off by less than 2^-20; adding 2^-14 before the floor therefore
+// puts ties on the upper side and moves nothing else.  max|x| / 7 is at least 2^-15 (relative) away from
+// every tie of its rounding to fp16, so the product with the rounded 1/7 rounds the same.  The norm's
+// mean square of a K row is summed in 64 bits: a reciprocal root that is one unit off would move
+// about one K in 4000 to the neighbouring fp16 number and now and then a code with it.  Q keeps
+// 32-bit statistics: its rows are rounded once and nothing is decided by them.
+//
+// A warp takes one head row of four neighbouring tokens, eight lanes to a row.  A lane owns 8
+// elements of the first half of head_dim and the 8 they rotate with, i.e. one 32-bit word of codes in
+// each of two groups; the words of lanes l and l ^ 4 make up one 16-byte chunk of the row.  Four
+// neighbouring tokens of a page are 256 contiguous bytes of codes and one 32-byte sector of scales.
+// HBM-bound: per token 2 * KH * 256 B read and 2 * KH * 72 B written (+ 2 * QH * 256 B of Q and 256 B of
+// cos / sin for the fused form).
+#include "kv4.cuh"
+#include "launch.h"
+
+namespace b200kv {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kD = kv4::kHeadDim;
+constexpr int kHalf = kD / 2;
+constexpr int kTokPerWarp = 4;
+constexpr float kMaxScale = 9352.f;   // 7 * 9352 = 65464 is a value fp16 can hold after rounding
+
+struct AppendParams {
+  const __half* k;            // kFused: the kv projection's rows (K heads, then V heads)
+  const __half* v;
+  int64_t k_tok_stride, v_tok_stride;
+  const int32_t* slots;
+  uint8_t* pool;
+  int64_t pool_tokens, page_stride;
+  int n_tokens, q_heads, kv_heads;
+  int rows_per_token;         // head rows of a token: 2 * kv_heads (+ q_heads)
+  int quads;                  // ceil(n_tokens / 4)
+  int step_quad, step_row;    // (warps in the grid) / and % rows_per_token
+  int32_t* status;
+  // fused form only
+  const __half* q;
+  __half* q_out;
+  int64_t q_tok_stride, q_out_tok_stride;
+  const __half* q_weight;     // nullptr: no norm
+  const __half* k_weight;
+  const __half* cos;
+  const __half* sin;
+  int64_t cs_tok_stride;
+  float eps;
+};
+
+__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
+  return make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+}
+// x * rrms rounded to fp16, times the fp16 weight in fp16 (the reference's roundings, qk_prologue.cu).
+__device__ __forceinline__ void norm8(float (&x)[8], float rrms, const uint4& w) {
+  const uint32_t wp[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 y = __floats2half2_rn(x[2 * i] * rrms, x[2 * i + 1] * rrms);
+    const float2 f = __half22float2(__hmul2(y, *reinterpret_cast<const __half2*>(&wp[i])));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// One group's share of a lane: its 8 elements -> a word of codes; the scale (fp16 bits) is the same in
+// the four lanes of the group.  Called by whole warps.
+__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& scale_bits) {
+  float amax = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) amax = max_nan(amax, fabsf(x[i]));
+  amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+  amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+  const bool fine = amax <= 65504.f;   // false for infinities and NaN
+  const __half sh = __float2half_rn(fminf(amax * (1.f / 7.f), kMaxScale));
+  const float s = __half2float(sh);
+  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
+  uint32_t word = 0;
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    const float t = fminf(fmaxf(fmaf(x[n], inv, 8.5f + 1.f / 16384.f), 0.f), 15.5f);
+    const uint32_t u = __float_as_uint(__fadd_rd(t, 8388608.f));   // low bits: floor(t)
+    const int shift = 4 * ((n >> 1) + 4 * (n & 1));
+    word |= (u << shift) & (15u << shift);
+  }
+  scale_bits = fine ? static_cast<uint32_t>(__half_as_ushort(sh)) : 0x7E00u;   // NaN: never read as a number
+  return fine ? word : 0x88888888u;
+}
+
+template <bool kFused>
+__global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendParams p) {
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+  const int lane = threadIdx.x & 31;
+  const int sub = lane & 7;
+  const unsigned warp = (blockIdx.x * kThreads + threadIdx.x) >> 5;
+  int quad = static_cast<int>(warp / static_cast<unsigned>(p.rows_per_token));
+  int row = static_cast<int>(warp % static_cast<unsigned>(p.rows_per_token));
+  while (quad < p.quads) {
+    const int64_t tok = static_cast<int64_t>(quad) * kTokPerWarp + (lane >> 3);
+    const bool live = tok < p.n_tokens;
+    // row of the warp: Q head, K head or V head (the same for all lanes)
+    const int kv_row = kFused ? row - p.q_heads : row;
+    const bool is_q = kFused && kv_row < 0;
+    const bool is_v = kv_row >= p.kv_heads;
+    uint4 ua = make_uint4(0, 0, 0, 0), ub = ua, uc = ua, us = ua;
+    int64_t slot = -1;
+    if (live) {
+      const __half* src;
+      if (is_q) src = p.q + tok * p.q_tok_stride + row * kD;
+      else if (is_v) src = p.v + tok * p.v_tok_stride + (kv_row - p.kv_heads) * kD;
+      else src = p.k + tok * p.k_tok_stride + kv_row * kD;
+      ua = __ldg(reinterpret_cast<const uint4*>(src + sub * 8));
+      ub = __ldg(reinterpret_cast<const uint4*>(src + kHalf + sub * 8));
+      if (kFused && !is_v) {
+        uc = __ldg(reinterpret_cast<const uint4*>(p.cos + tok * p.cs_tok_stride + sub * 8));
+        us = __ldg(reinterpret_cast<const uint4*>(p.sin + tok * p.cs_tok_stride + sub * 8));
+      }
+      if (!is_q) slot = __ldg(p.slots + tok);
+    }
+    float a[8], b[8];
+    unpack8(ua, a);
+    unpack8(ub, b);
+    if (kFused && !is_v) {
+      const __half* weight = is_q ? p.q_weight : p.k_weight;
+      if (weight != nullptr) {
+        const uint4 wa = __ldg(reinterpret_cast<const uint4*>(weight + sub * 8));
+        const uint4 wb = __ldg(reinterpret_cast<const uint4*>(weight + kHalf + sub * 8));
+        float mean;
+        if (is_q) {
+          float ss = 0.f;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
+#pragma unroll
+          for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+          mean = ss * (1.f / kD);
+        } else {
+          double ss = 0.;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)   // products of two fp16 numbers are exact in 32 bits
+            ss += static_cast<double>(a[i] * a[i]) + static_cast<double>(b[i] * b[i]);
+#pragma unroll
+          for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+          mean = static_cast<float>(ss * (1. / kD));
+        }
+        const float rrms = __fdiv_rn(1.f, __fsqrt_rn(mean + p.eps));
+        norm8(a, rrms, wa);
+        norm8(b, rrms, wb);
+      }
+      float c[8], s[8];
+      unpack8(uc, c);
+      unpack8(us, s);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {   // the products are exact, so each element is rounded once
+        const float x1 = a[i], x2 = b[i];
+        a[i] = x1 * c[i] - x2 * s[i];
+        b[i] = x2 * c[i] + x1 * s[i];
+      }
+      ua = pack8(a);
+      ub = pack8(b);
+    }
+    if (is_q) {
+      if (live) {
+        __half* dst = p.q_out + tok * p.q_out_tok_stride + row * kD;
+        *reinterpret_cast<uint4*>(dst + sub * 8) = ua;
+        *reinterpret_cast<uint4*>(dst + kHalf + sub * 8) = ub;
+      }
+    } else {
+      if (kFused && !is_v) {
+        unpack8(ua, a);
+        unpack8(ub, b);
+      }
+      uint32_t s1, s2;
+      const uint32_t w1 = quantise8(a, s1), w2 = quantise8(b, s2);   // groups sub / 4 and 2 + sub / 4
+      const uint32_t pw1 = __shfl_xor_sync(0xffffffffu, w1, 4), pw2 = __shfl_xor_sync(0xffffffffu, w2, 4);
+      const uint32_t ps = __shfl_xor_sync(0xffffffffu, s1 | (s2 << 16), 4);
+      if (live) {
+        if (slot < 0 || slot >= p.pool_tokens) {
+          set_status(p.status, B200KV_DEV_BAD_SLOT);
+        } else if (sub < 4) {
+          const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
+          uint8_t* block = p.pool + (slot / kv4::kPageTok) * p.page_stride + static_cast<int64_t>(kv_row) * kv4::kBlockBytes;
+          *reinterpret_cast<uint4*>(block + kv4::chunk_offset(t, sub)) = make_uint4(w1, pw1, w2, pw2);
+          if (sub == 0)
+            *reinterpret_cast<uint2*>(block + kv4::kScaleOffset + t * kv4::kScaleBytes) =
+                make_uint2(s1 | (ps << 16), s2 | (ps & 0xffff0000u));
+        }
+      }
+    }
+    quad += p.step_quad;
+    row += p.step_row;
+    if (row >= p.rows_per_token) {
+      row -= p.rows_per_token;
+      ++quad;
+    }
+  }
+}
+
+// Read-back: four lanes to a row, a lane reads one 16-byte chunk (8 elements in each of the four
+// groups) and the row's four scales and writes four 16-byte pieces; the four lanes of a row write 64
+// contiguous bytes per store.  A warp takes one head row of eight neighbouring tokens.  HBM-bound: per
+// token 2 * KH * (72 + 256) B.
+struct GatherParams {
+  const uint8_t* pool;
+  int64_t pool_tokens, page_stride;
+  const int32_t* slots;
+  __half* out;
+  int64_t out_tok_stride;
+  int n, rows;
+  int octets, step_octet, step_row;
+  int32_t* status;
+};
+
+__global__ void __launch_bounds__(kThreads) kv4_gather_kernel(GatherParams p) {
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+  const int lane = threadIdx.x & 31;
+  const int j = lane & 3;
+  const unsigned warp = (blockIdx.x * kThreads + threadIdx.x) >> 5;
+  int octet = static_cast<int>(warp / static_cast<unsigned>(p.rows));
+  int row = static_cast<int>(warp % static_cast<unsigned>(p.rows));
+  while (octet < p.octets) {
+    const int64_t tok = static_cast<int64_t>(octet) * 8 + (lane >> 2);
+    if (tok < p.n) {
+      const int64_t slot = __ldg(p.slots + tok);
+      uint4 codes = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+      uint2 scales = make_uint2(0, 0);
+      if (slot < 0 || slot >= p.pool_tokens) {
+        set_status(p.status, B200KV_DEV_BAD_SLOT);
+      } else {
+        const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
+        const uint8_t* block = kv4::block_at(p.pool, slot / kv4::kPageTok, p.page_stride, row);
+        codes = *reinterpret_cast<const uint4*>(block + kv4::chunk_offset(t, j));
+        scales = *reinterpret_cast<const uint2*>(block + kv4::kScaleOffset + t * kv4::kScaleBytes);
+      }
+      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+      const uint32_t s2[4] = {__byte_perm(scales.x, 0, 0x1010), __byte_perm(scales.x, 0, 0x3232),
+                              __byte_perm(scales.y, 0, 0x1010), __byte_perm(scales.y, 0, 0x3232)};
+      __half* dst = p.out + tok * p.out_tok_stride + row * kD + 8 * j;
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        uint32_t v[4];
+        kv4::unpack_word(w[g], v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = kv4::h2_mul(v[i], s2[g]);
+        *reinterpret_cast<uint4*>(dst + 32 * g) = make_uint4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    octet += p.step_octet;
+    row += p.step_row;
+    if (row >= p.rows) {
+      row -= p.rows;
+      ++octet;
+    }
+  }
+}
+
+inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// Grid of one warp per work item, at most `per_sm` CTAs of 256 threads per SM (grid-stride above).
+int grid_for(int64_t items, int per_sm, unsigned* blocks) {
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200KV_ECUDA;
+  int64_t b = (items + kThreads / 32 - 1) / (kThreads / 32);
+  const int64_t cap = static_cast<int64_t>(sms) * per_sm;
+  if (b > cap) b = cap;
+  *blocks = static_cast<unsigned>(b);
+  return B200KV_OK;
+}
+
+template <typename Kernel, typename Params>
+int launch(Kernel kernel, const Params& p, unsigned blocks, cudaStream_t stream) {
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(kThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  if (e != cudaSuccess) return record_cuda_error(e);
+  return check_launch();
+}
+
+constexpr int kCtasPerSm = 8;
+
+template <bool kFused>
+int launch_append(AppendParams p, cudaStream_t stream) {
+  p.rows_per_token = 2 * p.kv_heads + (kFused ? p.q_heads : 0);
+  p.quads = (p.n_tokens + kTokPerWarp - 1) / kTokPerWarp;
+  unsigned blocks = 0;
+  const int rc = grid_for(static_cast<int64_t>(p.quads) * p.rows_per_token, kCtasPerSm, &blocks);
+  if (rc != B200KV_OK) return rc;
+  const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
+  p.step_quad = static_cast<int>(warps / p.rows_per_token);
+  p.step_row = static_cast<int>(warps % p.rows_per_token);
+  return launch(kv4_append_kernel<kFused>, p, blocks, stream);
+}
+
+}  // namespace
+
+int kv4_check_pool(const void* pool, int64_t pool_pages, int64_t page_stride_bytes, int kv_heads) {
+  if (!pool || pool_pages <= 0 || kv_heads <= 0) return B200KV_EINVAL;
+  if (pool_pages > (int64_t{1} << 27)) return B200KV_ETOOLARGE;   // slots are int32
+  if (kv_heads > 1024) return B200KV_ETOOLARGE;
+  if (!aligned16(pool) || page_stride_bytes % 16 != 0) return B200KV_EALIGN;
+  if (page_stride_bytes < static_cast<int64_t>(2) * kv_heads * kv4::kBlockBytes) return B200KV_EINVAL;
+  return B200KV_OK;
+}
+
+int kv4_append(const Kv4AppendArgs& a, cudaStream_t stream) {
+  if (a.n_tokens < 0 || a.kv_heads <= 0) return B200KV_EINVAL;
+  if (a.head_dim != kD) return B200KV_EUNSUPPORTED;
+  if (a.n_tokens == 0) return B200KV_OK;
+  if (a.n_tokens > (1 << 30)) return B200KV_ETOOLARGE;
+  if (!a.k || !a.v || !a.slots) return B200KV_EINVAL;
+  int rc = kv4_check_pool(a.pool, a.pool_pages, a.page_stride_bytes, a.kv_heads);
+  if (rc != B200KV_OK) return rc;
+  if (a.k_tok_stride % 8 || a.v_tok_stride % 8 || !aligned16(a.k) || !aligned16(a.v)) return B200KV_EALIGN;
+  const int64_t half = static_cast<int64_t>(a.kv_heads) * kD;
+  if (a.k_tok_stride < half || a.v_tok_stride < half) return B200KV_EINVAL;
+  AppendParams p{};
+  p.k = static_cast<const __half*>(a.k);
+  p.v = static_cast<const __half*>(a.v);
+  p.k_tok_stride = a.k_tok_stride;
+  p.v_tok_stride = a.v_tok_stride;
+  p.slots = a.slots;
+  p.pool = static_cast<uint8_t*>(a.pool);
+  p.pool_tokens = a.pool_pages * kv4::kPageTok;
+  p.page_stride = a.page_stride_bytes;
+  p.n_tokens = static_cast<int>(a.n_tokens);
+  p.kv_heads = a.kv_heads;
+  p.status = a.status;
+  if (a.q == nullptr) return launch_append<false>(p, stream);
+
+  if (!a.q_out || !a.cos || !a.sin || a.q_heads <= 0 || !(a.eps >= 0.f)) return B200KV_EINVAL;
+  if (a.q_heads > 65536) return B200KV_ETOOLARGE;
+  if (a.q_tok_stride % 8 || a.q_out_tok_stride % 8 || a.cs_tok_stride % 8) return B200KV_EALIGN;
+  if (!aligned16(a.q) || !aligned16(a.q_out) || !aligned16(a.cos) || !aligned16(a.sin) ||
+      (a.q_weight && !aligned16(a.q_weight)) || (a.k_weight && !aligned16(a.k_weight)))
+    return B200KV_EALIGN;
+  if (a.q_tok_stride < static_cast<int64_t>(a.q_heads) * kD || a.q_out_tok_stride < static_cast<int64_t>(a.q_heads) * kD ||
+      a.cs_tok_stride < kHalf)
+    return B200KV_EINVAL;
+  p.q = static_cast<const __half*>(a.q);
+  p.q_out = static_cast<__half*>(a.q_out);
+  p.q_tok_stride = a.q_tok_stride;
+  p.q_out_tok_stride = a.q_out_tok_stride;
+  p.q_heads = a.q_heads;
+  p.q_weight = static_cast<const __half*>(a.q_weight);
+  p.k_weight = static_cast<const __half*>(a.k_weight);
+  p.cos = static_cast<const __half*>(a.cos);
+  p.sin = static_cast<const __half*>(a.sin);
+  p.cs_tok_stride = a.cs_tok_stride;
+  p.eps = a.eps;
+  return launch_append<true>(p, stream);
+}
+
+int kv4_gather(const void* pool, int64_t pool_pages, int64_t page_stride_bytes, const int32_t* slots, int64_t n,
+               void* out, int64_t out_tok_stride, int kv_heads, int head_dim, int32_t* status, cudaStream_t stream) {
+  if (n < 0 || kv_heads <= 0) return B200KV_EINVAL;
+  if (head_dim != kD) return B200KV_EUNSUPPORTED;
+  if (n == 0) return B200KV_OK;
+  if (n > (1 << 30)) return B200KV_ETOOLARGE;
+  if (!slots || !out) return B200KV_EINVAL;
+  int rc = kv4_check_pool(pool, pool_pages, page_stride_bytes, kv_heads);
+  if (rc != B200KV_OK) return rc;
+  if (!aligned16(out) || out_tok_stride % 8 != 0) return B200KV_EALIGN;
+  if (out_tok_stride < static_cast<int64_t>(2) * kv_heads * kD) return B200KV_EINVAL;
+  GatherParams p{};
+  p.pool = static_cast<const uint8_t*>(pool);
+  p.pool_tokens = pool_pages * kv4::kPageTok;
+  p.page_stride = page_stride_bytes;
+  p.slots = slots;
+  p.out = static_cast<__half*>(out);
+  p.out_tok_stride = out_tok_stride;
+  p.n = static_cast<int>(n);
+  p.rows = 2 * kv_heads;
+  p.octets = static_cast<int>((n + 7) / 8);
+  p.status = status;
+  unsigned blocks = 0;
+  rc = grid_for(static_cast<int64_t>(p.octets) * p.rows, kCtasPerSm, &blocks);
+  if (rc != B200KV_OK) return rc;
+  const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
+  p.step_octet = static_cast<int>(warps / p.rows);
+  p.step_row = static_cast<int>(warps % p.rows);
+  return launch(kv4_gather_kernel, p, blocks, stream);
+}
+
+}  // namespace b200kv

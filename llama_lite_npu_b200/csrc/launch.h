@@ -125,6 +125,67 @@ struct PrefillArgs {
   int32_t* status;
 };
 int paged_prefill(const PrefillArgs& a, cudaStream_t stream);
+
+// The 4-bit paged cache (include/b200kv_kv4.h).
+struct Kv4AppendArgs {
+  const void* k;   // fused form: the kv projection's rows, v = k + kv_heads * head_dim
+  const void* v;
+  int64_t k_tok_stride, v_tok_stride;
+  const int32_t* slots;
+  void* pool;
+  int64_t pool_pages, page_stride_bytes;
+  int64_t n_tokens;
+  int kv_heads, head_dim;
+  int32_t* status;
+  // fused norm + rotation (q == nullptr: none)
+  const void* q;
+  void* q_out;
+  int64_t q_tok_stride, q_out_tok_stride;
+  const void* q_weight;
+  const void* k_weight;
+  float eps;
+  const void* cos;
+  const void* sin;
+  int64_t cs_tok_stride;
+  int q_heads;
+};
+// Checks every entry point over a kv4 pool makes of the pool itself.
+int kv4_check_pool(const void* pool, int64_t pool_pages, int64_t page_stride_bytes, int kv_heads);
+int kv4_append(const Kv4AppendArgs& a, cudaStream_t stream);
+int kv4_gather(const void* pool, int64_t pool_pages, int64_t page_stride_bytes, const int32_t* slots, int64_t n,
+               void* out, int64_t out_tok_stride, int kv_heads, int head_dim, int32_t* status, cudaStream_t stream);
+
+struct Kv4DecodeArgs {
+  const void* q;
+  int64_t q_stride_b, q_stride_h;
+  const void* pool;
+  int64_t pool_pages, page_stride_bytes;
+  const int32_t* table;
+  int64_t table_row_stride;
+  int table_kind;
+  int table_rows;
+  int64_t table_cols;
+  const int32_t* row_ids;
+  const void* seq_lens;
+  int seq_lens_i64;
+  int batch, q_heads, kv_heads, head_dim, page_size;
+  float scale;
+  int64_t max_seq_len;
+  void* workspace;
+  size_t workspace_bytes;
+  void* out;
+  int64_t out_stride_b, out_stride_h;
+  int flags;
+  int32_t* status;
+};
+size_t kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim);
+int kv4_paged_decode(const Kv4DecodeArgs& a, cudaStream_t stream);
+struct Kv4PrefillArgs {
+  PrefillArgs args;   // k_base, v_base, kv strides and pool_tokens unused
+  const void* pool;
+  int64_t pool_pages, page_stride_bytes;
+};
+int kv4_paged_prefill(const Kv4PrefillArgs& a, cudaStream_t stream);
 int wait_selftest(uint64_t limit_ns, int32_t* result, int32_t* status, cudaStream_t stream);
 
 }  // namespace b200kv

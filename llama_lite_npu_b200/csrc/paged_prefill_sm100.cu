@@ -38,9 +38,21 @@
 // in the reference (:166, :220), output fp16.  Tensor-bound:
 // flops = 4 * 128 * sum over (query, visible key) pairs, per query head.
 //
+// Over a 4-bit cache (kKv4, include/b200kv_kv4.h) the same pipeline runs with two more warps: they read
+// the blocks of codes and scales straight from the pool, four pages ahead of use in registers, turn them
+// into fp16 (code - 8) * scale, and store each word of codes as one 16-byte piece of the K or V tile
+// where the copies would have put it.  A block read costs 72 bytes per row instead of 256, and a tile is
+// converted in less time than the tensor core and the softmax warps spend on it.  A group of V whose
+// scale is NaN must reach only the rows that see its token, and 0 * NaN would reach all: such groups
+// are stored as zeros, the first such position of each group is kept, and the read-out writes NaN from
+// that position on.
+//
 // Every wait is an mbarrier try-wait bounded by ~2 s of %globaltimer; a wait that runs out sets
 // B200KV_DEV_WAIT_TIMEOUT, and every warp still reaches the common exit where TMEM is freed.
+#include <climits>
+
 #include "common.cuh"
+#include "kv4.cuh"
 #include "launch.h"
 #include "tma.h"
 
@@ -59,7 +71,9 @@ constexpr int kGroups = 2;           // query tiles (heads) per CTA
 constexpr int kGroupWarps = 4;       // softmax warps per tile
 constexpr int kProducerWarp = kGroups * kGroupWarps;
 constexpr int kMmaWarp = kProducerWarp + 1;
-constexpr int kThreads = (kMmaWarp + 1) * 32;
+constexpr int kConvertWarps = 2;     // 4-bit pool only
+constexpr int kConvertThreads = kConvertWarps * 32;
+constexpr int threads_of(bool kv4) { return (kMmaWarp + 1 + (kv4 ? kConvertWarps : 0)) * 32; }
 constexpr int kQBytes = kBM * kD * 2;          // 32 KB: [2 d-chunks][128 rows][128 B]
 constexpr int kTileBytes = kBN * kD * 2;       // 32 KB: K or V tile, [2 d-chunks][128 keys][128 B]
 constexpr int kPBytes = kBM * kBN * 2;         // 32 KB: [2 key-chunks][128 rows][128 B]
@@ -192,9 +206,14 @@ struct PrefillParams {
   int64_t out_stride_t, out_stride_h;
   int32_t* status;
   int tiles_m;
+  // 4-bit pool only
+  const uint8_t* pool;
+  int64_t pool_pages, page_stride;
+  int kv_heads;
 };
 
-__global__ void __launch_bounds__(kThreads, 1)
+template <bool kKv4>
+__global__ void __launch_bounds__(threads_of(kKv4), 1)
 paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -202,6 +221,10 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
   const int lane = tid & 31;
   const int warp = tid >> 5;
 
+  if (kKv4) {   // lengths, rows and the pool may all come straight from the kernel before
+    cudaGridDependencySynchronize();
+    cudaTriggerProgrammaticLaunchCompletion();
+  }
   // ---- which work item is this? (heavy query tiles first) ------------------------------------
   const int pairs_per_group = (p.group + 1) / 2;
   const int kv_head = static_cast<int>(blockIdx.x) / pairs_per_group;
@@ -276,7 +299,8 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
   const uint32_t bar_sfree = bar_pvfull + 8 * kGroups;      // [kGroups] S_g of a tile is in registers
   const uint32_t bar_qfree = bar_sfree + 8 * kGroups;       // every S of a query tile has completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_qfree + 8 - sm_q));
-  static_assert(8 + 2 * 8 * kSlots + 4 * 8 * kGroups + 8 + 8 <= kBarBytes, "barrier area too small");
+  int* nan_pos = reinterpret_cast<int*>(tmem_slot + 2);    // [4] first position whose V group reads as NaN
+  static_assert(8 + 2 * 8 * kSlots + 4 * 8 * kGroups + 8 + 8 + 16 <= kBarBytes, "barrier area too small");
   if ((sm_q & 1023u) != 0) {  // swizzled boxes and UMMA descriptors assume 1024-byte alignment
     set_status(p.status, B200KV_DEV_BAD_PAGE);
     leave_early();
@@ -287,7 +311,7 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     mbar_init(bar_q, 1);
     mbar_init(bar_qfree, 1);
     for (int i = 0; i < kSlots; ++i) {
-      mbar_init(bar_full + 8 * i, 1);
+      mbar_init(bar_full + 8 * i, kKv4 ? kConvertThreads : 1);
       mbar_init(bar_empty + 8 * i, 1);
     }
     for (int g = 0; g < kGroups; ++g) {
@@ -296,6 +320,8 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
       mbar_init(bar_pvfull + 8 * g, 1);
       mbar_init(bar_sfree + 8 * g, kGroupWarps * 32);
     }
+    if (kKv4)
+      for (int g = 0; g < 4; ++g) nan_pos[g] = INT_MAX;
     fence_barrier_init();
   }
   if (warp == kMmaWarp) {  // TMEM allocation is a warp-wide operation
@@ -316,6 +342,13 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
   // phases simply keep counting across the CTA's query tiles.
   auto pos_k = [](int base, int t) { return base + (t == 0 ? 0 : 2 * t - 1); };
   auto pos_v = [](int base, int T, int t) { return base + (t == T - 1 ? 2 * T - 1 : 2 * t + 2); };
+  // Item n of a query tile in that order: which key tile, and K or V.
+  auto item_tile = [](int n, int n_tiles, bool& is_v) {
+    if (n == 0) { is_v = false; return 0; }
+    if (n == 2 * n_tiles - 1) { is_v = true; return n_tiles - 1; }
+    is_v = (n & 1) == 0;
+    return is_v ? (n - 2) / 2 : (n + 1) / 2;
+  };
   cudaGridDependencySynchronize();  // q and the pool belong to earlier kernels until here
   cudaTriggerProgrammaticLaunchCompletion();
 
@@ -326,8 +359,10 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     const uint64_t policy = l2_evict_first_policy();
     if (lane == 0) {
       prefetch_tensormap(&qmap);
-      prefetch_tensormap(&kmap);
-      prefetch_tensormap(&vmap);
+      if (!kKv4) {
+        prefetch_tensormap(&kmap);
+        prefetch_tensormap(&vmap);
+      }
     }
     const int my_page = lane >> 1;   // lanes 0..15: page of the tile
     const int my_half = lane & 1;    // low / high half of head_dim
@@ -355,25 +390,19 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
           tma_load_3d(sm_q + qh * kQBytes + qhalf * (kQBytes / 2) + qg * (kQBoxRows * 128), &qmap, bar_q,
                       qhalf * 64, head0 + qh, static_cast<int>(wk.q_tok0) + qg * kQBoxRows, policy);
       }
+      if (kKv4) continue;   // K and V are the converter warps' business
       // Raw table entry of this lane's page of a tile (0 when the page does not exist).
       auto fetch_id = [&](int j) -> int32_t {
         const int64_t lp = static_cast<int64_t>(j) * kTilePages + my_page;
         if (lane >= 16 || j >= n_tiles || lp >= n_pages || p.table_kind == B200KV_TABLE_DENSE) return 0;
         return __ldg(trow + (p.table_kind == B200KV_TABLE_BLOCK ? lp : lp * kPS));
       };
-      // Item n of the ring order above: which tile, and K or V.
-      auto item_tile = [n_tiles](int n, bool& is_v) {
-        if (n == 0) { is_v = false; return 0; }
-        if (n == 2 * n_tiles - 1) { is_v = true; return n_tiles - 1; }
-        is_v = (n & 1) == 0;
-        return is_v ? (n - 2) / 2 : (n + 1) / 2;
-      };
       bool v_cur;
-      int t_cur = item_tile(0, v_cur);
+      int t_cur = item_tile(0, n_tiles, v_cur);
       int32_t id_cur = fetch_id(t_cur);
       for (int nl = 0; ok && nl < 2 * n_tiles; ++nl) {
         bool v_next = false;
-        const int t_next = nl + 1 < 2 * n_tiles ? item_tile(nl + 1, v_next) : n_tiles;
+        const int t_next = nl + 1 < 2 * n_tiles ? item_tile(nl + 1, n_tiles, v_next) : n_tiles;
         const int32_t id_next = fetch_id(t_next);   // in flight while this item is issued
         const int64_t page0 = static_cast<int64_t>(t_cur) * kTilePages;
         const int np = static_cast<int>(n_pages - page0 < kTilePages ? n_pages - page0 : kTilePages);
@@ -508,6 +537,119 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
         item_base += 2 * n_tiles;
       }
       if (!ok) set_status(p.status, B200KV_DEV_WAIT_TIMEOUT);
+    }
+  } else if (kKv4 && warp > kMmaWarp) {
+    // ============================== 4-bit converters ========================================
+    // Lane = (token row of a page, chunk of its codes): warp 0 takes rows 0..7 of every page, warp 1
+    // rows 8..15; four lanes read a row's 64 bytes of codes and, all four, its 8 bytes of scales.  The
+    // four words of a chunk are the elements 32 g + 8 j .. + 7, one 16-byte piece of the tile each.
+    const int tp = (warp - kMmaWarp - 1) * 8 + (lane >> 2);
+    const int j = lane & 3;
+    const uint8_t* my_rows = p.pool + static_cast<int64_t>(kv_head) * kv4::kBlockBytes;
+    const int64_t v_from_k = static_cast<int64_t>(p.kv_heads) * kv4::kBlockBytes;
+    const int code_off = kv4::chunk_offset(tp, j);
+    const int scale_off = kv4::kScaleOffset + tp * kv4::kScaleBytes;
+    const int32_t* trow = p.table + static_cast<int64_t>(table_row) * p.table_row_stride;
+    const uint32_t dst_row = sm_ring + tp * 128;
+    const uint32_t piece0 = static_cast<uint32_t>((j ^ (tp & 7)) << 4), piece1 = static_cast<uint32_t>(((4 + j) ^ (tp & 7)) << 4);
+    // One ring item: the K or V rows of a key tile.  Lane i < 8 holds the table entry of its page i.
+    struct Item {
+      int w, nl, tile, np;
+      bool is_v, valid;
+      int32_t ids;
+    };
+    auto open_item = [&](int w, int nl) {
+      Item it;
+      const int nt = (w ? work1 : work0).n_tiles;
+      if (nl == 2 * nt) {
+        nl = 0;
+        ++w;
+      }
+      it.w = w;
+      it.nl = nl;
+      it.valid = w < n_work;
+      it.tile = 0;
+      it.np = 0;
+      it.is_v = false;
+      it.ids = 0;
+      if (it.valid) {
+        const Work& wk = w ? work1 : work0;
+        it.tile = item_tile(nl, wk.n_tiles, it.is_v);
+        const int64_t page0 = static_cast<int64_t>(it.tile) * kTilePages;
+        it.np = static_cast<int>(wk.n_pages - page0 < kTilePages ? wk.n_pages - page0 : kTilePages);
+        if (lane < it.np) it.ids = __ldg(trow + (p.table_kind == B200KV_TABLE_BLOCK ? page0 + lane : (page0 + lane) * kPS));
+      }
+      return it;
+    };
+    constexpr int kAhead = 4;     // pages in flight
+    uint4 codes[kAhead];
+    uint2 scales[kAhead];
+    auto load_page = [&](int slot, const Item& it, int i) {   // page i < it.np of the item
+      const int32_t id = __shfl_sync(0xffffffffu, it.ids, i);
+      int64_t page = id;
+      bool ok = true;
+      if (p.table_kind == B200KV_TABLE_TOKEN) {
+        ok = (id & (kPS - 1)) == 0;
+        page = id >> 4;
+      }
+      if (!ok || page < 0 || page >= p.pool_pages) {
+        set_status(p.status, B200KV_DEV_BAD_PAGE);
+        page = 0;  // never dereference a bad entry: report it and read page 0 instead
+      }
+      const uint8_t* block = my_rows + page * p.page_stride + (it.is_v ? v_from_k : 0);
+      codes[slot] = __ldg(reinterpret_cast<const uint4*>(block + code_off));
+      scales[slot] = __ldg(reinterpret_cast<const uint2*>(block + scale_off));
+    };
+    Item cur = open_item(0, 0);
+    Item nxt = open_item(cur.w, cur.nl + 1);
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i)
+      if (i < cur.np) load_page(i, cur, i);
+    for (int n = 0;; ++n) {
+      const int sl = n % kSlots;
+      if (n >= kSlots && !mbar_wait_bounded(bar_empty + 8 * sl, ((n / kSlots) - 1) & 1)) {
+        set_status(p.status, B200KV_DEV_WAIT_TIMEOUT);
+        break;
+      }
+#pragma unroll
+      for (int i = 0; i < kTilePages; ++i) {
+        const int slot = i % kAhead;
+        if (i < cur.np) {
+          const uint32_t w[4] = {codes[slot].x, codes[slot].y, codes[slot].z, codes[slot].w};
+          uint32_t s2[4] = {__byte_perm(scales[slot].x, 0, 0x1010), __byte_perm(scales[slot].x, 0, 0x3232),
+                            __byte_perm(scales[slot].y, 0, 0x1010), __byte_perm(scales[slot].y, 0, 0x3232)};
+          if (cur.is_v) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              if ((s2[g] & 0x7fffu) >= 0x7c00u) {
+                s2[g] = 0;
+                atomicMin(nan_pos + g, cur.tile * kBN + i * kPS + tp);
+              }
+            }
+          }
+          const uint32_t dst = dst_row + sl * kTileBytes + i * kHalfPage;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            uint32_t v[4];
+            kv4::unpack_word(w[g], v);
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (g >> 1) * (kTileBytes / 2) +
+                                                                          ((g & 1) ? piece1 : piece0)),
+                         "r"(kv4::h2_mul(v[0], s2[g])), "r"(kv4::h2_mul(v[1], s2[g])), "r"(kv4::h2_mul(v[2], s2[g])),
+                         "r"(kv4::h2_mul(v[3], s2[g]))
+                         : "memory");
+          }
+        }
+        if (i < kTilePages - kAhead) {
+          if (i + kAhead < cur.np) load_page(slot, cur, i + kAhead);
+        } else if (i - (kTilePages - kAhead) < nxt.np) {
+          load_page(slot, nxt, i - (kTilePages - kAhead));
+        }
+      }
+      fence_proxy_async_smem();   // the tile is visible to the tensor core
+      mbar_arrive(bar_full + 8 * sl);
+      if (!nxt.valid) break;
+      cur = nxt;
+      nxt = open_item(cur.w, cur.nl + 1);
     }
   } else {
     // ============================== softmax warps ===========================================
@@ -688,6 +830,7 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
           asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
                        : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                        : "r"(my_p + r * 256 + ((c ^ (r & 15)) << 4)));
+          if (kKv4 && ctx + row0 + r >= nan_pos[c >> 2]) v = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
           *reinterpret_cast<uint4*>(obase + static_cast<int64_t>(r) * p.out_stride_t + c * 8) = v;
         }
       }
@@ -718,14 +861,16 @@ int encode_q_tensor_map(CUtensorMap* out, const void* q, int64_t total_q, int64_
   return cached_kv_tensor_map(out, q, total_q, stride_t, stride_h, heads, kD, kQBoxRows);
 }
 
-}  // namespace
-
-int paged_prefill(const PrefillArgs& a, cudaStream_t stream) {
+// Checks that do not depend on where K and V come from; B200KV_OK with *nothing set when there is no work.
+int check_prefill(const PrefillArgs& a, bool* nothing) {
+  *nothing = false;
   if (a.batch < 0 || a.total_q < 0 || a.max_q_len < 0 || a.q_heads <= 0 || a.kv_heads <= 0)
     return B200KV_EINVAL;
-  if (a.batch == 0 || a.total_q == 0 || a.max_q_len == 0) return B200KV_OK;
-  if (!a.q || !a.k_base || !a.v_base || !a.q_start || !a.ctx_lens || !a.q_lens || !a.out)
-    return B200KV_EINVAL;
+  if (a.batch == 0 || a.total_q == 0 || a.max_q_len == 0) {
+    *nothing = true;
+    return B200KV_OK;
+  }
+  if (!a.q || !a.q_start || !a.ctx_lens || !a.q_lens || !a.out) return B200KV_EINVAL;
   if (a.table_kind != B200KV_TABLE_BLOCK && a.table_kind != B200KV_TABLE_TOKEN &&
       a.table_kind != B200KV_TABLE_DENSE)
     return B200KV_EINVAL;
@@ -736,21 +881,14 @@ int paged_prefill(const PrefillArgs& a, cudaStream_t stream) {
   if (a.head_dim != kD || a.page_size != kPS) return B200KV_EUNSUPPORTED;
   if (a.q_heads % a.kv_heads != 0) return B200KV_EUNSUPPORTED;
   if (a.batch > 65535 || a.q_heads > 65535 * 16) return B200KV_ETOOLARGE;
-  if (a.pool_tokens <= 0 || a.pool_tokens > (int64_t{1} << 31) - 1 || a.total_q > (int64_t{1} << 31) - 1)
-    return B200KV_ETOOLARGE;
+  if (a.total_q > (int64_t{1} << 31) - 1) return B200KV_ETOOLARGE;
   if ((reinterpret_cast<uintptr_t>(a.out) & 15u) != 0 || a.out_stride_t % 8 != 0 || a.out_stride_h % 8 != 0)
     return B200KV_EALIGN;
+  if ((a.max_q_len + kBM - 1) / kBM > 2 * 65535) return B200KV_ETOOLARGE;
+  return B200KV_OK;
+}
 
-  CUtensorMap qmap, kmap, vmap;
-  int rc = encode_q_tensor_map(&qmap, a.q, a.total_q, a.q_stride_t, a.q_stride_h, a.q_heads);
-  if (rc != B200KV_OK) return rc;
-  rc = cached_kv_tensor_map(&kmap, a.k_base, a.pool_tokens, a.kv_tok_stride, a.kv_head_stride,
-                            a.kv_heads, kD, kPS);
-  if (rc != B200KV_OK) return rc;
-  rc = cached_kv_tensor_map(&vmap, a.v_base, a.pool_tokens, a.kv_tok_stride, a.kv_head_stride,
-                            a.kv_heads, kD, kPS);
-  if (rc != B200KV_OK) return rc;
-
+PrefillParams common_params(const PrefillArgs& a) {
   PrefillParams p{};
   p.table = a.table;
   p.table_row_stride = a.table_row_stride;
@@ -774,13 +912,18 @@ int paged_prefill(const PrefillArgs& a, cudaStream_t stream) {
   p.out_stride_h = a.out_stride_h;
   p.status = a.status;
   p.tiles_m = static_cast<int>((a.max_q_len + kBM - 1) / kBM);
-  if (p.tiles_m > 2 * 65535) return B200KV_ETOOLARGE;
+  p.kv_heads = a.kv_heads;
+  return p;
+}
 
+template <bool kKv4>
+int launch_prefill(const PrefillParams& p, const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                   cudaStream_t stream) {
   static bool attr_done[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return record_cuda_error(cudaGetLastError());
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<kKv4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kSmemBytes);
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
@@ -790,16 +933,54 @@ int paged_prefill(const PrefillArgs& a, cudaStream_t stream) {
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
   // x: (KV head, pair of query heads of its group), adjacent so a group's CTAs share K/V in L2.
-  cfg.gridDim = dim3(static_cast<unsigned>(a.kv_heads * ((p.group + 1) / 2)),
-                     static_cast<unsigned>((p.tiles_m + 1) / 2), static_cast<unsigned>(a.batch));
-  cfg.blockDim = dim3(kThreads);
+  cfg.gridDim = dim3(static_cast<unsigned>(p.kv_heads * ((p.group + 1) / 2)),
+                     static_cast<unsigned>((p.tiles_m + 1) / 2), static_cast<unsigned>(p.batch));
+  cfg.blockDim = dim3(threads_of(kKv4));
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prefill_kernel, p, qmap, kmap, vmap);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<kKv4>, p, qmap, kmap, vmap);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
+}
+
+}  // namespace
+
+int paged_prefill(const PrefillArgs& a, cudaStream_t stream) {
+  bool nothing = false;
+  int rc = check_prefill(a, &nothing);
+  if (rc != B200KV_OK || nothing) return rc;
+  if (!a.k_base || !a.v_base) return B200KV_EINVAL;
+  if (a.pool_tokens <= 0 || a.pool_tokens > (int64_t{1} << 31) - 1) return B200KV_ETOOLARGE;
+  CUtensorMap qmap, kmap, vmap;
+  rc = encode_q_tensor_map(&qmap, a.q, a.total_q, a.q_stride_t, a.q_stride_h, a.q_heads);
+  if (rc != B200KV_OK) return rc;
+  rc = cached_kv_tensor_map(&kmap, a.k_base, a.pool_tokens, a.kv_tok_stride, a.kv_head_stride,
+                            a.kv_heads, kD, kPS);
+  if (rc != B200KV_OK) return rc;
+  rc = cached_kv_tensor_map(&vmap, a.v_base, a.pool_tokens, a.kv_tok_stride, a.kv_head_stride,
+                            a.kv_heads, kD, kPS);
+  if (rc != B200KV_OK) return rc;
+  return launch_prefill<false>(common_params(a), qmap, kmap, vmap, stream);
+}
+
+int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
+  const PrefillArgs& a = k.args;
+  bool nothing = false;
+  int rc = check_prefill(a, &nothing);
+  if (rc != B200KV_OK || nothing) return rc;
+  if (a.table_kind == B200KV_TABLE_DENSE) return B200KV_EINVAL;
+  rc = kv4_check_pool(k.pool, k.pool_pages, k.page_stride_bytes, a.kv_heads);
+  if (rc != B200KV_OK) return rc;
+  CUtensorMap qmap;
+  rc = encode_q_tensor_map(&qmap, a.q, a.total_q, a.q_stride_t, a.q_stride_h, a.q_heads);
+  if (rc != B200KV_OK) return rc;
+  PrefillParams p = common_params(a);
+  p.pool = static_cast<const uint8_t*>(k.pool);
+  p.pool_pages = k.pool_pages;
+  p.page_stride = k.page_stride_bytes;
+  return launch_prefill<true>(p, qmap, qmap, qmap, stream);
 }
 
 }  // namespace b200kv
