@@ -13,36 +13,42 @@
 // logical operation and one packed add per pair, a shift per word) on its way to mma.sync m16n8k16
 // (fp16 in, fp32 accumulate; tokens or head_dim are the M rows, the query heads the N columns).
 //
-// P * s_V is an fp16 operand, so its range matters: P is at most 2^8 (the running maximum is moved only
-// when it has grown by more than that) and s_V is multiplied by 2^a with the largest scale seen so far
-// below 2^(6 - a), a <= 15; products are at most 2^14 and lose bits only below 2^-14, 2^28 under the
-// largest.  A new largest scale rescales O, as a new maximum does.
+// P * s_V is an fp16 operand, so its range matters.  P = 2^(score - m) with a reference m that is kept
+// about 2^7 under the running maximum (it cancels between O and the sum of P): P is at most 2^14 and
+// P * s_V at most 2^15, and m is moved, and O rescaled, only when a score or a V scale would
+// exceed that.  V scales of 2 and more (values of 14 and more) lower the bound on P accordingly.  A
+// product loses bits only below 2^-14, i.e. where it is 2^-21 of the largest weight times one scale unit;
+// the absolute error of such a token, 2^-25 * 2^-7 * 8 per code, is far under half a step of the output.
 //
-// A warp streams its own pages: page k of a piece belongs to warp k % 4, and every warp keeps a ring of
-// kStages pages (K block + V block, 2304 bytes) filled by two bulk copies per page that its lane 0
-// issues as soon as the page's ring slot has been read.  No producer warp, no CTA-wide barrier in the
-// steady state; the blocks are stored in the order in which the lanes read them (conflict-free 16-byte
-// shared loads).  The page table is read 32 entries at a time, one block of entries ahead of use.
-// Every wait is an mbarrier wait bounded by ~2 s.
+// A warp streams its own pages: page k of a piece belongs to warp k % 4, two of them make up one step
+// (one wait, one look at the maxima, one request, and twice the independent arithmetic in flight).  Every
+// warp keeps a ring of kStages page pairs (2 x (K block + V block), 4608 bytes) that its own lanes fill with
+// 16-byte asynchronous copies, nine per lane and pair, as soon as the slot has been read (bulk copies by
+// one lane cost three times the instructions here: their operands are uniform registers).  No producer
+// warp, no barrier in the steady state; the blocks are stored in the order in which the lanes read
+// them (conflict-free 16-byte shared loads).  The page table is read 32 entries at a time, one block of
+// entries ahead of use.
 //
 // Bytes per token and KV head: 2 * 72 (a page is 2304 B where fp16 has 8192).
 #include "common.cuh"
 #include "decode_plan.cuh"
 #include "kv4.cuh"
 #include "launch.h"
-#include "tma.h"
 
 namespace b200kv {
 
 namespace {
 
 constexpr int kThreads = kConsumerThreads;
-constexpr int kStages = 4;
+constexpr int kStages = 2;
 constexpr int kPageBytes = 2 * kv4::kBlockBytes;   // K and V block of one page of one head
-constexpr int kRingBytes = kConsumerWarps * kStages * kPageBytes;
+constexpr int kPairBytes = 2 * kPageBytes;
+constexpr int kRingBytes = kConsumerWarps * kStages * kPairBytes;
+// Resident CTAs per SM.  Three of them leave 168 registers, which a step of two pages needs (four spill
+// and were slower: 36.4 against 33.0 us on 32 sequences of 1-4 k tokens, 64/8 heads).
+constexpr int ctas_per_sm(int rows) { return rows == 8 ? 3 : 2; }
 constexpr int kSeqCache = kThreads;                // lengths and table rows kept in shared memory
-constexpr int kDefaultPieceCost = 8;
-constexpr int kMaxTeams = kConsumerWarps * kD;     // a sequence's weights must fit the merge buffer
+constexpr int kDefaultPieceCost = 16;
 static_assert(kPS == kv4::kPageTok && kD == kv4::kHeadDim, "one geometry");
 
 struct Kv4DecodeParams : DecodePlan {
@@ -56,42 +62,31 @@ struct Kv4DecodeParams : DecodePlan {
   float scale_log2;
 };
 
-__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar, uint64_t policy) {
-  asm volatile(
-      "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1], %2, [%3], %4;\n"
-      :
-      : "r"(dst), "l"(src), "r"(bytes), "r"(bar), "l"(policy)
-      : "memory");
+__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src, uint64_t policy) {
+  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;\n" : : "r"(dst), "l"(src), "l"(policy) : "memory");
+}
+__device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;\n" : : : "memory"); }
+template <int N>
+__device__ __forceinline__ void async_wait() {
+  asm volatile("cp.async.wait_group %0;\n" : : "n"(N) : "memory");
 }
 __device__ __forceinline__ void bulk_prefetch_l2(const void* src, uint32_t bytes) {
   asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;\n" : : "l"(src), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
-  return v;
-}
-__device__ __forceinline__ uint2 lds64(uint32_t addr) {
-  uint2 v;
-  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(v.x), "=r"(v.y) : "r"(addr));
-  return v;
-}
-// D = A * B (no accumulator input)
-__device__ __forceinline__ void mma_16816_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+// The tensor instructions are pure functions of registers: not volatile, so that the compiler may
+// interleave the two pages of a step.  D = A * B + C.
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                    uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};\n"
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t a) {
   uint32_t d;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(d) : "r"(a));
   return d;
 }
-__device__ __forceinline__ float half_bits_to_float(uint32_t bits) {
-  return __half2float(__ushort_as_half(static_cast<unsigned short>(bits & 0xffffu)));
-}
+__device__ __forceinline__ float2 h2_to_f2(uint32_t h2) { return __half22float2(*reinterpret_cast<const __half2*>(&h2)); }
 __device__ __forceinline__ uint32_t h2_max(uint32_t a, uint32_t b) {
   uint32_t d;
   asm("max.f16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
@@ -146,14 +141,28 @@ __device__ __forceinline__ int warp_pages(const Piece& pc, int warp) {
   return pc.valid ? (pc.end - pc.begin - warp + kConsumerWarps - 1) / kConsumerWarps : 0;
 }
 
-// The pages a warp requests, in order, with their table entries: lane l holds the entry of page
-// begin + warp + 4 * (32 * block + l) of the piece; the next block of entries (of this piece, or
+// The pages a warp requests, in order and two at a time: lane l holds the number of page
+// begin + warp + 4 * (32 * block + l) of the piece; the next block of table entries (of this piece, or
 // the first of the next piece) is already on its way.
 struct PageStream {
   Piece pc, nx;
   int m, cnt;            // next page of this warp in pc, and how many it has there
-  int32_t ids, ids_next;
+  int32_t ids, ids_next; // page numbers in use; raw table entries of the next block
 
+  // Raw table entry -> page number; an entry that names no page is reported and page 0 read instead.
+  __device__ __forceinline__ static int32_t checked(const Kv4DecodeParams& p, int32_t id) {
+    int32_t page = id;
+    bool ok = true;
+    if (p.table_kind == B200KV_TABLE_TOKEN) {
+      ok = (id & (kPS - 1)) == 0;
+      page = id >> 4;
+    }
+    if (!ok || page < 0 || page >= p.pool_pages) {
+      set_status(p.status, B200KV_DEV_BAD_PAGE);
+      page = 0;
+    }
+    return page;
+  }
   __device__ __forceinline__ int32_t load_ids(const Kv4DecodeParams& p, const Piece& from, int warp, int lane, int first) const {
     const int page = from.begin + warp + kConsumerWarps * (first + lane);
     if (!from.valid || page >= from.end) return 0;
@@ -177,35 +186,285 @@ struct PageStream {
     while (pc.valid && warp_pages(pc, warp) <= 0) next_piece(p, seq, range_end, pc);
     m = 0;
     cnt = warp_pages(pc, warp);
-    ids = load_ids(p, pc, warp, lane, 0);
+    ids = checked(p, load_ids(p, pc, warp, lane, 0));
     if (pc.valid) refill(p, seq, range_end, warp, lane);
   }
   __device__ __forceinline__ bool more() const { return pc.valid; }
   __device__ __forceinline__ void advance(const Kv4DecodeParams& p, const SeqCache& seq, int64_t range_end, int warp, int lane) {
-    ++m;
-    if (m == cnt) {
+    m += 2;
+    const bool done = m >= cnt;
+    if (!done && (m & 31) != 0) return;
+    if (done) {
       pc = nx;
       m = 0;
       cnt = warp_pages(pc, warp);
-      ids = ids_next;
-      if (pc.valid) refill(p, seq, range_end, warp, lane);
-    } else if ((m & 31) == 0) {
-      ids = ids_next;
-      refill(p, seq, range_end, warp, lane);
     }
+    ids = checked(p, ids_next);
+    if (pc.valid) refill(p, seq, range_end, warp, lane);
   }
 };
 
+// S^T of 16 tokens: k_at and c_at are this lane's chunk of token r and that token's scales.
+template <int NB>
+__device__ __forceinline__ void page_scores(const uint8_t* k_at, const uint8_t* c_at, const uint32_t (&qf)[NB][8][2],
+                                            float scale, float (&s)[NB][4]) {
+  const uint4 k0 = *reinterpret_cast<const uint4*>(k_at), k1 = *reinterpret_cast<const uint4*>(k_at + 8 * kv4::kRowBytes);
+  const uint2 c0 = *reinterpret_cast<const uint2*>(c_at), c1 = *reinterpret_cast<const uint2*>(c_at + 8 * kv4::kScaleBytes);
+  const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+  const float2 f0a = h2_to_f2(c0.x), f0b = h2_to_f2(c0.y), f1a = h2_to_f2(c1.x), f1b = h2_to_f2(c1.y);
+  const float f0[4] = {f0a.x, f0a.y, f0b.x, f0b.y}, f1[4] = {f1a.x, f1a.y, f1b.x, f1b.y};
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t a[4], b[4];
+    kv4::unpack_word(w0[g], a);
+    kv4::unpack_word(w1[g], b);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float d[4];
+      mma(d, a[0], b[0], a[1], b[1], qf[nb][2 * g][0], qf[nb][2 * g][1], 0.f, 0.f, 0.f, 0.f);
+      mma(d, a[2], b[2], a[3], b[3], qf[nb][2 * g + 1][0], qf[nb][2 * g + 1][1], d[0], d[1], d[2], d[3]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float f = i < 2 ? f0[g] : f1[g];
+        s[nb][i] = g == 0 ? f * d[i] : s[nb][i] + f * d[i];
+      }
+    }
+  }
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s[nb][i] *= scale;
+}
+
+// V scales of tokens 2jq, 2jq+1 | 2jq+8, 2jq+9 as fp16 pairs per group.
+__device__ __forceinline__ void page_v_scales(const uint8_t* at, uint32_t (&sv)[4][2]) {
+  const uint4 t0 = *reinterpret_cast<const uint4*>(at), t1 = *reinterpret_cast<const uint4*>(at + 8 * kv4::kScaleBytes);
+  sv[0][0] = __byte_perm(t0.x, t0.z, 0x5410);
+  sv[1][0] = __byte_perm(t0.x, t0.z, 0x7632);
+  sv[2][0] = __byte_perm(t0.y, t0.w, 0x5410);
+  sv[3][0] = __byte_perm(t0.y, t0.w, 0x7632);
+  sv[0][1] = __byte_perm(t1.x, t1.z, 0x5410);
+  sv[1][1] = __byte_perm(t1.x, t1.z, 0x7632);
+  sv[2][1] = __byte_perm(t1.y, t1.w, 0x5410);
+  sv[3][1] = __byte_perm(t1.y, t1.w, 0x7632);
+}
+
+// O^T += V^T (P^T s_V) of 16 tokens.
+template <int NB>
+__device__ __forceinline__ void page_pv(const uint8_t* v_at, uint32_t vsel, const uint32_t (&sv)[4][2],
+                                        const uint32_t (&pb)[NB][2], float (&o)[8][NB][4]) {
+  const uint4 v0 = *reinterpret_cast<const uint4*>(v_at), v1 = *reinterpret_cast<const uint4*>(v_at + kv4::kRowBytes);
+  const uint4 v2 = *reinterpret_cast<const uint4*>(v_at + 8 * kv4::kRowBytes);
+  const uint4 v3 = *reinterpret_cast<const uint4*>(v_at + 9 * kv4::kRowBytes);
+  const uint32_t x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
+  const uint32_t x2[4] = {v2.x, v2.y, v2.z, v2.w}, x3[4] = {v3.x, v3.y, v3.z, v3.w};
+#pragma unroll
+  for (int g = 0; g < 4; ++g) {
+    uint32_t a[4], b[4];
+    kv4::unpack_word(__byte_perm(x0[g], x1[g], vsel), a);
+    kv4::unpack_word(__byte_perm(x2[g], x3[g], vsel), b);
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      const uint32_t q0 = kv4::h2_mul(pb[nb][0], sv[g][0]), q1 = kv4::h2_mul(pb[nb][1], sv[g][1]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float(&acc)[4] = o[2 * g + e][nb];
+        mma(acc, a[2 * e], a[2 * e + 1], b[2 * e], b[2 * e + 1], q0, q1, acc[0], acc[1], acc[2], acc[3]);
+      }
+    }
+  }
+}
+
+// Column sums of what `n` contributors hold, in the order of the O^T fragments: a thread takes 16-byte
+// pieces (M block j, lane) with the head columns 2 jq and 2 jq + 1 of N block nb.
+struct Weighted {
+  float m[2], l[2];
+  float acc[4];
+  __device__ __forceinline__ void add(const float4& v, float w0, float w1) {
+    acc[0] += w0 * v.x;
+    acc[1] += w1 * v.y;
+    acc[2] += w0 * v.z;
+    acc[3] += w1 * v.w;
+  }
+};
+
+__device__ __forceinline__ unsigned atomic_inc_acq_rel(unsigned* ctr, unsigned limit) {
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;\n" : "=r"(old) : "l"(ctr), "r"(limit) : "memory");
+  return old;
+}
+
+// The end of a piece.  The four warps put their O^T fragments, as they are, and their (m, l) into shared
+// memory; every thread then combines 2 * NB of the 16-byte pieces over the warps and writes the final
+// rows (whole sequence) or the partial, in the same fragment order (16-byte accesses without bank
+// conflicts or strides all the way).  A partial is published by one release-acquire count on the
+// (sequence, head) counter, which wraps to zero on the last arrival; the CTA that arrives last
+// combines the partials of all pieces the same way.
 template <int ROWS>
-__global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : 3) kv4_decode_kernel(Kv4DecodeParams p) {
+__device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Piece& pc, bool whole, int team, int head, int tid,
+                                             const float (&o)[8][ROWS / 8][4], const float (&m_ref)[ROWS / 8][2],
+                                             const float (&l_run)[ROWS / 8][2], float4* merge_o, float2* merge_ml,
+                                             int* note) {
+  constexpr int NB = ROWS / 8;
+  constexpr int kParts = 8 * NB;               // fragments of a warp
+  const int lane = tid & 31, warp = tid >> 5;
+  const int r = lane >> 2, jq = lane & 3;
+  consumer_bar();   // the previous piece's merge has read the buffers
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      merge_o[(warp * kParts + nb * 8 + j) * 32 + lane] = make_float4(o[j][nb][0], o[j][nb][1], o[j][nb][2], o[j][nb][3]);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float l = l_run[nb][h];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      if (r == 0) merge_ml[warp * ROWS + nb * 8 + 2 * jq + h] = make_float2(m_ref[nb][h], l);
+    }
+  }
+  consumer_bar();
+  // O / l of one fragment (M block j = 2 g + e: elements d0 and d0 + 2, heads 2 jq, 2 jq + 1) -> out
+  auto write_out = [&](int nb, int j, const Weighted& w) {
+    const int d0 = 32 * (j >> 1) + 8 * (r >> 1) + 4 * (j & 1) + (r & 1);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int hq = nb * 8 + 2 * jq + h;
+      if (hq < p.group) {
+        __half* dst = p.out + static_cast<int64_t>(pc.b) * p.out_stride_b +
+                      (static_cast<int64_t>(head) * p.group + hq) * p.out_stride_h + d0;
+        dst[0] = __float2half_rn(w.acc[h] / w.l[h]);
+        dst[2] = __float2half_rn(w.acc[h + 2] / w.l[h]);
+      }
+    }
+  };
+  const int64_t slot = (static_cast<int64_t>(team) + pc.b) * p.kv_heads + head;
+  float4* part = reinterpret_cast<float4*>(p.part_o) + slot * kParts * 32;
+  float2* part_ml = reinterpret_cast<float2*>(p.part_lse) + slot * ROWS;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    // (m, l) of the four warps for this lane's two heads
+    float2 ml[kConsumerWarps][2];
+    float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int w = 0; w < kConsumerWarps; ++w) {
+      const float4 v = *reinterpret_cast<const float4*>(merge_ml + w * ROWS + nb * 8 + 2 * jq);
+      ml[w][0] = make_float2(v.x, v.y);
+      ml[w][1] = make_float2(v.z, v.w);
+      top[0] = fmaxf(top[0], v.x);
+      top[1] = fmaxf(top[1], v.z);
+    }
+    float wt[kConsumerWarps][2];
+    Weighted sum[2];
+    float l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int w = 0; w < kConsumerWarps; ++w)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        // a warp without a page of this piece, or with only NaN scores: its sums enter as they are
+        wt[w][h] = ml[w][h].x == -INFINITY ? 1.f : fast_exp2(ml[w][h].x - top[h]);
+        l[h] += wt[w][h] * ml[w][h].y;
+      }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const int j = 2 * warp + k;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[k].acc[i] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kConsumerWarps; ++w)
+        sum[k].add(merge_o[(w * kParts + nb * 8 + j) * 32 + lane], wt[w][0], wt[w][1]);
+      if (whole) {
+        sum[k].l[0] = l[0];
+        sum[k].l[1] = l[1];
+        write_out(nb, j, sum[k]);
+      } else {
+        __stcg(part + (nb * 8 + j) * 32 + lane, make_float4(sum[k].acc[0], sum[k].acc[1], sum[k].acc[2], sum[k].acc[3]));
+      }
+    }
+    if (!whole && warp == 0 && r == 0)
+      __stcg(reinterpret_cast<float4*>(part_ml + nb * 8 + 2 * jq), make_float4(top[0], l[0], top[1], l[1]));
+  }
+  if (whole) return;
+  const int first_team = note[1], pieces = note[2];   // thread 0 rewrites both when the next piece begins
+  consumer_bar();   // all of the CTA's partial is written; the count below publishes it
+  if (tid == 0)
+    note[0] = atomic_inc_acq_rel(p.piece_ctr + static_cast<int64_t>(pc.b) * p.kv_heads + head,
+                                 static_cast<unsigned>(pieces - 1)) == static_cast<unsigned>(pieces - 1);
+  consumer_bar();
+  if (note[0] == 0) return;
+  // Last to arrive: the partials of all pieces (this CTA's own among them) lie in neighbouring slots.
+  const int64_t slot0 = (static_cast<int64_t>(first_team) + pc.b) * p.kv_heads + head;
+  const int64_t step = p.kv_heads;
+  constexpr int kBatch = 4;                    // partials in flight
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb) {
+    Weighted sum[2];
+    float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < 2; ++k)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) sum[k].acc[i] = 0.f;
+#pragma unroll 1
+    for (int p0 = 0; p0 < pieces; p0 += kBatch) {
+      float4 ml[kBatch], v[kBatch][2];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (p0 + i < pieces) {
+          const int64_t sl = slot0 + (p0 + i) * step;
+          ml[i] = __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float2*>(p.part_lse) + sl * ROWS + nb * 8 + 2 * jq));
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            v[i][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o) + (sl * kParts + nb * 8 + 2 * warp + k) * 32 + lane);
+        } else {
+          ml[i] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+          v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+      }
+      float was[2] = {top[0], top[1]};
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        top[0] = fmaxf(top[0], ml[i].x);
+        top[1] = fmaxf(top[1], ml[i].z);
+      }
+      float re[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        re[h] = was[h] == -INFINITY ? 1.f : fast_exp2(was[h] - top[h]);
+        l[h] *= re[h];
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sum[k].acc[i] *= re[i & 1];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        const float w0 = ml[i].x == -INFINITY ? 1.f : fast_exp2(ml[i].x - top[0]);
+        const float w1 = ml[i].z == -INFINITY ? 1.f : fast_exp2(ml[i].z - top[1]);
+        l[0] += w0 * ml[i].y;
+        l[1] += w1 * ml[i].w;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) sum[k].add(v[i][k], w0, w1);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      sum[k].l[0] = l[0];
+      sum[k].l[1] = l[1];
+      write_out(nb, 2 * warp + k, sum[k]);
+    }
+  }
+}
+
+template <int ROWS>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel(Kv4DecodeParams p) {
   static_assert(ROWS == 8 || ROWS == 16, "query-group heads are padded to 8 or 16");
   constexpr int NB = ROWS / 8;
   extern __shared__ __align__(128) uint8_t smem[];
-  float* merge_o = reinterpret_cast<float*>(smem + kRingBytes);            // [4][128][ROWS]
-  float* merge_ml = merge_o + kConsumerWarps * kD * ROWS;                  // [4][ROWS][2]
-  uint64_t* bars = reinterpret_cast<uint64_t*>(merge_ml + kConsumerWarps * ROWS * 2);   // [4][kStages]
-  int* arrival = reinterpret_cast<int*>(bars + kConsumerWarps * kStages);
-  int* seq_len_s = arrival + 4;                                            // [kSeqCache]
+  float4* merge_o = reinterpret_cast<float4*>(smem + kRingBytes);          // [4 warps][8 * NB][32 lanes]
+  float2* merge_ml = reinterpret_cast<float2*>(merge_o + kConsumerWarps * 8 * NB * 32);   // [4][ROWS] (m, l)
+  int* note = reinterpret_cast<int*>(merge_ml + kConsumerWarps * ROWS);    // [0] this CTA merges, [1] first team, [2] pieces
+  int* seq_len_s = note + 4;                                               // [kSeqCache]
   int* seq_row_s = seq_len_s + kSeqCache;
   int* scan = reinterpret_cast<int*>(merge_o);
 
@@ -214,12 +473,7 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : 3) kv4_decode_kernel
   const int warp = tid >> 5;
   const int team = blockIdx.x / p.kv_heads;
   const int head = blockIdx.x - team * p.kv_heads;
-  const uint32_t ring = smem_u32(smem) + warp * (kStages * kPageBytes);
-  const uint32_t bar = smem_u32(bars) + warp * (kStages * 8);
-  if (tid == 0) {
-    for (int i = 0; i < kConsumerWarps * kStages; ++i) mbar_init(smem_u32(bars) + 8 * i, 1);
-    fence_barrier_init();
-  }
+  const uint8_t* ring = smem + warp * (kStages * kPairBytes);
   const TeamRange range = plan_team_range(p, team, tid, scan);
   if (range.any) {
     const int b = range.start_b + tid;
@@ -237,26 +491,12 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : 3) kv4_decode_kernel
     enter_piece(p, seq, range.end, pc, range.start_b, range.start_page);
     st.start(p, seq, range.end, pc, warp, lane);
   }
-  // Raw table entry -> page number; an entry that names no page is reported and page 0 read instead.
-  auto page_of = [&](int32_t id) -> int64_t {
-    int64_t page = id;
-    bool ok = true;
-    if (p.table_kind == B200KV_TABLE_TOKEN) {
-      ok = (id & (kPS - 1)) == 0;
-      page = id >> 4;
-    }
-    if (!ok || page < 0 || page >= p.pool_pages) {
-      set_status(p.status, B200KV_DEV_BAD_PAGE);
-      page = 0;
-    }
-    return page;
-  };
   const uint8_t* k_rows = p.pool + static_cast<int64_t>(head) * kv4::kBlockBytes;
   const int64_t v_from_k = static_cast<int64_t>(p.kv_heads) * kv4::kBlockBytes;
   // First pages towards L2 while the previous kernel is still finishing: L2 is the point of coherence,
   // so rows that kernel writes afterwards are still seen by the copies below.
-  if (range.any && st.more() && lane < min(st.cnt, kStages)) {
-    const uint8_t* src = k_rows + page_of(st.ids) * p.page_stride;
+  if (range.any && st.more() && lane < min(st.cnt, 2 * kStages)) {
+    const uint8_t* src = k_rows + st.ids * p.page_stride;
     bulk_prefetch_l2(src, kv4::kBlockBytes);
     bulk_prefetch_l2(src + v_from_k, kv4::kBlockBytes);
   }
@@ -273,35 +513,51 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : 3) kv4_decode_kernel
   if (!range.any) return;
 
   const uint64_t policy = l2_evict_first_policy();
+  // The next two pages into ring slot `stage`: 288 16-byte pieces, piece i * 32 + lane by this lane; 72
+  // pieces are a block, the blocks are K and V of the first page, K and V of the second.
+  const uint32_t ring_dst = smem_u32(ring) + lane * 16;
   auto request = [&](int stage) {
-    const int32_t id = __shfl_sync(0xffffffffu, st.ids, st.m & 31);
-    if (lane == 0) {
-      const uint8_t* src = k_rows + page_of(id) * p.page_stride;
-      const uint32_t dst = ring + stage * kPageBytes;
-      mbar_arrive_expect_tx(bar + 8 * stage, kPageBytes);
-      bulk_load(dst, src, kv4::kBlockBytes, bar + 8 * stage, policy);
-      bulk_load(dst + kv4::kBlockBytes, src + v_from_k, kv4::kBlockBytes, bar + 8 * stage, policy);
+    if (st.more()) {
+      const bool two = st.cnt - st.m >= 2;
+      const int32_t id0 = __shfl_sync(0xffffffffu, st.ids, st.m & 31);
+      const int32_t id1 = __shfl_sync(0xffffffffu, st.ids, (st.m & 31) + 1);
+      const uint8_t* k0 = k_rows + id0 * p.page_stride + lane * 16;
+      const uint8_t* v0 = k0 + v_from_k - kv4::kBlockBytes;
+      const uint8_t* k1 = k_rows + id1 * p.page_stride + lane * 16 - 2 * kv4::kBlockBytes;
+      const uint8_t* v1 = k1 + v_from_k - kv4::kBlockBytes;
+      const uint32_t dst = ring_dst + stage * kPairBytes;
+      async_copy16(dst, k0, policy);
+      async_copy16(dst + 512, k0 + 512, policy);
+      async_copy16(dst + 1024, (lane < 8 ? k0 : v0) + 1024, policy);
+      async_copy16(dst + 1536, v0 + 1536, policy);
+      if (two || lane < 16) async_copy16(dst + 2048, (lane < 16 ? v0 : k1) + 2048, policy);
+      if (two) {
+        async_copy16(dst + 2560, k1 + 2560, policy);
+        async_copy16(dst + 3072, (lane < 24 ? k1 : v1) + 3072, policy);
+        async_copy16(dst + 3584, v1 + 3584, policy);
+        async_copy16(dst + 4096, v1 + 4096, policy);
+      }
+      st.advance(p, seq, range.end, warp, lane);
     }
-    st.advance(p, seq, range.end, warp, lane);
+    async_commit();   // an empty group too: the wait below counts groups
   };
-  int pending = 0;             // pages requested and not yet waited for
-  for (int s = 0; s < kStages && st.more(); ++s, ++pending) request(s);
+  for (int s = 0; s < kStages; ++s) request(s);
 
   const int r = lane >> 2;     // fragment row: token (S^T) or one of the 8 row pairs of head_dim (O^T); also a head column
   const int jq = lane & 3;     // fragment column pair
   const int jv = r >> 1;       // V: chunk of the token rows that holds this lane's elements ...
   const uint32_t vsel = (r & 1) ? 0x7632u : 0x5410u;   // ... and which half of its words
-  const uint32_t k_off = static_cast<uint32_t>(kv4::chunk_offset(r, jq));      // token r; token r + 8 is 512 bytes on
-  const uint32_t v_off = static_cast<uint32_t>(kv4::chunk_offset(2 * jq, jv)); // token 2 jq; 2 jq + 1 is 64 bytes on
-  bool alive = true;           // false once a wait of this warp ran out: keep walking, stop computing
-  unsigned seen_arrivals = 0;
+  // this lane's places in a pair: K chunk and scales of token r, V chunk and scales of token 2 jq
+  const uint8_t* k_at = ring + kv4::chunk_offset(r, jq);
+  const uint8_t* kc_at = ring + kv4::kScaleOffset + r * kv4::kScaleBytes;
+  const uint8_t* v_at = ring + kv4::kBlockBytes + kv4::chunk_offset(2 * jq, jv);
+  const uint8_t* vc_at = ring + kv4::kBlockBytes + kv4::kScaleOffset + 2 * jq * kv4::kScaleBytes;
   int stage = 0;
-  uint32_t parity = 0;
 
   while (pc.valid) {
     uint32_t qf[NB][8][2];     // Q^T as B fragments
-    float o[8][NB][4];         // O^T * 2^a: 8 M blocks of 16 along head_dim
-    float m_run[NB][2], l_run[NB][2];
+    float o[8][NB][4];         // O^T: 8 M blocks of 16 along head_dim
+    float m_ref[NB][2], l_run[NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
       const int hq = nb * 8 + r;
@@ -315,242 +571,145 @@ __global__ void __launch_bounds__(kThreads, ROWS == 8 ? 4 : 3) kv4_decode_kernel
         qf[nb][2 * g + 1][0] = v.z;
         qf[nb][2 * g + 1][1] = v.w;
       }
-      m_run[nb][0] = m_run[nb][1] = -INFINITY;
+      m_ref[nb][0] = m_ref[nb][1] = -INFINITY;
       l_run[nb][0] = l_run[nb][1] = 0.f;
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) o[j][nb][0] = o[j][nb][1] = o[j][nb][2] = o[j][nb][3] = 0.f;
-    int shift = 15;            // a: V scales are multiplied by 2^a
+    float p_room = 14.f;       // log2 of the largest P allowed: P * (largest V scale) stays under 2^15
+    uint32_t sv_lim = 0x4000u; // V scales seen are below this fp16 number (2 to begin with)
     const bool whole = pc.begin == 0 && pc.end == pc.np;
     const int cnt = warp_pages(pc, warp);
+    if (tid == 0 && !whole) {   // the teams that hold a piece of this sequence; read at the end of the piece
+      const int64_t u0 = (pc.flat - pc.begin) + static_cast<int64_t>(p.piece_cost) * (pc.kseq + 1);
+      note[1] = team_of(u0, range.nteams_eff, range.units_total);
+      note[2] = team_of(u0 + pc.np - 1, range.nteams_eff, range.units_total) - note[1] + 1;
+    }
 
 #pragma unroll 1
-    for (int m = 0; m < cnt; ++m) {
-      if (tid == 0 && m == cnt - 1 && !whole) {
-        // How many of the other pieces have arrived already (see emit_piece).
-        asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];\n"
-                     : "=r"(seen_arrivals)
-                     : "l"(p.piece_ctr + static_cast<int64_t>(pc.b) * p.kv_heads + head)
-                     : "memory");
-      }
-      if (alive) {
-        if (!mbar_wait_bounded(bar + 8 * stage, parity)) {
-          set_status(p.status, B200KV_DEV_WAIT_TIMEOUT);
-          alive = false;
-          for (int i = 1; i < pending; ++i) {   // what else is in flight lands (or gives up) before the CTA may end
-            const int s2 = stage + i < kStages ? stage + i : stage + i - kStages;
-            mbar_wait_bounded(bar + 8 * s2, stage + i < kStages ? parity : parity ^ 1);
-          }
-        }
-        --pending;
-      }
-      if (alive) {
-        const int wtok = min(kPS, pc.len - (pc.begin + warp + kConsumerWarps * m) * kPS);   // valid tokens of the page
-        const uint32_t kb = ring + stage * kPageBytes;
-        const uint32_t vb = kb + kv4::kBlockBytes;
-        // ---- S^T = K Q^T ----------------------------------------------------------------------
-        float s[NB][4];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) s[nb][0] = s[nb][1] = s[nb][2] = s[nb][3] = 0.f;
-        {
-          const uint4 k0 = lds128(kb + k_off), k1 = lds128(kb + k_off + 8 * kv4::kRowBytes);
-          const uint2 c0 = lds64(kb + kv4::kScaleOffset + r * kv4::kScaleBytes);
-          const uint2 c1 = lds64(kb + kv4::kScaleOffset + (r + 8) * kv4::kScaleBytes);
-          const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
-          const uint32_t sc0[4] = {c0.x, c0.x >> 16, c0.y, c0.y >> 16}, sc1[4] = {c1.x, c1.x >> 16, c1.y, c1.y >> 16};
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint32_t a[4], b[4];
-            kv4::unpack_word(w0[g], a);
-            kv4::unpack_word(w1[g], b);
-            const float f0 = half_bits_to_float(sc0[g]), f1 = half_bits_to_float(sc1[g]);
-#pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              float d[4];
-              mma_16816_first(d, a[0], b[0], a[1], b[1], qf[nb][2 * g][0], qf[nb][2 * g][1]);
-              const uint32_t a2[4] = {a[2], b[2], a[3], b[3]};
-              mma_16816(d, a2, qf[nb][2 * g + 1][0], qf[nb][2 * g + 1][1]);
-              s[nb][0] += f0 * d[0];
-              s[nb][1] += f0 * d[1];
-              s[nb][2] += f1 * d[2];
-              s[nb][3] += f1 * d[3];
-            }
-          }
-        }
-        // ---- V scales of tokens 2jq, 2jq+1 | 2jq+8, 2jq+9 as fp16 pairs per group ----------------
-        uint32_t sv[4][2];
-        {
-          const uint4 t0 = lds128(vb + kv4::kScaleOffset + 2 * jq * kv4::kScaleBytes);
-          const uint4 t1 = lds128(vb + kv4::kScaleOffset + (2 * jq + 8) * kv4::kScaleBytes);
-          sv[0][0] = __byte_perm(t0.x, t0.z, 0x5410);
-          sv[1][0] = __byte_perm(t0.x, t0.z, 0x7632);
-          sv[2][0] = __byte_perm(t0.y, t0.w, 0x5410);
-          sv[3][0] = __byte_perm(t0.y, t0.w, 0x7632);
-          sv[0][1] = __byte_perm(t1.x, t1.z, 0x5410);
-          sv[1][1] = __byte_perm(t1.x, t1.z, 0x7632);
-          sv[2][1] = __byte_perm(t1.y, t1.w, 0x5410);
-          sv[3][1] = __byte_perm(t1.y, t1.w, 0x7632);
-        }
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[nb][i] *= p.scale_log2;
-        if (wtok < kPS) {
-          // Rows past the length were never written and may hold anything, NaN scales included.
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (r >= wtok) s[nb][0] = s[nb][1] = -INFINITY;
-            if (r + 8 >= wtok) s[nb][2] = s[nb][3] = -INFINITY;
-          }
-          const uint32_t keep0 = (2 * jq < wtok ? 0xffffu : 0u) | (2 * jq + 1 < wtok ? 0xffff0000u : 0u);
-          const uint32_t keep1 = (2 * jq + 8 < wtok ? 0xffffu : 0u) | (2 * jq + 9 < wtok ? 0xffff0000u : 0u);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            sv[g][0] &= keep0;
-            sv[g][1] &= keep1;
-          }
-        }
-        // ---- has a maximum, or the largest V scale, outgrown its reference? ------------------------
-        uint32_t sv_max = h2_max(h2_max(sv[0][0], sv[0][1]), h2_max(sv[1][0], sv[1][1]));
-        sv_max = h2_max(sv_max, h2_max(h2_max(sv[2][0], sv[2][1]), h2_max(sv[3][0], sv[3][1])));
-        const float sv_hi = fmaxf(half_bits_to_float(sv_max), half_bits_to_float(sv_max >> 16));
-        const float sv_lim = __int_as_float((127 + 6 - shift) << 23);   // 2^(6 - a)
-        bool grow = sv_hi > sv_lim;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) grow |= s[nb][i] > m_run[nb][i & 1] + 8.f;
-        if (__any_sync(0xffffffffu, grow)) {
-          float hi = sv_hi;
-          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
-          hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 2));
-          int new_shift = shift;
-          if (hi > sv_lim) {   // smallest power of two that is not below the scale: exponent of hi rounded up
-            const int e = static_cast<int>((__float_as_uint(hi) + 0x7fffffu) >> 23) - 127;
-            new_shift = max(6 - e, -8);
-          }
-          const float re = __int_as_float((127 + new_shift - shift) << 23);
-          shift = new_shift;
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              float mx = fmaxf(s[nb][h], s[nb][h + 2]);
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-              mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-              const float m_new = fmaxf(m_run[nb][h], mx);
-              const float alpha = m_run[nb][h] == -INFINITY ? 0.f : fast_exp2(m_run[nb][h] - m_new);
-              m_run[nb][h] = m_new;
-              l_run[nb][h] *= alpha;
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                o[j][nb][h] *= alpha * re;
-                o[j][nb][h + 2] *= alpha * re;
-              }
-            }
-        }
-        // ---- P^T -> B fragments ----------------------------------------------------------------------
-        uint32_t pb[NB][2];
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float pr[4];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float msub = m_run[nb][h] == -INFINITY ? 0.f : m_run[nb][h];
-            pr[h] = fast_exp2(s[nb][h] - msub);
-            pr[h + 2] = fast_exp2(s[nb][h + 2] - msub);
-            l_run[nb][h] += pr[h] + pr[h + 2];
-          }
-          pb[nb][0] = movmatrix_trans(pack_half2(pr[0], pr[1]));
-          pb[nb][1] = movmatrix_trans(pack_half2(pr[2], pr[3]));
-        }
-        // ---- O^T += V^T P^T ------------------------------------------------------------------------------
-        const uint32_t up = static_cast<uint32_t>(shift + 15) << 10;   // 2^a in fp16
-        const uint32_t up2 = up | (up << 16);
-        const uint4 v0 = lds128(vb + v_off), v1 = lds128(vb + v_off + kv4::kRowBytes);
-        const uint4 v2 = lds128(vb + v_off + 8 * kv4::kRowBytes), v3 = lds128(vb + v_off + 9 * kv4::kRowBytes);
-        const uint32_t x0[4] = {v0.x, v0.y, v0.z, v0.w}, x1[4] = {v1.x, v1.y, v1.z, v1.w};
-        const uint32_t x2[4] = {v2.x, v2.y, v2.z, v2.w}, x3[4] = {v3.x, v3.y, v3.z, v3.w};
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          uint32_t a[4], b[4];
-          kv4::unpack_word(__byte_perm(x0[g], x1[g], vsel), a);
-          kv4::unpack_word(__byte_perm(x2[g], x3[g], vsel), b);
-          const uint32_t u0 = kv4::h2_mul(sv[g][0], up2), u1 = kv4::h2_mul(sv[g][1], up2);
-#pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const uint32_t q0 = kv4::h2_mul(pb[nb][0], u0), q1 = kv4::h2_mul(pb[nb][1], u1);
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t av[4] = {a[2 * e], a[2 * e + 1], b[2 * e], b[2 * e + 1]};
-              mma_16816(o[2 * g + e][nb], av, q0, q1);
-            }
-          }
-        }
-      }
-      __syncwarp();   // every lane has read the slot
-      if (alive && st.more()) {
-        request(stage);
-        ++pending;
-      }
-      if (++stage == kStages) {
-        stage = 0;
-        parity ^= 1;
-      }
-    }
-
-    // ---- the piece is done: this warp's state to the merge buffer ----------------------------------
-    const float down = __int_as_float((127 - shift) << 23);   // 2^-a
-    consumer_bar();
-    float* mo = merge_o + warp * kD * ROWS;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
+    for (int m = 0; m < cnt; m += 2) {
+      const bool last_step = m + 2 >= cnt;
+      async_wait<kStages - 1>();
+      __syncwarp();   // the pair's pieces were copied by all lanes
+      const int pair = stage * kPairBytes;
+      float s[2][NB][4];
+      uint32_t sv[2][4][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        float l = l_run[nb][h];
-        l += __shfl_xor_sync(0xffffffffu, l, 4);
-        l += __shfl_xor_sync(0xffffffffu, l, 8);
-        l += __shfl_xor_sync(0xffffffffu, l, 16);
-        if (r == 0) {
-          float* ml = merge_ml + (warp * ROWS + nb * 8 + 2 * jq + h) * 2;
-          ml[0] = m_run[nb][h];
-          ml[1] = l;
+        page_scores<NB>(k_at + pair + h * kPageBytes, kc_at + pair + h * kPageBytes, qf, p.scale_log2, s[h]);
+        page_v_scales(vc_at + pair + h * kPageBytes, sv[h]);
+      }
+      if (last_step) {
+        // Rows past the length were never written and a missing second page was not loaded: they may
+        // hold anything, NaN scales included.
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int page = pc.begin + warp + kConsumerWarps * (m + h);
+          const int n = m + h < cnt ? pc.len - page * kPS : 0;   // valid tokens, if fewer than 16
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            if (r >= n) s[h][nb][0] = s[h][nb][1] = -INFINITY;
+            if (r + 8 >= n) s[h][nb][2] = s[h][nb][3] = -INFINITY;
+          }
+          const uint32_t keep0 = (2 * jq < n ? 0xffffu : 0u) | (2 * jq + 1 < n ? 0xffff0000u : 0u);
+          const uint32_t keep1 = (2 * jq + 8 < n ? 0xffffu : 0u) | (2 * jq + 9 < n ? 0xffff0000u : 0u);
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            sv[h][g][0] &= keep0;
+            sv[h][g][1] &= keep1;
+          }
+        }
+      }
+      // ---- would a weight, or a weight times its V scale, leave fp16's range? --------------------
+      uint32_t any_sv = 0;     // bitwise or of non-negative numbers: not below the largest
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) any_sv |= sv[h][g][0] | sv[h][g][1];
+      bool grow = ((any_sv + (0x8000u - sv_lim) * 0x10001u) & 0x80008000u) != 0;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float top = fmaxf(fmaxf(s[0][nb][i], s[0][nb][i + 2]), fmaxf(s[1][nb][i], s[1][nb][i + 2]));
+          grow |= top > m_ref[nb][i] + p_room;
+        }
+      if (__any_sync(0xffffffffu, grow)) {
+        uint32_t top2 = 0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) top2 = h2_max(top2, h2_max(sv[h][g][0], sv[h][g][1]));   // NaN is passed over
+        const float2 tf = h2_to_f2(top2);
+        float hi = fmaxf(tf.x, tf.y);
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 1));
+        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, 2));
+        const int e = min(static_cast<int>(__float_as_uint(hi) >> 23) - 127 + 1, 16);   // hi < 2^e
+        if (e > 1) {
+          p_room = fminf(p_room, static_cast<float>(15 - e));
+          sv_lim = max(sv_lim, static_cast<uint32_t>(e + 15) << 10);
+        }
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            float mx = fmaxf(fmaxf(s[0][nb][i], s[0][nb][i + 2]), fmaxf(s[1][nb][i], s[1][nb][i + 2]));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            // the largest weight so far becomes 2^(p_room - 7), unless the reference is higher already
+            const float m_new = fmaxf(m_ref[nb][i], mx - (p_room - 7.f));
+            const float alpha = m_ref[nb][i] == -INFINITY ? 0.f : fast_exp2(m_ref[nb][i] - m_new);
+            m_ref[nb][i] = m_new;
+            l_run[nb][i] *= alpha;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              o[j][nb][i] *= alpha;
+              o[j][nb][i + 2] *= alpha;
+            }
+          }
+      }
+      // ---- P^T -> B fragments, O^T += V^T (P^T s_V) -------------------------------------------------
+      uint32_t pb[2][NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        const float m0 = m_ref[nb][0] == -INFINITY ? 0.f : m_ref[nb][0];
+        const float m1 = m_ref[nb][1] == -INFINITY ? 0.f : m_ref[nb][1];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float p0 = fast_exp2(s[h][nb][0] - m0), p1 = fast_exp2(s[h][nb][1] - m1);
+          const float p2 = fast_exp2(s[h][nb][2] - m0), p3 = fast_exp2(s[h][nb][3] - m1);
+          l_run[nb][0] += p0 + p2;
+          l_run[nb][1] += p1 + p3;
+          pb[h][nb][0] = movmatrix_trans(pack_half2(p0, p1));
+          pb[h][nb][1] = movmatrix_trans(pack_half2(p2, p3));
         }
       }
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {   // M block j = 2 g + e: rows r and r + 8 are elements d0 and d0 + 2
-        const int d0 = 32 * (j >> 1) + 8 * jv + 4 * (j & 1) + (r & 1);
-        *reinterpret_cast<float2*>(mo + d0 * ROWS + nb * 8 + 2 * jq) = make_float2(o[j][nb][0] * down, o[j][nb][1] * down);
-        *reinterpret_cast<float2*>(mo + (d0 + 2) * ROWS + nb * 8 + 2 * jq) =
-            make_float2(o[j][nb][2] * down, o[j][nb][3] * down);
-      }
+      for (int h = 0; h < 2; ++h) page_pv<NB>(v_at + pair + h * kPageBytes, vsel, sv[h], pb[h], o);
+      __syncwarp();   // every lane has read the slot
+      request(stage);
+      if (++stage == kStages) stage = 0;
     }
-    Tile t{};
-    t.b = pc.b;
-    t.np = pc.np;
-    t.units0 = (pc.flat - pc.begin) + static_cast<int64_t>(p.piece_cost) * pc.kseq;
-    t.whole = whole;
-    emit_piece<ROWS>(p, t, team, head, tid, range.nteams_eff, range.units_total, seen_arrivals, merge_o, merge_ml, arrival);
+
+    finish_piece<ROWS>(p, pc, whole, team, head, tid, o, m_ref, l_run, merge_o, merge_ml, note);
     next_piece(p, seq, range.end, pc);
   }
 }
 
 inline int rows_for_group(int group) { return group <= 8 ? 8 : 16; }
-inline int ctas_per_sm(int rows) { return rows == 8 ? 4 : 3; }
 inline int max_teams(int sms, int kv_heads, int rows) {
-  int t = sms * ctas_per_sm(rows) / kv_heads;
-  if (t > kMaxTeams) t = kMaxTeams;
+  const int t = sms * ctas_per_sm(rows) / kv_heads;
   return t < 1 ? 1 : t;
 }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 template <int ROWS>
 int launch_decode(const Kv4DecodeParams& p, bool programmatic, cudaStream_t stream) {
-  constexpr int smem = kRingBytes + kConsumerWarps * ROWS * kD * 4 + kConsumerWarps * ROWS * 2 * 4 +
-                       kConsumerWarps * kStages * 8 + 4 * 4 + 2 * kSeqCache * 4;
+  constexpr int smem = kRingBytes + kConsumerWarps * ROWS * kD * 4 + kConsumerWarps * ROWS * 2 * 4 + 4 * 4 +
+                       2 * kSeqCache * 4;
   static bool attr_done[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return record_cuda_error(cudaGetLastError());
@@ -585,7 +744,7 @@ size_t kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head
   const int rows = rows_for_group(q_heads / kv_heads);
   const size_t nslots = static_cast<size_t>(max_teams(sms, kv_heads, rows)) + static_cast<size_t>(batch);
   return kCounterBytes + align_up(nslots * kv_heads * rows * kD * sizeof(float), 256) +
-         align_up(nslots * kv_heads * rows * sizeof(float), 256);
+         align_up(nslots * kv_heads * rows * sizeof(float2), 256);
 }
 
 int kv4_paged_decode(const Kv4DecodeArgs& a, cudaStream_t stream) {
