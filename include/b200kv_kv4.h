@@ -21,7 +21,7 @@
  * holds an infinity or a NaN gets a NaN scale: it reads back as NaN, never as a number.
  *
  * A block is contiguous and 16-byte aligned, the rows of a page follow one another, and pages are
- * page_stride_bytes apart (a multiple of 16, at least 2*kv_heads*B200KV_KV4_BLOCK_BYTES).  Slots, page
+ * page_stride_bytes apart (a multiple of 16, at least 2*kv_heads*B200KV_KV4_BLOCK_BYTES, below 2^31).  Slots, page
  * tables, lengths, status words, return codes, stream ordering and the programmatic-launch rule are
  * those of b200kv.h.  head_dim is 128 and page_size 16.
  *

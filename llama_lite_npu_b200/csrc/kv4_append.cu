@@ -331,6 +331,7 @@ int kv4_check_pool(const void* pool, int64_t pool_pages, int64_t page_stride_byt
   if (pool_pages > (int64_t{1} << 27)) return B200KV_ETOOLARGE;   // slots are int32
   if (kv_heads > 1024) return B200KV_ETOOLARGE;
   if (!aligned16(pool) || page_stride_bytes % 16 != 0) return B200KV_EALIGN;
+  if (page_stride_bytes > (int64_t{1} << 31) - 16) return B200KV_ETOOLARGE;   // kernels multiply 32 x 32 bits
   if (page_stride_bytes < static_cast<int64_t>(2) * kv_heads * kv4::kBlockBytes) return B200KV_EINVAL;
   return B200KV_OK;
 }

@@ -38,11 +38,11 @@
 // in the reference (:166, :220), output fp16.  Tensor-bound:
 // flops = 4 * 128 * sum over (query, visible key) pairs, per query head.
 //
-// Over a 4-bit cache (kKv4, include/b200kv_kv4.h) the same pipeline runs with two more warps: they read
-// the blocks of codes and scales straight from the pool, four pages ahead of use in registers, turn them
-// into fp16 (code - 8) * scale, and store each word of codes as one 16-byte piece of the K or V tile
-// where the copies would have put it.  A block read costs 72 bytes per row instead of 256, and a tile is
-// converted in less time than the tensor core and the softmax warps spend on it.  A group of V whose
+// Over a 4-bit cache (kKv4, include/b200kv_kv4.h) the same pipeline runs with a fourth warpgroup: its four
+// warps read the blocks of codes and scales straight from the pool, one ring item ahead of use in
+// registers, turn them into fp16 (code - 8) * scale, and store each word of codes as one 16-byte piece of
+// the K or V tile where the copies would have put it (72 bytes read per row instead of 256).  The
+// registers are split 168 for the softmax warps, 88 for the rest.  A group of V whose
 // scale is NaN must reach only the rows that see its token, and 0 * NaN would reach all: such groups
 // are stored as zeros, the first such position of each group is kept, and the read-out writes NaN from
 // that position on.
@@ -71,9 +71,14 @@ constexpr int kGroups = 2;           // query tiles (heads) per CTA
 constexpr int kGroupWarps = 4;       // softmax warps per tile
 constexpr int kProducerWarp = kGroups * kGroupWarps;
 constexpr int kMmaWarp = kProducerWarp + 1;
-constexpr int kConvertWarps = 2;     // 4-bit pool only
+// 4-bit pool only: a warpgroup of converters (the two warps between it and the MMA warp idle)
+constexpr int kConvertWarp0 = 12;
+constexpr int kConvertWarps = 4;
 constexpr int kConvertThreads = kConvertWarps * 32;
-constexpr int threads_of(bool kv4) { return (kMmaWarp + 1 + (kv4 ? kConvertWarps : 0)) * 32; }
+constexpr int threads_of(bool kv4) { return (kv4 ? kConvertWarp0 + kConvertWarps : kMmaWarp + 1) * 32; }
+// Register split of the 512-thread launch (128 each at launch): 8 * 32 * 168 + 8 * 32 * 88 = 512 * 128.
+constexpr int kSoftmaxRegs = 168, kOtherRegs = 88;
+static_assert(8 * 32 * (kSoftmaxRegs + kOtherRegs) == threads_of(true) * 128, "the split is what the launch has");
 constexpr int kQBytes = kBM * kD * 2;          // 32 KB: [2 d-chunks][128 rows][128 B]
 constexpr int kTileBytes = kBN * kD * 2;       // 32 KB: K or V tile, [2 d-chunks][128 keys][128 B]
 constexpr int kPBytes = kBM * kBN * 2;         // 32 KB: [2 key-chunks][128 rows][128 B]
@@ -210,6 +215,7 @@ struct PrefillParams {
   const uint8_t* pool;
   int64_t pool_pages, page_stride;
   int kv_heads;
+  int one_tile;           // a CTA takes one query tile instead of two
 };
 
 template <bool kKv4>
@@ -254,11 +260,12 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     return;
   }
   const int t_b = static_cast<int>((q_len + kBM - 1) / kBM);   // query tiles of the request
-  if (pair_k > t_b - 1 - pair_k) {                              // also q_len == 0
+  const bool one_tile = kKv4 && p.one_tile;
+  if (one_tile ? pair_k >= t_b : pair_k > t_b - 1 - pair_k) {   // also q_len == 0
     leave_early();
     return;
   }
-  const int n_work = pair_k < t_b - 1 - pair_k ? 2 : 1;
+  const int n_work = !one_tile && pair_k < t_b - 1 - pair_k ? 2 : 1;
   const int64_t q_start_b = static_cast<int64_t>(__ldg(p.q_start + b));
   struct Work {
     int64_t row0;      // first query row of the tile in its request
@@ -352,6 +359,10 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
   cudaGridDependencySynchronize();  // q and the pool belong to earlier kernels until here
   cudaTriggerProgrammaticLaunchCompletion();
 
+  if (warp >= kProducerWarp) {
+  // Register split (4-bit pool): whole warpgroups, one instruction for each side, inside the branch so that
+  // the compiler knows which limit holds there.
+  if (kKv4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" : : "n"(kOtherRegs));
   if (warp == kProducerWarp) {
     // ============================== TMA producer ============================================
     // Ring items alternate K_0, V_0, K_1, V_1, ...; item n lives in slot n % kSlots.  A K or V
@@ -538,121 +549,154 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
       }
       if (!ok) set_status(p.status, B200KV_DEV_WAIT_TIMEOUT);
     }
-  } else if (kKv4 && warp > kMmaWarp) {
+  } else if (kKv4 && warp >= kConvertWarp0) {
     // ============================== 4-bit converters ========================================
-    // Lane = (token row of a page, chunk of its codes): warp 0 takes rows 0..7 of every page, warp 1
-    // rows 8..15; four lanes read a row's 64 bytes of codes and, all four, its 8 bytes of scales.  The
-    // four words of a chunk are the elements 32 g + 8 j .. + 7, one 16-byte piece of the tile each.
-    const int tp = (warp - kMmaWarp - 1) * 8 + (lane >> 2);
+    // A ring item (the K or V rows of a key tile) is 8 pages x 16 rows.  Converter warp c takes rows 8 (c & 1)
+    // .. + 7 of pages (c >> 1), (c >> 1) + 2, ..: four units, all four in flight one item ahead.  Four
+    // lanes read a row's 64 bytes of codes and, all four, its 8 bytes of scales; the four words of a
+    // lane's chunk are the elements 32 g + 8 j .. + 7, one 16-byte piece of the tile each.
+    constexpr int kUnits = kTilePages * 2 / kConvertWarps;
+    const int c = warp - kConvertWarp0;
+    // Token row of the page.  Eight neighbouring lanes store to rows a and a + 4, whose swizzled pieces lie
+    // in different banks (rows a and a + 1 would share them).
+    const int tp = (c & 1) * 8 + ((lane >> 3) | ((lane & 4) ? 4 : 0));
     const int j = lane & 3;
-    const uint8_t* my_rows = p.pool + static_cast<int64_t>(kv_head) * kv4::kBlockBytes;
-    const int64_t v_from_k = static_cast<int64_t>(p.kv_heads) * kv4::kBlockBytes;
-    const int code_off = kv4::chunk_offset(tp, j);
-    const int scale_off = kv4::kScaleOffset + tp * kv4::kScaleBytes;
-    const int32_t* trow = p.table + static_cast<int64_t>(table_row) * p.table_row_stride;
-    const uint32_t dst_row = sm_ring + tp * 128;
+    // This lane's codes and scales of a page are at block + code_off and block + scale_off.
+    const uint8_t* k_lane = p.pool + kv_head * kv4::kBlockBytes + kv4::chunk_offset(tp, j);
+    const int v_from_k = p.kv_heads * kv4::kBlockBytes;
+    const int scale_from_code = kv4::kScaleOffset + tp * kv4::kScaleBytes - kv4::chunk_offset(tp, j);
+    const uint32_t page_stride = static_cast<uint32_t>(p.page_stride);   // the host refuses strides of 2^31 and more
+    const int pool_pages = static_cast<int>(p.pool_pages);
+    const bool by_token = p.table_kind == B200KV_TABLE_TOKEN;
+    const int32_t* trow = p.table + static_cast<int64_t>(table_row) * p.table_row_stride + (by_token ? lane * kPS : lane);
+    const uint32_t dst_row = sm_ring + (c >> 1) * kHalfPage + tp * 128;
     const uint32_t piece0 = static_cast<uint32_t>((j ^ (tp & 7)) << 4), piece1 = static_cast<uint32_t>(((4 + j) ^ (tp & 7)) << 4);
-    // One ring item: the K or V rows of a key tile.  Lane i < 8 holds the table entry of its page i.
+    // One ring item: K or V of key tile `tile` of query tile w; pages 0 .. np - 1 of it exist.
     struct Item {
-      int w, nl, tile, np;
-      bool is_v, valid;
-      int32_t ids;
+      int w, tile, np;
+      bool is_v;
     };
-    auto open_item = [&](int w, int nl) {
-      Item it;
-      const int nt = (w ? work1 : work0).n_tiles;
-      if (nl == 2 * nt) {
-        nl = 0;
-        ++w;
+    auto tiles_of = [&](int w) { return w ? work1.n_tiles : work0.n_tiles; };
+    auto pages_of = [&](int w) { return static_cast<int>(w ? work1.n_pages : work0.n_pages); };
+    auto next_item = [&](Item it) {   // ring order K_0 K_1 V_0 K_2 V_1 ... ; np == 0 after the last
+      const int T = tiles_of(it.w);
+      if (!it.is_v) {
+        if (it.tile == 0 && T > 1) it.tile = 1;
+        else { it.is_v = true; it.tile = it.tile > 0 ? it.tile - 1 : 0; }
+      } else if (it.tile + 2 < T) {
+        it.is_v = false;
+        it.tile += 2;
+      } else if (it.tile + 1 < T) {
+        it.tile += 1;
+      } else {
+        ++it.w;
+        it.is_v = false;
+        it.tile = 0;
       }
-      it.w = w;
-      it.nl = nl;
-      it.valid = w < n_work;
-      it.tile = 0;
-      it.np = 0;
-      it.is_v = false;
-      it.ids = 0;
-      if (it.valid) {
-        const Work& wk = w ? work1 : work0;
-        it.tile = item_tile(nl, wk.n_tiles, it.is_v);
-        const int64_t page0 = static_cast<int64_t>(it.tile) * kTilePages;
-        it.np = static_cast<int>(wk.n_pages - page0 < kTilePages ? wk.n_pages - page0 : kTilePages);
-        if (lane < it.np) it.ids = __ldg(trow + (p.table_kind == B200KV_TABLE_BLOCK ? page0 + lane : (page0 + lane) * kPS));
-      }
+      it.np = it.w < n_work ? min(kTilePages, pages_of(it.w) - it.tile * kTilePages) : 0;
       return it;
     };
-    constexpr int kAhead = 4;     // pages in flight
-    uint4 codes[kAhead];
-    uint2 scales[kAhead];
-    auto load_page = [&](int slot, const Item& it, int i) {   // page i < it.np of the item
-      const int32_t id = __shfl_sync(0xffffffffu, it.ids, i);
-      int64_t page = id;
-      bool ok = true;
-      if (p.table_kind == B200KV_TABLE_TOKEN) {
-        ok = (id & (kPS - 1)) == 0;
-        page = id >> 4;
-      }
-      if (!ok || page < 0 || page >= p.pool_pages) {
-        set_status(p.status, B200KV_DEV_BAD_PAGE);
-        page = 0;  // never dereference a bad entry: report it and read page 0 instead
-      }
-      const uint8_t* block = my_rows + page * p.page_stride + (it.is_v ? v_from_k : 0);
-      codes[slot] = __ldg(reinterpret_cast<const uint4*>(block + code_off));
-      scales[slot] = __ldg(reinterpret_cast<const uint2*>(block + scale_off));
+    auto raw_id = [&](const Item& it) -> int32_t {   // lane i: table entry of page i of the item
+      if (lane >= it.np) return 0;
+      return __ldg(trow + static_cast<int64_t>(it.tile) * (by_token ? kTilePages * kPS : kTilePages));
     };
-    Item cur = open_item(0, 0);
-    Item nxt = open_item(cur.w, cur.nl + 1);
+    // Where this lane finds its codes of the item's pages (c >> 1) + 2 u.  A table entry that names no page
+    // is reported and page 0 read instead.
+    const uint8_t* src[kUnits];
+    auto locate = [&](const Item& it, int32_t id) {
+      bool ok = true;
+      if (by_token) {
+        ok = (id & (kPS - 1)) == 0;
+        id >>= 4;
+      }
+      if (!ok || id < 0 || id >= pool_pages) {
+        set_status(p.status, B200KV_DEV_BAD_PAGE);
+        id = 0;
+      }
+      const uint8_t* base = k_lane + (it.is_v ? v_from_k : 0);
+      int32_t page[kUnits];
 #pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-      if (i < cur.np) load_page(i, cur, i);
-    for (int n = 0;; ++n) {
-      const int sl = n % kSlots;
-      if (n >= kSlots && !mbar_wait_bounded(bar_empty + 8 * sl, ((n / kSlots) - 1) & 1)) {
+      for (int u = 0; u < kUnits; ++u) page[u] = __shfl_sync(0xffffffffu, id, (c >> 1) + 2 * u);
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) src[u] = base + static_cast<uint64_t>(static_cast<uint32_t>(page[u])) * page_stride;
+    };
+    uint4 codes[kUnits];
+    uint2 scales[kUnits];
+    auto load_unit = [&](int u, const Item& it) {
+      if ((c >> 1) + 2 * u < it.np) {
+        codes[u] = __ldg(reinterpret_cast<const uint4*>(src[u]));
+        scales[u] = __ldg(reinterpret_cast<const uint2*>(src[u] + scale_from_code));
+      }
+    };
+    Item cur{0, 0, min(kTilePages, pages_of(0)), false};
+    locate(cur, raw_id(cur));
+#pragma unroll
+    for (int u = 0; u < kUnits; ++u) load_unit(u, cur);
+    Item nxt = next_item(cur);
+    int32_t id_nxt = raw_id(nxt);
+    for (int n = 0, sl = 0, par = 1;; ++n) {
+      if (n >= kSlots && !mbar_wait_bounded(bar_empty + 8 * sl, par)) {
         set_status(p.status, B200KV_DEV_WAIT_TIMEOUT);
         break;
       }
+      if (nxt.np > 0) locate(nxt, id_nxt);
+      const Item after = nxt.np > 0 ? next_item(nxt) : nxt;
+      id_nxt = raw_id(after);     // in flight while this item is converted
+      if (cur.is_v) {
+        // Exponent field all ones in one of the scales (adding one exponent step carries into bit 15)?
+        uint32_t odd = 0;
 #pragma unroll
-      for (int i = 0; i < kTilePages; ++i) {
-        const int slot = i % kAhead;
-        if (i < cur.np) {
-          const uint32_t w[4] = {codes[slot].x, codes[slot].y, codes[slot].z, codes[slot].w};
-          uint32_t s2[4] = {__byte_perm(scales[slot].x, 0, 0x1010), __byte_perm(scales[slot].x, 0, 0x3232),
-                            __byte_perm(scales[slot].y, 0, 0x1010), __byte_perm(scales[slot].y, 0, 0x3232)};
-          if (cur.is_v) {
+        for (int u = 0; u < kUnits; ++u)
+          if ((c >> 1) + 2 * u < cur.np) odd |= (scales[u].x + 0x04000400u) | (scales[u].y + 0x04000400u);
+        if (odd & 0x80008000u) {
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-              if ((s2[g] & 0x7fffu) >= 0x7c00u) {
-                s2[g] = 0;
-                atomicMin(nan_pos + g, cur.tile * kBN + i * kPS + tp);
-              }
-            }
+          for (int u = 0; u < kUnits; ++u) {
+            if ((c >> 1) + 2 * u >= cur.np) continue;
+            const int pos = cur.tile * kBN + ((c >> 1) + 2 * u) * kPS + tp;
+            if ((scales[u].x & 0x7c00u) == 0x7c00u) { scales[u].x &= 0xffff0000u; atomicMin(nan_pos + 0, pos); }
+            if ((scales[u].x & 0x7c000000u) == 0x7c000000u) { scales[u].x &= 0xffffu; atomicMin(nan_pos + 1, pos); }
+            if ((scales[u].y & 0x7c00u) == 0x7c00u) { scales[u].y &= 0xffff0000u; atomicMin(nan_pos + 2, pos); }
+            if ((scales[u].y & 0x7c000000u) == 0x7c000000u) { scales[u].y &= 0xffffu; atomicMin(nan_pos + 3, pos); }
           }
-          const uint32_t dst = dst_row + sl * kTileBytes + i * kHalfPage;
+        }
+      }
+      const uint32_t dst = dst_row + sl * kTileBytes;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        if ((c >> 1) + 2 * u < cur.np) {
+          const uint32_t w[4] = {codes[u].x, codes[u].y, codes[u].z, codes[u].w};
+          const uint32_t s2[4] = {__byte_perm(scales[u].x, 0, 0x1010), __byte_perm(scales[u].x, 0, 0x3232),
+                                  __byte_perm(scales[u].y, 0, 0x1010), __byte_perm(scales[u].y, 0, 0x3232)};
+          uint32_t v[4][4];
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
-            uint32_t v[4];
-            kv4::unpack_word(w[g], v);
-            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + (g >> 1) * (kTileBytes / 2) +
-                                                                          ((g & 1) ? piece1 : piece0)),
-                         "r"(kv4::h2_mul(v[0], s2[g])), "r"(kv4::h2_mul(v[1], s2[g])), "r"(kv4::h2_mul(v[2], s2[g])),
-                         "r"(kv4::h2_mul(v[3], s2[g]))
-                         : "memory");
+            kv4::unpack_word(w[g], v[g]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[g][i] = kv4::h2_mul(v[g][i], s2[g]);
           }
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};\n" ::"r"(dst + 2 * u * kHalfPage + (g >> 1) * (kTileBytes / 2) +
+                                                                          ((g & 1) ? piece1 : piece0)),
+                         "r"(v[g][0]), "r"(v[g][1]), "r"(v[g][2]), "r"(v[g][3])
+                         : "memory");
         }
-        if (i < kTilePages - kAhead) {
-          if (i + kAhead < cur.np) load_page(slot, cur, i + kAhead);
-        } else if (i - (kTilePages - kAhead) < nxt.np) {
-          load_page(slot, nxt, i - (kTilePages - kAhead));
-        }
+        load_unit(u, nxt);
       }
       fence_proxy_async_smem();   // the tile is visible to the tensor core
       mbar_arrive(bar_full + 8 * sl);
-      if (!nxt.valid) break;
+      if (nxt.np <= 0) break;
       cur = nxt;
-      nxt = open_item(cur.w, cur.nl + 1);
+      nxt = after;
+      if (++sl == kSlots) {
+        sl = 0;
+        par ^= 1;
+      }
     }
+  }   // (the two warps between the MMA warp and the converters idle)
   } else {
     // ============================== softmax warps ===========================================
+    if (kKv4) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" : : "n"(kSoftmaxRegs));
     // O accumulates in TMEM.  The running maximum used to scale P and O (m_used) is only moved
     // when the true row maximum has grown by more than 8 (a factor 256, harmless for fp16 P and
     // fp32 accumulation): then O and l are rescaled once; otherwise a tile costs no pass over O.
@@ -934,7 +978,7 @@ int launch_prefill(const PrefillParams& p, const CUtensorMap& qmap, const CUtens
   cudaLaunchConfig_t cfg{};
   // x: (KV head, pair of query heads of its group), adjacent so a group's CTAs share K/V in L2.
   cfg.gridDim = dim3(static_cast<unsigned>(p.kv_heads * ((p.group + 1) / 2)),
-                     static_cast<unsigned>((p.tiles_m + 1) / 2), static_cast<unsigned>(p.batch));
+                     static_cast<unsigned>(p.one_tile ? p.tiles_m : (p.tiles_m + 1) / 2), static_cast<unsigned>(p.batch));
   cfg.blockDim = dim3(threads_of(kKv4));
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
@@ -980,6 +1024,13 @@ int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
   p.pool = static_cast<const uint8_t*>(k.pool);
   p.pool_pages = k.pool_pages;
   p.page_stride = k.page_stride_bytes;
+  // Two query tiles per CTA balance the causal work of many CTAs; where those pairs would leave SMs empty,
+  // one tile per CTA spreads a long tile list over twice as many (chunks of 500 on contexts of 9-16 k,
+  // 2 requests, 32/4 heads: 520 us paired on 64 CTAs, 273 us as 128).
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200KV_ECUDA;
+  const int64_t paired = static_cast<int64_t>(a.kv_heads) * ((p.group + 1) / 2) * ((p.tiles_m + 1) / 2) * a.batch;
+  p.one_tile = paired < sms && p.tiles_m <= 65535;
   return launch_prefill<true>(p, qmap, qmap, qmap, stream);
 }
 

@@ -759,31 +759,79 @@ def empty_kv4_buffer(num_pages: int, kv_heads: int, device="cuda:0") -> torch.Te
     return torch.empty((int(num_pages), 2 * int(kv_heads), KV4_BLOCK_BYTES), dtype=torch.uint8, device=device)
 
 
-def _kv4_pool(KV4_Buffer: torch.Tensor):
-    """``(device index, pointer, pages, page stride in bytes, kv_heads)`` of a 4-bit pool."""
-    t = KV4_Buffer
-    dev = _device_index(t)
-    if t.dtype != torch.uint8 or t.dim() != 3 or t.shape[2] != KV4_BLOCK_BYTES or t.shape[1] % 2 != 0 \
-            or t.shape[1] == 0:
+def _kv4_pool(t: torch.Tensor):
+    """``(device index, pointer, pages, page stride in bytes, kv_heads)`` of a 4-bit pool.
+
+    These operators run once per layer and step, and their kernels take a few microseconds: each
+    tensor attribute is read once and nothing is formatted unless it is raised."""
+    dev = t.get_device()
+    if dev < 0:
+        _device_index(t)     # raises
+    if t.dtype is not torch.uint8 or t.dim() != 3:
         raise ValueError(f"KV4_Buffer must be uint8 [num_pages, 2*kv_heads, {KV4_BLOCK_BYTES}]")
+    pages, rows, block = t.shape
     s0, s1, s2 = t.stride()
+    if block != KV4_BLOCK_BYTES or rows == 0 or rows & 1:
+        raise ValueError(f"KV4_Buffer must be uint8 [num_pages, 2*kv_heads, {KV4_BLOCK_BYTES}]")
     if s2 != 1 or s1 != KV4_BLOCK_BYTES:
         raise ValueError("KV4_Buffer must be contiguous inside a page")
-    pages = t.shape[0]
     if pages <= 1:          # the stride of a dimension of one may be anything
-        s0 = max(s0, t.shape[1] * KV4_BLOCK_BYTES)
-    return dev, t.data_ptr(), pages, s0, t.shape[1] // 2
+        s0 = max(s0, rows * KV4_BLOCK_BYTES)
+    return dev, t.data_ptr(), pages, s0, rows >> 1
 
 
-def _on_pool_device(KV4_Buffer: torch.Tensor, **tensors) -> None:
-    for name, t in tensors.items():
-        if t is not None and t.device != KV4_Buffer.device:
-            raise ValueError(f"{name} must be on the pool's device {KV4_Buffer.device} (got {t.device})")
+def _off_device(name: str, t: torch.Tensor, dev: int) -> ValueError:
+    return ValueError(f"{name} must be on the pool's device cuda:{dev} (got {t.device})")
 
 
-def _slots_arg(Select_Index: torch.Tensor) -> torch.Tensor:
-    _require(Select_Index.dtype == torch.int32 and Select_Index.dim() == 1, "Select_Index must be a 1-D int32 tensor")
-    return Select_Index if Select_Index.is_contiguous() else Select_Index.contiguous()
+def _slots_arg(slots: torch.Tensor, dev: int) -> torch.Tensor:
+    if slots.dtype is not torch.int32 or slots.dim() != 1:
+        raise ValueError("Select_Index must be a 1-D int32 tensor")
+    if slots.get_device() != dev:
+        raise _off_device("Select_Index", slots, dev)
+    return slots if slots.is_contiguous() else slots.contiguous()
+
+
+def _table_arg(tbl: torch.Tensor, table_kind: str, dev: int):
+    """``(pointer, row stride, kind, rows, columns)`` of a page or token table."""
+    kind = _TABLE_KINDS.get(table_kind, -1)
+    if kind != TABLE_BLOCK and kind != TABLE_TOKEN:
+        raise ValueError("the 4-bit operators take a 'token' or 'block' table")
+    if tbl.dtype is not torch.int32 or tbl.dim() != 2 or tbl.stride(1) != 1:
+        raise ValueError("the table must be a 2-D int32 tensor contiguous along its last dimension")
+    if tbl.get_device() != dev:
+        raise _off_device("the table", tbl, dev)
+    rows, cols = tbl.shape
+    return tbl.data_ptr(), tbl.stride(0) if rows > 1 else cols, kind, rows, cols
+
+
+def _ints_arg(t: torch.Tensor, name: str, n: int, dev: int, wide: bool) -> int:
+    """Pointer of a contiguous 1-D tensor of ``n`` int32 (or, where ``wide``, int64) values."""
+    if (t.dtype is not torch.int32 and not (wide and t.dtype is torch.int64)) or t.dim() != 1 \
+            or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous 1-D {'int32 or int64' if wide else 'int32'} tensor of {n} values")
+    if t.get_device() != dev:
+        raise _off_device(name, t, dev)
+    return t.data_ptr()
+
+
+def _rows_arg(t: torch.Tensor, name: str, heads: int, n: int, dev: int):
+    """``(pointer, token stride)`` of fp16 head rows ``[>= n, heads, 128]``, contiguous inside a token."""
+    if t.dtype is not torch.float16 or t.dim() != 3:
+        raise ValueError(f"{name} must be float16 [tokens, {heads}, {KV4_HEAD_DIM}]")
+    m, h, d = t.shape
+    s0, s1, s2 = t.stride()
+    if h != heads or d != KV4_HEAD_DIM or m < n:
+        raise ValueError(f"{name} must be float16 [{n} or more, {heads}, {KV4_HEAD_DIM}] (got {tuple(t.shape)})")
+    if s2 != 1 or (s1 != KV4_HEAD_DIM and heads > 1):
+        raise ValueError(f"{name} must be contiguous inside a token")
+    if t.get_device() != dev:
+        raise _off_device(name, t, dev)
+    return t.data_ptr(), s0 if n > 1 else heads * KV4_HEAD_DIM
+
+
+_capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing") else \
+    torch.cuda.is_current_stream_capturing
 
 
 def _capture_of(stream: int) -> int:
@@ -795,15 +843,18 @@ def _capture_of(stream: int) -> int:
     return found.value
 
 
-def _status_ptr(device_index: int, capture: int = 0) -> int:
+def _status_ptr(device_index: int) -> int:
     """The status word's address; none when it would first have to be created inside a capture (its
     zero-fill would become part of the graph)."""
-    if capture and device_index not in _status:
-        return 0
-    return status_tensor(device_index).data_ptr()
+    st = _status.get(device_index)
+    if st is None:
+        if _capturing():
+            return 0
+        st = status_tensor(device_index)
+    return st.data_ptr()
 
 
-def kv4_decode_workspace(device_index: int, stream: int, capture: int, batch: int, q_heads: int, kv_heads: int,
+def kv4_decode_workspace(device_index: int, stream: int, batch: int, q_heads: int, kv_heads: int,
                          head_dim: int) -> torch.Tensor:
     """Scratch of :func:`flash_decoding_kv4`: arrival counters (zero between calls) and partials.
 
@@ -819,6 +870,7 @@ def kv4_decode_workspace(device_index: int, stream: int, capture: int, batch: in
                              f"batch * kv_heads at most {DECODE_COUNTER_BYTES // 4}")
         _workspace_need[key] = need
     where = (device_index, stream)
+    capture = _capture_of(stream) if _capturing() else 0
     if capture:
         held = _kv4_graph_workspace.get(where)
         if held is not None and held[0] == capture and held[1].numel() >= need:
@@ -836,69 +888,51 @@ def kv4_decode_workspace(device_index: int, stream: int, capture: int, batch: in
     return ws
 
 
-def _kv4_append_call(k_ptr, v_ptr, n, k_stride, v_stride, slots, KV4_Buffer, pool) -> None:
-    dev, ptr, pages, page_stride, kvh = pool
-    with _on_device(dev):
-        stream = _stream(dev)
-        rc = _lib.lib().b200kv_kv4_append(
-            k_ptr, v_ptr, n, k_stride, v_stride, slots.data_ptr(), ptr, pages, page_stride, kvh, KV4_HEAD_DIM,
-            _status_ptr(dev, 0 if dev in _status else _capture_of(stream)), stream)
-    _lib.check(rc)
-    _after_call(dev)
+def _kv4_done(rc: int, dev: int) -> None:
+    if rc != 0:
+        _lib.check(rc)
+    if _DEBUG:
+        check_status(dev)
 
 
-@torch.no_grad()
 def update_kv_buffer_kv4(KV_Values: torch.Tensor, Select_Index: torch.Tensor, KV4_Buffer: torch.Tensor) -> None:
     """:func:`update_kv_buffer` into a 4-bit pool: row ``i`` of ``KV_Values`` ``[num_tokens, 2*kv_heads,
     128]`` (fp16) is quantised in groups of 32 elements and written to slot ``Select_Index[i]``.
 
     A slot outside the pool is skipped and reported in the device status.  Two tokens of one call
     may name the same slot only with identical rows."""
-    pool = _kv4_pool(KV4_Buffer)
-    kvh = pool[4]
-    _on_pool_device(KV4_Buffer, KV_Values=KV_Values, Select_Index=Select_Index)
-    _require(KV_Values.dtype == torch.float16 and KV_Values.dim() == 3
-             and KV_Values.shape[1:] == (2 * kvh, KV4_HEAD_DIM),
-             f"KV_Values must be float16 [num_tokens, {2 * kvh}, {KV4_HEAD_DIM}]")
-    _require(KV_Values.stride(2) == 1 and KV_Values.stride(1) == KV4_HEAD_DIM,
-             "KV_Values must be contiguous inside a token")
-    slots = _slots_arg(Select_Index)
+    dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
+    slots = _slots_arg(Select_Index, dev)
     n = slots.shape[0]
-    _require(KV_Values.shape[0] >= n, "KV_Values has fewer rows than Select_Index")
+    k_ptr, stride = _rows_arg(KV_Values, "KV_Values", 2 * kvh, n, dev)
     if n == 0:
         return
     if _DEBUG:
-        _debug_check_append(KV_Values, slots, pool[2] * KV4_PAGE_SIZE)
-    stride = KV_Values.stride(0) if n > 1 else 2 * kvh * KV4_HEAD_DIM
-    k_ptr = KV_Values.data_ptr()
-    _kv4_append_call(k_ptr, k_ptr + kvh * KV4_HEAD_DIM * 2, n, stride, stride, slots, KV4_Buffer, pool)
+        _debug_check_append(KV_Values, slots, pages * KV4_PAGE_SIZE)
+    with _on_device(dev):
+        rc = _lib.lib().b200kv_kv4_append(k_ptr, k_ptr + kvh * KV4_HEAD_DIM * 2, n, stride, stride, slots.data_ptr(),
+                                          ptr, pages, page_stride, kvh, KV4_HEAD_DIM, _status_ptr(dev), _stream(dev))
+    _kv4_done(rc, dev)
 
 
-@torch.no_grad()
 def update_kv_buffer_kv4_split(xk: torch.Tensor, xv: torch.Tensor, Select_Index: torch.Tensor,
                                KV4_Buffer: torch.Tensor) -> None:
     """:func:`update_kv_buffer_kv4` with K and V given separately (``[num_tokens, kv_heads, 128]`` each)."""
-    pool = _kv4_pool(KV4_Buffer)
-    kvh = pool[4]
-    _on_pool_device(KV4_Buffer, xk=xk, xv=xv, Select_Index=Select_Index)
-    for t, name in ((xk, "xk"), (xv, "xv")):
-        _require(t.dtype == torch.float16 and t.dim() == 3 and t.shape[1:] == (kvh, KV4_HEAD_DIM),
-                 f"{name} must be float16 [num_tokens, {kvh}, {KV4_HEAD_DIM}]")
-        _require(t.stride(2) == 1 and (kvh == 1 or t.stride(1) == KV4_HEAD_DIM),
-                 f"{name} must be contiguous inside a token")
-    slots = _slots_arg(Select_Index)
+    dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
+    slots = _slots_arg(Select_Index, dev)
     n = slots.shape[0]
-    _require(xk.shape[0] >= n and xv.shape[0] >= n, "xk or xv has fewer rows than Select_Index")
+    k_ptr, k_stride = _rows_arg(xk, "xk", kvh, n, dev)
+    v_ptr, v_stride = _rows_arg(xv, "xv", kvh, n, dev)
     if n == 0:
         return
     if _DEBUG:
-        _debug_check_append(torch.cat([xk[:n], xv[:n]], dim=1), slots, pool[2] * KV4_PAGE_SIZE)
-    row = kvh * KV4_HEAD_DIM
-    _kv4_append_call(xk.data_ptr(), xv.data_ptr(), n, xk.stride(0) if n > 1 else row,
-                     xv.stride(0) if n > 1 else row, slots, KV4_Buffer, pool)
+        _debug_check_append(torch.cat([xk[:n], xv[:n]], dim=1), slots, pages * KV4_PAGE_SIZE)
+    with _on_device(dev):
+        rc = _lib.lib().b200kv_kv4_append(k_ptr, v_ptr, n, k_stride, v_stride, slots.data_ptr(), ptr, pages, page_stride,
+                                          kvh, KV4_HEAD_DIM, _status_ptr(dev), _stream(dev))
+    _kv4_done(rc, dev)
 
 
-@torch.no_grad()
 def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
                                   k_norm_weight: Optional[torch.Tensor], eps: float, cos: torch.Tensor,
                                   sin: torch.Tensor, Select_Index: torch.Tensor, KV4_Buffer: torch.Tensor,
@@ -906,79 +940,82 @@ def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_we
     """:func:`fused_qk_norm_rope_append` into a 4-bit pool: QK-RMSNorm, rotary embedding, and the
     quantising append of K (normalised, rotated, rounded to fp16) and V in one launch.  Arguments and
     return value as there."""
-    pool = _kv4_pool(KV4_Buffer)
-    dev, ptr, pages, page_stride, kvh = pool
+    dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
     d = KV4_HEAD_DIM
-    _require(xq.dim() == 3 and xq.dtype == torch.float16 and xq.shape[2] == d and xq.shape[1] > 0,
-             f"xq must be float16 [n, q_heads, {d}]")
+    if xq.dim() != 3 or xq.shape[1] == 0:
+        raise ValueError(f"xq must be float16 [n, q_heads, {d}]")
     n, qh, _ = xq.shape
-    out = xq if out is None else out
-    _on_pool_device(KV4_Buffer, xq=xq, xkv=xkv, q_norm_weight=q_norm_weight, k_norm_weight=k_norm_weight, cos=cos,
-                    sin=sin, Select_Index=Select_Index, out=out)
-    _require(xkv.dim() in (2, 3) and xkv.shape[0] == n, "xkv must be [n, 2*kv_heads*head_dim], one row per token")
-    xkv = xkv.reshape(n, 2 * kvh * d) if xkv.dim() != 2 and xkv.numel() == n * 2 * kvh * d else xkv
-    _require(xkv.dtype == torch.float16 and xkv.shape == (n, 2 * kvh * d) and xkv.stride(1) == 1,
-             "xkv must be [n, 2*kv_heads*head_dim] float16, contiguous rows")
-    _require(out.shape == xq.shape and out.dtype == torch.float16, "out must match xq")
-    for t, name in ((xq, "xq"), (out, "out")):
-        _require(t.stride(2) == 1 and (qh == 1 or t.stride(1) == d), f"{name} must be contiguous inside a token")
-    cos2, sin2 = cos.reshape(-1, cos.shape[-1]), sin.reshape(-1, sin.shape[-1])
-    _require(cos2.dtype == torch.float16 and sin2.dtype == torch.float16, "cos and sin must be float16")
-    _require(cos2.shape == sin2.shape and cos2.shape[0] == n and cos2.shape[1] in (d, d // 2)
-             and cos2.stride(1) == 1 and sin2.stride(1) == 1 and (n <= 1 or cos2.stride(0) == sin2.stride(0)),
-             "cos and sin must be one row of head_dim (or head_dim/2) per token with equal strides")
+    q_ptr, q_stride = _rows_arg(xq, "xq", qh, n, dev)
+    if out is None:
+        out, out_ptr, out_stride = xq, q_ptr, q_stride
+    else:
+        if out.shape != xq.shape:
+            raise ValueError("out must match xq")
+        out_ptr, out_stride = _rows_arg(out, "out", qh, n, dev)
+    row = 2 * kvh * d
+    if xkv.dim() == 3 and xkv.shape[1:] == (2 * kvh, d):
+        xkv = xkv.reshape(n, row) if xkv.shape[0] == n else xkv
+    if xkv.dtype is not torch.float16 or xkv.dim() != 2 or xkv.shape != (n, row) or xkv.stride(1) != 1:
+        raise ValueError("xkv must be [n, 2*kv_heads*head_dim] float16, contiguous rows")
+    if xkv.get_device() != dev:
+        raise _off_device("xkv", xkv, dev)
+    if cos.dim() != 2 or sin.dim() != 2:
+        cos, sin = cos.reshape(-1, cos.shape[-1]), sin.reshape(-1, sin.shape[-1])
+    width = cos.shape[1]
+    if cos.dtype is not torch.float16 or sin.dtype is not torch.float16:
+        raise ValueError("cos and sin must be float16")
+    if cos.shape != (n, width) or sin.shape != (n, width) or (width != d and width != d // 2) \
+            or cos.stride(1) != 1 or sin.stride(1) != 1 or (n > 1 and cos.stride(0) != sin.stride(0)):
+        raise ValueError("cos and sin must be one row of head_dim (or head_dim/2) per token with equal strides")
+    if cos.get_device() != dev or sin.get_device() != dev:
+        raise _off_device("cos and sin", cos if cos.get_device() != dev else sin, dev)
     for w, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        _require(w is None or (w.dtype == torch.float16 and w.shape == (d,) and w.is_contiguous()),
-                 f"{name} must be a contiguous float16 [head_dim] tensor or None")
-    slots = _slots_arg(Select_Index)
-    _require(slots.shape[0] == n, "Select_Index must name one slot per token")
+        if w is not None:
+            if w.dtype is not torch.float16 or w.shape != (d,) or not w.is_contiguous():
+                raise ValueError(f"{name} must be a contiguous float16 [head_dim] tensor or None")
+            if w.get_device() != dev:
+                raise _off_device(name, w, dev)
+    slots = _slots_arg(Select_Index, dev)
+    if slots.shape[0] != n:
+        raise ValueError("Select_Index must name one slot per token")
     if n == 0:
         return out
     if _DEBUG:
         _debug_check_append(xkv, slots, pages * KV4_PAGE_SIZE)
-    one = n == 1
     with _on_device(dev):
-        stream = _stream(dev)
         rc = _lib.lib().b200kv_kv4_qk_norm_rope_append(
-            xq.data_ptr(), out.data_ptr(), qh * d if one else xq.stride(0), qh * d if one else out.stride(0),
-            xkv.data_ptr(), 2 * kvh * d if one else xkv.stride(0),
+            q_ptr, out_ptr, q_stride, out_stride, xkv.data_ptr(), xkv.stride(0) if n > 1 else row,
             0 if q_norm_weight is None else q_norm_weight.data_ptr(),
             0 if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps),
-            cos2.data_ptr(), sin2.data_ptr(), d if one else cos2.stride(0), slots.data_ptr(),
-            ptr, pages, page_stride, n, qh, kvh, d,
-            _status_ptr(dev, 0 if dev in _status else _capture_of(stream)), stream)
-    _lib.check(rc)
-    _after_call(dev)
+            cos.data_ptr(), sin.data_ptr(), cos.stride(0) if n > 1 else d, slots.data_ptr(),
+            ptr, pages, page_stride, n, qh, kvh, d, _status_ptr(dev), _stream(dev))
+    _kv4_done(rc, dev)
     return out
 
 
-@torch.no_grad()
 def gather_kv_buffer_kv4(KV4_Buffer: torch.Tensor, Select_Index: torch.Tensor,
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The rows a 4-bit pool stands for: fp16 ``[n, 2*kv_heads, 128]``, row ``i`` from slot
     ``Select_Index[i]``.  A slot outside the pool gives zeros and is reported in the device status."""
     dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
-    _on_pool_device(KV4_Buffer, Select_Index=Select_Index, out=out)
-    slots = _slots_arg(Select_Index)
+    slots = _slots_arg(Select_Index, dev)
     n, d = slots.shape[0], KV4_HEAD_DIM
     if out is None:
-        out = torch.empty((n, 2 * kvh, d), dtype=torch.float16, device=KV4_Buffer.device)
+        out = torch.empty((n, 2 * kvh, d), dtype=torch.float16, device=slots.device)
+        out_ptr, out_stride = out.data_ptr(), 2 * kvh * d
     else:
-        _require(out.dtype == torch.float16 and out.shape == (n, 2 * kvh, d) and out.stride(2) == 1
-                 and out.stride(1) == d, f"out must be float16 [{n}, {2 * kvh}, {d}], contiguous inside a token")
+        out_ptr, out_stride = _rows_arg(out, "out", 2 * kvh, n, dev)
+        if out.shape[0] != n:
+            raise ValueError(f"out must hold {n} rows")
     if n == 0:
         return out
     with _on_device(dev):
-        stream = _stream(dev)
-        rc = _lib.lib().b200kv_kv4_gather(
-            ptr, pages, page_stride, slots.data_ptr(), n, out.data_ptr(), out.stride(0) if n > 1 else 2 * kvh * d,
-            kvh, d, _status_ptr(dev, 0 if dev in _status else _capture_of(stream)), stream)
-    _lib.check(rc)
-    _after_call(dev)
+        rc = _lib.lib().b200kv_kv4_gather(ptr, pages, page_stride, slots.data_ptr(), n, out_ptr, out_stride, kvh, d,
+                                          _status_ptr(dev), _stream(dev))
+    _kv4_done(rc, dev)
     return out
 
 
-@torch.no_grad()
 def flash_decoding_kv4(
     q: torch.Tensor,
     KV4_Buffer: torch.Tensor,
@@ -996,53 +1033,50 @@ def flash_decoding_kv4(
     """:func:`flash_decoding` over a 4-bit pool; the pool is passed whole instead of as a K and a V view.
     Every element counts as scale * (code - 8); a sequence of length 0 gives a zero row."""
     dev, ptr, pages, page_stride, kv_heads = _kv4_pool(KV4_Buffer)
-    tbl = b_req_tokens_table
-    if q.dtype != torch.float16 or q.dim() != 3 or q.shape[2] != KV4_HEAD_DIM or q.stride(2) != 1:
+    if q.dtype is not torch.float16 or q.dim() != 3:
         raise ValueError(f"q must be float16 [batch, heads, {KV4_HEAD_DIM}], contiguous along head_dim")
     batch, q_heads, d = q.shape
-    _on_pool_device(KV4_Buffer, q=q, b_req_tokens_table=tbl, b_seq_len=b_seq_len, b_req_idx=b_req_idx, out=out)
-    kind = _TABLE_KINDS.get(table_kind, -1)
-    if kind not in (TABLE_BLOCK, TABLE_TOKEN):
-        raise ValueError("decode takes a 'token' or 'block' table")
-    if tbl.dtype != torch.int32 or tbl.dim() != 2 or tbl.stride(1) != 1:
-        raise ValueError("the table must be a 2-D int32 tensor contiguous along its last dimension")
-    tbl_rows, tbl_cols = tbl.shape
-    lens_dtype = b_seq_len.dtype
-    if lens_dtype not in (torch.int64, torch.int32) or b_seq_len.shape != (batch,) or not b_seq_len.is_contiguous():
-        raise ValueError("b_seq_len must be a contiguous int32 or int64 tensor with one entry per batch row")
+    q_sb, q_sh, q_sd = q.stride()
+    if d != KV4_HEAD_DIM or q_sd != 1:
+        raise ValueError(f"q must be float16 [batch, heads, {KV4_HEAD_DIM}], contiguous along head_dim")
+    if q.get_device() != dev:
+        raise _off_device("q", q, dev)
+    tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols = _table_arg(b_req_tokens_table, table_kind, dev)
+    lens_ptr = _ints_arg(b_seq_len, "b_seq_len", batch, dev, True)
     if b_req_idx is not None:
-        if b_req_idx.dtype != torch.int32 or b_req_idx.shape != (batch,) or not b_req_idx.is_contiguous():
-            raise ValueError("b_req_idx must be contiguous int32 [batch]")
-    elif tbl_rows < batch:
-        raise ValueError("the table has fewer rows than the batch")
+        rows_ptr = _ints_arg(b_req_idx, "b_req_idx", batch, dev, False)
+    else:
+        rows_ptr = 0
+        if tbl_rows < batch:
+            raise ValueError("the table has fewer rows than the batch")
     max_len = int(max_actual_seq_len)
     if not 0 <= max_len <= tbl_cols * (page_size if kind == TABLE_BLOCK else 1):
         raise ValueError("max_actual_seq_len exceeds the table width")
     if out is None:
         out = torch.empty((batch, q_heads, d), dtype=torch.float16, device=q.device)
-    elif out.shape != q.shape or out.dtype != torch.float16 or out.stride(2) != 1:
-        raise ValueError("out must match q")
+        out_sb, out_sh = q_heads * d, d
+    else:
+        out_sb, out_sh, out_sd = out.stride() if out.dim() == 3 else (0, 0, 0)
+        if out.shape != q.shape or out.dtype is not torch.float16 or out_sd != 1:
+            raise ValueError("out must match q")
+        if out.get_device() != dev:
+            raise _off_device("out", out, dev)
     if batch == 0:
         return out
     if _DEBUG:
         _debug_check_lengths(b_seq_len, max_len, b_req_idx, tbl_rows, "decode")
     with _on_device(dev):
         stream = _stream(dev)
-        capture = _capture_of(stream)
-        ws = kv4_decode_workspace(dev, stream, capture, batch, q_heads, kv_heads, d)
+        ws = kv4_decode_workspace(dev, stream, batch, q_heads, kv_heads, d)
         rc = _lib.lib().b200kv_kv4_paged_decode(
-            q.data_ptr(), q.stride(0), q.stride(1), ptr, pages, page_stride,
-            tbl.data_ptr(), tbl.stride(0) if tbl_rows > 1 else tbl_cols, kind, tbl_rows, tbl_cols,
-            0 if b_req_idx is None else b_req_idx.data_ptr(), b_seq_len.data_ptr(), lens_dtype == torch.int64,
-            batch, q_heads, kv_heads, d, int(page_size), float(qk_scale), max_len, ws.data_ptr(), ws.numel(),
-            out.data_ptr(), out.stride(0), out.stride(1), DECODE_SERIALIZED if metadata_fresh else 0,
-            _status_ptr(dev, capture), stream)
-    _lib.check(rc)
-    _after_call(dev)
+            q.data_ptr(), q_sb, q_sh, ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols,
+            rows_ptr, lens_ptr, b_seq_len.dtype is torch.int64, batch, q_heads, kv_heads, d, int(page_size), float(qk_scale),
+            max_len, ws.data_ptr(), ws.numel(), out.data_ptr(), out_sb, out_sh,
+            DECODE_SERIALIZED if metadata_fresh else 0, _status_ptr(dev), stream)
+    _kv4_done(rc, dev)
     return out
 
 
-@torch.no_grad()
 def paged_chunk_flash_attention_kv4(
     q: torch.Tensor,
     KV4_Buffer: torch.Tensor,
@@ -1060,43 +1094,33 @@ def paged_chunk_flash_attention_kv4(
     """:func:`paged_chunk_flash_attention` over a 4-bit pool (passed whole); the chunk's own rows have been
     appended to it.  ``sm_scale`` carries log2(e), as there.  Returns a tensor like ``q``."""
     dev, ptr, pages, page_stride, kv_heads = _kv4_pool(KV4_Buffer)
-    _require(q.dtype == torch.float16 and q.dim() == 3 and q.shape[2] == KV4_HEAD_DIM and q.stride(2) == 1,
-             f"q must be float16 [tokens, heads, {KV4_HEAD_DIM}], contiguous along head_dim")
-    kind = _TABLE_KINDS.get(table_kind, -1)
-    _require(kind in (TABLE_BLOCK, TABLE_TOKEN), "paged prefill takes a 'token' or 'block' table")
-    tbl = req_token_table
-    _on_pool_device(KV4_Buffer, q=q, req_token_table=tbl, req_ids=req_ids, q_start_loc=q_start_loc,
-                    context_lens=context_lens, q_seq_lens=q_seq_lens)
-    _require(tbl.dtype == torch.int32 and tbl.dim() == 2 and tbl.stride(1) == 1,
-             "the table must be a 2-D int32 tensor contiguous along its last dimension")
-    qlen_ptr, lens_i64 = _lens_arg(q_seq_lens, "q_seq_lens")
-    batch = int(q_seq_lens.shape[0])
-    _require(req_ids.dtype == torch.int32 and req_ids.shape == (batch,) and req_ids.is_contiguous(),
-             "req_ids must be contiguous int32 [batch]")
-    _require(q_start_loc.dtype == torch.int32 and q_start_loc.shape == (batch,)
-             and q_start_loc.is_contiguous(), "q_start_loc must be contiguous int32 [batch]")
-    _require(context_lens.dtype == q_seq_lens.dtype and context_lens.shape == (batch,),
-             "context_lens and q_seq_lens must share dtype and shape")
-    ctx_ptr, _ = _lens_arg(context_lens, "context_lens")
+    if q.dtype is not torch.float16 or q.dim() != 3 or q.shape[2] != KV4_HEAD_DIM or q.stride(2) != 1:
+        raise ValueError(f"q must be float16 [tokens, heads, {KV4_HEAD_DIM}], contiguous along head_dim")
+    if q.get_device() != dev:
+        raise _off_device("q", q, dev)
+    tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols = _table_arg(req_token_table, table_kind, dev)
+    batch = q_seq_lens.shape[0] if q_seq_lens.dim() == 1 else -1
+    qlen_ptr = _ints_arg(q_seq_lens, "q_seq_lens", batch, dev, True)
+    ctx_ptr = _ints_arg(context_lens, "context_lens", batch, dev, True)
+    if context_lens.dtype is not q_seq_lens.dtype:
+        raise ValueError("context_lens and q_seq_lens must share dtype and shape")
+    ids_ptr = _ints_arg(req_ids, "req_ids", batch, dev, False)
+    start_ptr = _ints_arg(q_start_loc, "q_start_loc", batch, dev, False)
     total_q, q_heads, d = q.shape
     output = torch.empty((total_q, q_heads, d), dtype=torch.float16, device=q.device)
-    if q.numel() == 0 or batch == 0:
+    if total_q == 0 or q_heads == 0 or batch == 0:
         return output
     if _DEBUG:
-        width = tbl.shape[1] * (page_size if kind == TABLE_BLOCK else 1)
-        _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, tbl.shape[0], "paged prefill")
+        width = tbl_cols * (page_size if kind == TABLE_BLOCK else 1)
+        _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, tbl_rows, "paged prefill")
         _debug_check_lengths(q_seq_lens, int(max_q_len), None, 0, "paged prefill chunk")
     with _on_device(dev):
-        stream = _stream(dev)
         rc = _lib.lib().b200kv_kv4_paged_prefill(
             q.data_ptr(), q.stride(0) if total_q > 1 else q_heads * d, q.stride(1) if q_heads > 1 else d,
-            ptr, pages, page_stride, tbl.data_ptr(), tbl.stride(0) if tbl.shape[0] > 1 else tbl.shape[1], kind,
-            tbl.shape[0], tbl.shape[1], req_ids.data_ptr(), q_start_loc.data_ptr(), ctx_ptr, qlen_ptr, lens_i64,
-            batch, total_q, int(max_q_len), q_heads, kv_heads, d, int(page_size), float(sm_scale),
-            output.data_ptr(), output.stride(0), output.stride(1),
-            _status_ptr(dev, 0 if dev in _status else _capture_of(stream)), stream)
-    _lib.check(rc)
-    _after_call(dev)
+            ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols, ids_ptr, start_ptr, ctx_ptr,
+            qlen_ptr, q_seq_lens.dtype is torch.int64, batch, total_q, int(max_q_len), q_heads, kv_heads, d,
+            int(page_size), float(sm_scale), output.data_ptr(), q_heads * d, d, _status_ptr(dev), _stream(dev))
+    _kv4_done(rc, dev)
     return output
 
 
