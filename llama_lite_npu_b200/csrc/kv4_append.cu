@@ -16,10 +16,13 @@
 // about one K in 4000 to the neighbouring fp16 number and now and then a code with it.  Q keeps
 // 32-bit statistics: its rows are rounded once and nothing is decided by them.
 //
-// A warp takes one head row of four neighbouring tokens, eight lanes to a row.  A lane owns 8
-// elements of the first half of head_dim and the 8 they rotate with, i.e. one 32-bit word of codes in
-// each of two groups; the words of lanes l and l ^ 4 make up one 16-byte chunk of the row.  Four
-// neighbouring tokens of a page are 256 contiguous bytes of codes and one 32-byte sector of scales.
+// A warp takes kRows (one, or four where there are enough tokens to fill the GPU with them) head rows of
+// four neighbouring tokens, eight lanes to a row, all of its loads in flight before the first is used.
+// A lane owns 8 elements of the first half of head_dim and the 8 they rotate with, i.e. one 32-bit word
+// of codes in each of two groups; the words of lanes l and l ^ 4 make up one 16-byte chunk of the row.
+// Four neighbouring tokens of a page are 256 contiguous bytes of codes and one 32-byte sector of scales.
+// The arithmetic is kept short, or it and not HBM would bound the launch (4 instructions per element:
+// to 32 bits, multiply-add, floor by a directed addition, shift-add into the word).
 // HBM-bound: per token 2 * KH * 256 B read and 2 * KH * 72 B written (+ 2 * QH * 256 B of Q and 256 B of
 // cos / sin for the fused form).
 #include "kv4.cuh"
@@ -44,8 +47,9 @@ struct AppendParams {
   int64_t pool_tokens, page_stride;
   int n_tokens, q_heads, kv_heads;
   int rows_per_token;         // head rows of a token: 2 * kv_heads (+ q_heads)
+  int groups;                 // ceil(rows_per_token / kRows): warps a token quad needs
   int quads;                  // ceil(n_tokens / 4)
-  int step_quad, step_row;    // (warps in the grid) / and % rows_per_token
+  int step_quad, step_grp;    // (warps in the grid) / and % groups
   int32_t* status;
   // fused form only
   const __half* q;
@@ -82,140 +86,163 @@ __device__ __forceinline__ void norm8(float (&x)[8], float rrms, const uint4& w)
     x[2 * i + 1] = f.y;
   }
 }
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(d) : "f"(a), "f"(b));
+__device__ __forceinline__ uint32_t h2_abs_max_nan(uint32_t a, uint32_t b) {   // of non-negative a; b taken absolute
+  uint32_t d;
+  asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b & 0x7fff7fffu));
   return d;
 }
 
-// One group's share of a lane: its 8 elements -> a word of codes; the scale (fp16 bits) is the same in
-// the four lanes of the group.  Called by whole warps.
-__device__ __forceinline__ uint32_t quantise8(const float (&x)[8], uint32_t& scale_bits) {
-  float amax = fabsf(x[0]);
-#pragma unroll
-  for (int i = 1; i < 8; ++i) amax = max_nan(amax, fabsf(x[i]));
-  amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-  amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-  const bool fine = amax <= 65504.f;   // false for infinities and NaN
+// One group's share of a lane: its 8 elements (fp16 in `h`, 32-bit in `x`) -> a word of codes; the scale
+// (fp16 bits) is the same in the four lanes of the group.  Called by whole warps.
+__device__ __forceinline__ uint32_t quantise8(const uint4& h, const float (&x)[8], uint32_t& scale_bits) {
+  uint32_t m = h2_abs_max_nan(h2_abs_max_nan(h2_abs_max_nan(h.x & 0x7fff7fffu, h.y), h.z), h.w);
+  m = h2_abs_max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = h2_abs_max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const float2 mf = __half22float2(*reinterpret_cast<const __half2*>(&m));
+  const float amax = fmaxf(mf.x, mf.y);
+  const bool fine = mf.x <= 65504.f && mf.y <= 65504.f;   // false for infinities and NaN
   const __half sh = __float2half_rn(fminf(amax * (1.f / 7.f), kMaxScale));
   const float s = __half2float(sh);
   const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  uint32_t word = 0;
+  // floor(x / s + 8.5) is 1 .. 15 when s is a normal number (|x| / s <= 7 (1 + 2^-11)); only a subnormal s,
+  // rounded coarsely, can be exceeded by more, and then the sum is limited first.
+  float t[8];
+#pragma unroll
+  for (int n = 0; n < 8; ++n) t[n] = fmaf(x[n], inv, 8.5f + 1.f / 16384.f);
+  if (s < 6.104e-5f) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) t[n] = fminf(fmaxf(t[n], 0.f), 15.5f);
+  }
+  // Adding 2^23 rounding down leaves the floor in the low bits of 0x4B000000; the eight of them are shifted
+  // into place and added up, and the constant parts taken off (all but two are shifted out).
+  uint32_t word = 0u - 0x4B000000u - (0x4B000000u << 4);
 #pragma unroll
   for (int n = 0; n < 8; ++n) {
-    const float t = fminf(fmaxf(fmaf(x[n], inv, 8.5f + 1.f / 16384.f), 0.f), 15.5f);
-    const uint32_t u = __float_as_uint(__fadd_rd(t, 8388608.f));   // low bits: floor(t)
     const int shift = 4 * ((n >> 1) + 4 * (n & 1));
-    word |= (u << shift) & (15u << shift);
+    word += __float_as_uint(__fadd_rd(t[n], 8388608.f)) << shift;
   }
   scale_bits = fine ? static_cast<uint32_t>(__half_as_ushort(sh)) : 0x7E00u;   // NaN: never read as a number
   return fine ? word : 0x88888888u;
 }
 
-template <bool kFused>
+template <bool kFused, int kRows>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendParams p) {
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
   const int lane = threadIdx.x & 31;
   const int sub = lane & 7;
   const unsigned warp = (blockIdx.x * kThreads + threadIdx.x) >> 5;
-  int quad = static_cast<int>(warp / static_cast<unsigned>(p.rows_per_token));
-  int row = static_cast<int>(warp % static_cast<unsigned>(p.rows_per_token));
+  int quad = static_cast<int>(warp / static_cast<unsigned>(p.groups));
+  int grp = static_cast<int>(warp % static_cast<unsigned>(p.groups));
   while (quad < p.quads) {
     const int64_t tok = static_cast<int64_t>(quad) * kTokPerWarp + (lane >> 3);
     const bool live = tok < p.n_tokens;
-    // row of the warp: Q head, K head or V head (the same for all lanes)
-    const int kv_row = kFused ? row - p.q_heads : row;
-    const bool is_q = kFused && kv_row < 0;
-    const bool is_v = kv_row >= p.kv_heads;
-    uint4 ua = make_uint4(0, 0, 0, 0), ub = ua, uc = ua, us = ua;
+    const int row0 = grp * kRows;
+    // Rows q_heads .. of a token are its K heads, then its V heads; row < q_heads is a Q head.  The same
+    // for all lanes of the warp.
+    uint4 ua[kRows], ub[kRows], uc = make_uint4(0, 0, 0, 0), us = uc;
     int64_t slot = -1;
+#pragma unroll
+    for (int i = 0; i < kRows; ++i) {
+      ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
+      const int row = row0 + i;
+      if (live && row < p.rows_per_token) {
+        const int kv_row = kFused ? row - p.q_heads : row;
+        const __half* src;
+        if (kFused && kv_row < 0) src = p.q + tok * p.q_tok_stride + row * kD;
+        else if (kv_row >= p.kv_heads) src = p.v + tok * p.v_tok_stride + (kv_row - p.kv_heads) * kD;
+        else src = p.k + tok * p.k_tok_stride + kv_row * kD;
+        ua[i] = __ldg(reinterpret_cast<const uint4*>(src + sub * 8));
+        ub[i] = __ldg(reinterpret_cast<const uint4*>(src + kHalf + sub * 8));
+      }
+    }
     if (live) {
-      const __half* src;
-      if (is_q) src = p.q + tok * p.q_tok_stride + row * kD;
-      else if (is_v) src = p.v + tok * p.v_tok_stride + (kv_row - p.kv_heads) * kD;
-      else src = p.k + tok * p.k_tok_stride + kv_row * kD;
-      ua = __ldg(reinterpret_cast<const uint4*>(src + sub * 8));
-      ub = __ldg(reinterpret_cast<const uint4*>(src + kHalf + sub * 8));
-      if (kFused && !is_v) {
+      if (kFused && row0 < p.q_heads + p.kv_heads) {
         uc = __ldg(reinterpret_cast<const uint4*>(p.cos + tok * p.cs_tok_stride + sub * 8));
         us = __ldg(reinterpret_cast<const uint4*>(p.sin + tok * p.cs_tok_stride + sub * 8));
       }
-      if (!is_q) slot = __ldg(p.slots + tok);
+      if (!kFused || row0 + kRows > p.q_heads) slot = __ldg(p.slots + tok);
     }
-    float a[8], b[8];
-    unpack8(ua, a);
-    unpack8(ub, b);
-    if (kFused && !is_v) {
-      const __half* weight = is_q ? p.q_weight : p.k_weight;
-      if (weight != nullptr) {
-        const uint4 wa = __ldg(reinterpret_cast<const uint4*>(weight + sub * 8));
-        const uint4 wb = __ldg(reinterpret_cast<const uint4*>(weight + kHalf + sub * 8));
-        float mean;
-        if (is_q) {
-          float ss = 0.f;
+    const bool slot_ok = slot >= 0 && slot < p.pool_tokens;
+    const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
+    uint8_t* page = p.pool + (slot_ok ? slot / kv4::kPageTok : 0) * p.page_stride;
 #pragma unroll
-          for (int i = 0; i < 8; ++i) ss += a[i] * a[i] + b[i] * b[i];
-#pragma unroll
-          for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-          mean = ss * (1.f / kD);
-        } else {
-          double ss = 0.;
-#pragma unroll
-          for (int i = 0; i < 8; ++i)   // products of two fp16 numbers are exact in 32 bits
-            ss += static_cast<double>(a[i] * a[i]) + static_cast<double>(b[i] * b[i]);
-#pragma unroll
-          for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-          mean = static_cast<float>(ss * (1. / kD));
-        }
-        const float rrms = __fdiv_rn(1.f, __fsqrt_rn(mean + p.eps));
-        norm8(a, rrms, wa);
-        norm8(b, rrms, wb);
-      }
-      float c[8], s[8];
-      unpack8(uc, c);
-      unpack8(us, s);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {   // the products are exact, so each element is rounded once
-        const float x1 = a[i], x2 = b[i];
-        a[i] = x1 * c[i] - x2 * s[i];
-        b[i] = x2 * c[i] + x1 * s[i];
-      }
-      ua = pack8(a);
-      ub = pack8(b);
-    }
-    if (is_q) {
-      if (live) {
-        __half* dst = p.q_out + tok * p.q_out_tok_stride + row * kD;
-        *reinterpret_cast<uint4*>(dst + sub * 8) = ua;
-        *reinterpret_cast<uint4*>(dst + kHalf + sub * 8) = ub;
-      }
-    } else {
+    for (int i = 0; i < kRows; ++i) {
+      const int row = row0 + i;
+      if (row >= p.rows_per_token) break;
+      const int kv_row = kFused ? row - p.q_heads : row;
+      const bool is_q = kFused && kv_row < 0;
+      const bool is_v = kv_row >= p.kv_heads;
+      float a[8], b[8];
+      unpack8(ua[i], a);
+      unpack8(ub[i], b);
       if (kFused && !is_v) {
-        unpack8(ua, a);
-        unpack8(ub, b);
+        const __half* weight = is_q ? p.q_weight : p.k_weight;
+        if (weight != nullptr) {
+          const uint4 wa = __ldg(reinterpret_cast<const uint4*>(weight + sub * 8));
+          const uint4 wb = __ldg(reinterpret_cast<const uint4*>(weight + kHalf + sub * 8));
+          float mean;
+          if (is_q) {
+            float ss = 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
+#pragma unroll
+            for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            mean = ss * (1.f / kD);
+          } else {
+            double ss = 0.;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)   // products of two fp16 numbers are exact in 32 bits
+              ss += static_cast<double>(a[e] * a[e]) + static_cast<double>(b[e] * b[e]);
+#pragma unroll
+            for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            mean = static_cast<float>(ss * (1. / kD));
+          }
+          const float rrms = __fdiv_rn(1.f, __fsqrt_rn(mean + p.eps));
+          norm8(a, rrms, wa);
+          norm8(b, rrms, wb);
+        }
+        float c[8], s[8];
+        unpack8(uc, c);
+        unpack8(us, s);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {   // the products are exact, so each element is rounded once
+          const float x1 = a[e], x2 = b[e];
+          a[e] = x1 * c[e] - x2 * s[e];
+          b[e] = x2 * c[e] + x1 * s[e];
+        }
+        ua[i] = pack8(a);
+        ub[i] = pack8(b);
       }
-      uint32_t s1, s2;
-      const uint32_t w1 = quantise8(a, s1), w2 = quantise8(b, s2);   // groups sub / 4 and 2 + sub / 4
-      const uint32_t pw1 = __shfl_xor_sync(0xffffffffu, w1, 4), pw2 = __shfl_xor_sync(0xffffffffu, w2, 4);
-      const uint32_t ps = __shfl_xor_sync(0xffffffffu, s1 | (s2 << 16), 4);
-      if (live) {
-        if (slot < 0 || slot >= p.pool_tokens) {
-          set_status(p.status, B200KV_DEV_BAD_SLOT);
-        } else if (sub < 4) {
-          const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
-          uint8_t* block = p.pool + (slot / kv4::kPageTok) * p.page_stride + static_cast<int64_t>(kv_row) * kv4::kBlockBytes;
+      if (is_q) {
+        if (live) {
+          __half* dst = p.q_out + tok * p.q_out_tok_stride + row * kD;
+          *reinterpret_cast<uint4*>(dst + sub * 8) = ua[i];
+          *reinterpret_cast<uint4*>(dst + kHalf + sub * 8) = ub[i];
+        }
+      } else {
+        if (kFused && !is_v) {
+          unpack8(ua[i], a);
+          unpack8(ub[i], b);
+        }
+        uint32_t s1, s2;
+        const uint32_t w1 = quantise8(ua[i], a, s1), w2 = quantise8(ub[i], b, s2);   // groups sub / 4 and 2 + sub / 4
+        const uint32_t pw1 = __shfl_xor_sync(0xffffffffu, w1, 4), pw2 = __shfl_xor_sync(0xffffffffu, w2, 4);
+        const uint32_t ps = __shfl_xor_sync(0xffffffffu, s1 | (s2 << 16), 4);
+        if (slot_ok && sub < 4) {
+          uint8_t* block = page + kv_row * kv4::kBlockBytes;
           *reinterpret_cast<uint4*>(block + kv4::chunk_offset(t, sub)) = make_uint4(w1, pw1, w2, pw2);
           if (sub == 0)
             *reinterpret_cast<uint2*>(block + kv4::kScaleOffset + t * kv4::kScaleBytes) =
                 make_uint2(s1 | (ps << 16), s2 | (ps & 0xffff0000u));
         }
+        if (live && !slot_ok && sub == 0) set_status(p.status, B200KV_DEV_BAD_SLOT);
       }
     }
     quad += p.step_quad;
-    row += p.step_row;
-    if (row >= p.rows_per_token) {
-      row -= p.rows_per_token;
+    grp += p.step_grp;
+    if (grp >= p.groups) {
+      grp -= p.groups;
       ++quad;
     }
   }
@@ -223,8 +250,8 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendParams p) {
 
 // Read-back: four lanes to a row, a lane reads one 16-byte chunk (8 elements in each of the four
 // groups) and the row's four scales and writes four 16-byte pieces; the four lanes of a row write 64
-// contiguous bytes per store.  A warp takes one head row of eight neighbouring tokens.  HBM-bound: per
-// token 2 * KH * (72 + 256) B.
+// contiguous bytes per store.  A warp takes kRows head rows of eight neighbouring tokens, all loads in
+// flight first.  HBM-bound: per token 2 * KH * (72 + 256) B.
 struct GatherParams {
   const uint8_t* pool;
   int64_t pool_tokens, page_stride;
@@ -232,49 +259,61 @@ struct GatherParams {
   __half* out;
   int64_t out_tok_stride;
   int n, rows;
-  int octets, step_octet, step_row;
+  int octets, groups, step_octet, step_grp;
   int32_t* status;
 };
 
+template <int kRows>
 __global__ void __launch_bounds__(kThreads) kv4_gather_kernel(GatherParams p) {
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
   const int lane = threadIdx.x & 31;
   const int j = lane & 3;
   const unsigned warp = (blockIdx.x * kThreads + threadIdx.x) >> 5;
-  int octet = static_cast<int>(warp / static_cast<unsigned>(p.rows));
-  int row = static_cast<int>(warp % static_cast<unsigned>(p.rows));
+  int octet = static_cast<int>(warp / static_cast<unsigned>(p.groups));
+  int grp = static_cast<int>(warp % static_cast<unsigned>(p.groups));
   while (octet < p.octets) {
     const int64_t tok = static_cast<int64_t>(octet) * 8 + (lane >> 2);
     if (tok < p.n) {
+      const int row0 = grp * kRows;
       const int64_t slot = __ldg(p.slots + tok);
-      uint4 codes = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
-      uint2 scales = make_uint2(0, 0);
-      if (slot < 0 || slot >= p.pool_tokens) {
-        set_status(p.status, B200KV_DEV_BAD_SLOT);
-      } else {
-        const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
-        const uint8_t* block = kv4::block_at(p.pool, slot / kv4::kPageTok, p.page_stride, row);
-        codes = *reinterpret_cast<const uint4*>(block + kv4::chunk_offset(t, j));
-        scales = *reinterpret_cast<const uint2*>(block + kv4::kScaleOffset + t * kv4::kScaleBytes);
+      const bool ok = slot >= 0 && slot < p.pool_tokens;
+      if (!ok && j == 0) set_status(p.status, B200KV_DEV_BAD_SLOT);
+      const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
+      const uint8_t* block = kv4::block_at(p.pool, ok ? slot / kv4::kPageTok : 0, p.page_stride, row0);
+      uint4 codes[kRows];
+      uint2 scales[kRows];
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        codes[i] = make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u);
+        scales[i] = make_uint2(0, 0);
+        if (ok && row0 + i < p.rows) {
+          codes[i] = *reinterpret_cast<const uint4*>(block + i * kv4::kBlockBytes + kv4::chunk_offset(t, j));
+          scales[i] = *reinterpret_cast<const uint2*>(block + i * kv4::kBlockBytes + kv4::kScaleOffset + t * kv4::kScaleBytes);
+        }
       }
-      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
-      const uint32_t s2[4] = {__byte_perm(scales.x, 0, 0x1010), __byte_perm(scales.x, 0, 0x3232),
-                              __byte_perm(scales.y, 0, 0x1010), __byte_perm(scales.y, 0, 0x3232)};
-      __half* dst = p.out + tok * p.out_tok_stride + row * kD + 8 * j;
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        uint32_t v[4];
-        kv4::unpack_word(w[g], v);
+      for (int i = 0; i < kRows; ++i) {
+        if (row0 + i < p.rows) {
+          const uint32_t w[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
+          const uint32_t s2[4] = {__byte_perm(scales[i].x, 0, 0x1010), __byte_perm(scales[i].x, 0, 0x3232),
+                                  __byte_perm(scales[i].y, 0, 0x1010), __byte_perm(scales[i].y, 0, 0x3232)};
+          __half* dst = p.out + tok * p.out_tok_stride + (row0 + i) * kD + 8 * j;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = kv4::h2_mul(v[i], s2[g]);
-        *reinterpret_cast<uint4*>(dst + 32 * g) = make_uint4(v[0], v[1], v[2], v[3]);
+          for (int g = 0; g < 4; ++g) {
+            uint32_t v[4];
+            kv4::unpack_word(w[g], v);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = kv4::h2_mul(v[e], s2[g]);
+            *reinterpret_cast<uint4*>(dst + 32 * g) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
       }
     }
     octet += p.step_octet;
-    row += p.step_row;
-    if (row >= p.rows) {
-      row -= p.rows;
+    grp += p.step_grp;
+    if (grp >= p.groups) {
+      grp -= p.groups;
       ++octet;
     }
   }
@@ -311,17 +350,45 @@ int launch(Kernel kernel, const Params& p, unsigned blocks, cudaStream_t stream)
 
 constexpr int kCtasPerSm = 8;
 
-template <bool kFused>
-int launch_append(AppendParams p, cudaStream_t stream) {
-  p.rows_per_token = 2 * p.kv_heads + (kFused ? p.q_heads : 0);
-  p.quads = (p.n_tokens + kTokPerWarp - 1) / kTokPerWarp;
+// Rows per warp: four when that still gives every SM this many warps, one otherwise (a decode step's few
+// tokens: 3.8 against 4.3 us for four tokens of 16 + 16 rows and their read-back).
+constexpr int kWarpsForFour = 16;
+inline bool four_rows(int64_t token_groups, int rows, int sms) {
+  return token_groups * ((rows + 3) / 4) >= static_cast<int64_t>(sms) * kWarpsForFour;
+}
+
+template <bool kFused, int kRows>
+int launch_append_rows(AppendParams p, cudaStream_t stream) {
+  p.groups = (p.rows_per_token + kRows - 1) / kRows;
   unsigned blocks = 0;
-  const int rc = grid_for(static_cast<int64_t>(p.quads) * p.rows_per_token, kCtasPerSm, &blocks);
+  const int rc = grid_for(static_cast<int64_t>(p.quads) * p.groups, kCtasPerSm, &blocks);
   if (rc != B200KV_OK) return rc;
   const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
-  p.step_quad = static_cast<int>(warps / p.rows_per_token);
-  p.step_row = static_cast<int>(warps % p.rows_per_token);
-  return launch(kv4_append_kernel<kFused>, p, blocks, stream);
+  p.step_quad = static_cast<int>(warps / p.groups);
+  p.step_grp = static_cast<int>(warps % p.groups);
+  return launch(kv4_append_kernel<kFused, kRows>, p, blocks, stream);
+}
+
+template <bool kFused>
+int launch_append(AppendParams p, cudaStream_t stream) {
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200KV_ECUDA;
+  p.rows_per_token = 2 * p.kv_heads + (kFused ? p.q_heads : 0);
+  p.quads = (p.n_tokens + kTokPerWarp - 1) / kTokPerWarp;
+  return four_rows(p.quads, p.rows_per_token, sms) ? launch_append_rows<kFused, 4>(p, stream)
+                                                   : launch_append_rows<kFused, 1>(p, stream);
+}
+
+template <int kRows>
+int launch_gather(GatherParams p, cudaStream_t stream) {
+  p.groups = (p.rows + kRows - 1) / kRows;
+  unsigned blocks = 0;
+  const int rc = grid_for(static_cast<int64_t>(p.octets) * p.groups, kCtasPerSm, &blocks);
+  if (rc != B200KV_OK) return rc;
+  const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
+  p.step_octet = static_cast<int>(warps / p.groups);
+  p.step_grp = static_cast<int>(warps % p.groups);
+  return launch(kv4_gather_kernel<kRows>, p, blocks, stream);
 }
 
 }  // namespace
@@ -406,13 +473,9 @@ int kv4_gather(const void* pool, int64_t pool_pages, int64_t page_stride_bytes, 
   p.rows = 2 * kv_heads;
   p.octets = static_cast<int>((n + 7) / 8);
   p.status = status;
-  unsigned blocks = 0;
-  rc = grid_for(static_cast<int64_t>(p.octets) * p.rows, kCtasPerSm, &blocks);
-  if (rc != B200KV_OK) return rc;
-  const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
-  p.step_octet = static_cast<int>(warps / p.rows);
-  p.step_row = static_cast<int>(warps % p.rows);
-  return launch(kv4_gather_kernel, p, blocks, stream);
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200KV_ECUDA;
+  return four_rows(p.octets, p.rows, sms) ? launch_gather<4>(p, stream) : launch_gather<1>(p, stream);
 }
 
 }  // namespace b200kv
