@@ -17,7 +17,7 @@
 // 32-bit statistics: its rows are rounded once and nothing is decided by them.
 //
 // A warp takes kRows (one, or four where there are enough tokens to fill the GPU with them) head rows of
-// four neighbouring tokens, eight lanes to a row, all of its loads in flight before the first is used.
+// four neighbouring tokens, eight lanes to a row, the loads in flight before they are used.
 // A lane owns 8 elements of the first half of head_dim and the 8 they rotate with, i.e. one 32-bit word
 // of codes in each of two groups; the words of lanes l and l ^ 4 make up one 16-byte chunk of the row.
 // Four neighbouring tokens of a page are 256 contiguous bytes of codes and one 32-byte sector of scales.
@@ -47,7 +47,7 @@ struct AppendParams {
   int64_t pool_tokens, page_stride;
   int n_tokens, q_heads, kv_heads;
   int rows_per_token;         // head rows of a token: 2 * kv_heads (+ q_heads)
-  int groups;                 // ceil(rows_per_token / kRows): warps a token quad needs
+  int groups;                 // warps a token quad needs: rows_per_token / kRows, rounded up (fused: by kind of row)
   int quads;                  // ceil(n_tokens / 4)
   int step_quad, step_grp;    // (warps in the grid) / and % groups
   int32_t* status;
@@ -72,18 +72,31 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
     x[2 * i + 1] = f.y;
   }
 }
-__device__ __forceinline__ uint4 pack8(const float (&x)[8]) {
-  return make_uint4(pack_half2(x[0], x[1]), pack_half2(x[2], x[3]), pack_half2(x[4], x[5]), pack_half2(x[6], x[7]));
+// c + a * b of the low (high) halves, the product exact, one rounding to 32 bits.
+__device__ __forceinline__ float fma_lo(uint32_t a, uint32_t b, float c) {
+  float d;
+  asm("{\n\t.reg .b16 al, ah, bl, bh;\n\tmov.b32 {al, ah}, %1;\n\tmov.b32 {bl, bh}, %2;\n\t"
+      "fma.rn.f32.f16 %0, al, bl, %3;\n\t}\n" : "=f"(d) : "r"(a), "r"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float fma_hi(uint32_t a, uint32_t b, float c) {
+  float d;
+  asm("{\n\t.reg .b16 al, ah, bl, bh;\n\tmov.b32 {al, ah}, %1;\n\tmov.b32 {bl, bh}, %2;\n\t"
+      "fma.rn.f32.f16 %0, ah, bh, %3;\n\t}\n" : "=f"(d) : "r"(a), "r"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ void words(const uint4& u, uint32_t (&w)[4]) {
+  w[0] = u.x;
+  w[1] = u.y;
+  w[2] = u.z;
+  w[3] = u.w;
 }
 // x * rrms rounded to fp16, times the fp16 weight in fp16 (the reference's roundings, qk_prologue.cu).
-__device__ __forceinline__ void norm8(float (&x)[8], float rrms, const uint4& w) {
-  const uint32_t wp[4] = {w.x, w.y, w.z, w.w};
+__device__ __forceinline__ void norm8(uint32_t (&x)[4], float rrms, const uint32_t (&w)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const __half2 y = __floats2half2_rn(x[2 * i] * rrms, x[2 * i + 1] * rrms);
-    const float2 f = __half22float2(__hmul2(y, *reinterpret_cast<const __half2*>(&wp[i])));
-    x[2 * i] = f.x;
-    x[2 * i + 1] = f.y;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x[i]));
+    x[i] = kv4::h2_mul(pack_half2(f.x * rrms, f.y * rrms), w[i]);
   }
 }
 __device__ __forceinline__ uint32_t h2_abs_max_nan(uint32_t a, uint32_t b) {   // of non-negative a; b taken absolute
@@ -125,7 +138,23 @@ __device__ __forceinline__ uint32_t quantise8(const uint4& h, const float (&x)[8
   return fine ? word : 0x88888888u;
 }
 
-template <bool kFused, int kRows>
+// The codes and scales of four rows (eight lanes each) of one head row to their places: lane `sub` of a row
+// holds the words of groups sub / 4 and 2 + sub / 4, lane sub ^ 4 the others of the same chunk.
+__device__ __forceinline__ void store_row(const uint4& ha, const uint4& hb, const float (&a)[8], const float (&b)[8],
+                                          int sub, bool slot_ok, uint8_t* block, int t) {
+  uint32_t s1, s2;
+  const uint32_t w1 = quantise8(ha, a, s1), w2 = quantise8(hb, b, s2);
+  const uint32_t pw1 = __shfl_xor_sync(0xffffffffu, w1, 4), pw2 = __shfl_xor_sync(0xffffffffu, w2, 4);
+  const uint32_t ps = __shfl_xor_sync(0xffffffffu, s1 | (s2 << 16), 4);
+  if (slot_ok && sub < 4) {
+    *reinterpret_cast<uint4*>(block + kv4::chunk_offset(t, sub)) = make_uint4(w1, pw1, w2, pw2);
+    if (sub == 0)
+      *reinterpret_cast<uint2*>(block + kv4::kScaleOffset + t * kv4::kScaleBytes) =
+          make_uint2(s1 | (ps << 16), s2 | (ps & 0xffff0000u));
+  }
+}
+
+template <int kRows>
 __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendParams p) {
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
@@ -138,105 +167,181 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendParams p) {
     const int64_t tok = static_cast<int64_t>(quad) * kTokPerWarp + (lane >> 3);
     const bool live = tok < p.n_tokens;
     const int row0 = grp * kRows;
-    // Rows q_heads .. of a token are its K heads, then its V heads; row < q_heads is a Q head.  The same
-    // for all lanes of the warp.
-    uint4 ua[kRows], ub[kRows], uc = make_uint4(0, 0, 0, 0), us = uc;
+    uint4 ua[kRows], ub[kRows];
     int64_t slot = -1;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
       ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
-      const int row = row0 + i;
+      const int row = row0 + i;   // K heads, then V heads
       if (live && row < p.rows_per_token) {
-        const int kv_row = kFused ? row - p.q_heads : row;
-        const __half* src;
-        if (kFused && kv_row < 0) src = p.q + tok * p.q_tok_stride + row * kD;
-        else if (kv_row >= p.kv_heads) src = p.v + tok * p.v_tok_stride + (kv_row - p.kv_heads) * kD;
-        else src = p.k + tok * p.k_tok_stride + kv_row * kD;
+        const __half* src = row >= p.kv_heads ? p.v + tok * p.v_tok_stride + (row - p.kv_heads) * kD
+                                              : p.k + tok * p.k_tok_stride + row * kD;
         ua[i] = __ldg(reinterpret_cast<const uint4*>(src + sub * 8));
         ub[i] = __ldg(reinterpret_cast<const uint4*>(src + kHalf + sub * 8));
       }
     }
-    if (live) {
-      if (kFused && row0 < p.q_heads + p.kv_heads) {
-        uc = __ldg(reinterpret_cast<const uint4*>(p.cos + tok * p.cs_tok_stride + sub * 8));
-        us = __ldg(reinterpret_cast<const uint4*>(p.sin + tok * p.cs_tok_stride + sub * 8));
-      }
-      if (!kFused || row0 + kRows > p.q_heads) slot = __ldg(p.slots + tok);
-    }
+    if (live) slot = __ldg(p.slots + tok);
     const bool slot_ok = slot >= 0 && slot < p.pool_tokens;
+    if (live && !slot_ok && sub == 0) set_status(p.status, B200KV_DEV_BAD_SLOT);
     const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
     uint8_t* page = p.pool + (slot_ok ? slot / kv4::kPageTok : 0) * p.page_stride;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      const int row = row0 + i;
-      if (row >= p.rows_per_token) break;
-      const int kv_row = kFused ? row - p.q_heads : row;
-      const bool is_q = kFused && kv_row < 0;
-      const bool is_v = kv_row >= p.kv_heads;
+      if (row0 + i >= p.rows_per_token) break;
       float a[8], b[8];
       unpack8(ua[i], a);
       unpack8(ub[i], b);
-      if (kFused && !is_v) {
-        const __half* weight = is_q ? p.q_weight : p.k_weight;
-        if (weight != nullptr) {
-          const uint4 wa = __ldg(reinterpret_cast<const uint4*>(weight + sub * 8));
-          const uint4 wb = __ldg(reinterpret_cast<const uint4*>(weight + kHalf + sub * 8));
-          float mean;
-          if (is_q) {
-            float ss = 0.f;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) ss += a[e] * a[e] + b[e] * b[e];
-#pragma unroll
-            for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            mean = ss * (1.f / kD);
-          } else {
-            double ss = 0.;
-#pragma unroll
-            for (int e = 0; e < 8; ++e)   // products of two fp16 numbers are exact in 32 bits
-              ss += static_cast<double>(a[e] * a[e]) + static_cast<double>(b[e] * b[e]);
-#pragma unroll
-            for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-            mean = static_cast<float>(ss * (1. / kD));
-          }
-          const float rrms = __fdiv_rn(1.f, __fsqrt_rn(mean + p.eps));
-          norm8(a, rrms, wa);
-          norm8(b, rrms, wb);
-        }
-        float c[8], s[8];
-        unpack8(uc, c);
-        unpack8(us, s);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {   // the products are exact, so each element is rounded once
-          const float x1 = a[e], x2 = b[e];
-          a[e] = x1 * c[e] - x2 * s[e];
-          b[e] = x2 * c[e] + x1 * s[e];
-        }
-        ua[i] = pack8(a);
-        ub[i] = pack8(b);
+      store_row(ua[i], ub[i], a, b, sub, slot_ok, page + (row0 + i) * kv4::kBlockBytes, t);
+    }
+    quad += p.step_quad;
+    grp += p.step_grp;
+    if (grp >= p.groups) {
+      grp -= p.groups;
+      ++quad;
+    }
+  }
+}
+
+// The fused form.  A warp's rows are all Q, all K or all V heads of its four tokens (a row kind has a body
+// of its own and the loops are not unrolled: the kernel has to stay inside the instruction cache), and
+// the next row is on its way while one is worked on.
+template <int kRows>
+__global__ void __launch_bounds__(kThreads, 4) kv4_prologue_kernel(AppendParams p) {
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+  const int lane = threadIdx.x & 31;
+  const int sub = lane & 7;
+  const unsigned warp = (blockIdx.x * kThreads + threadIdx.x) >> 5;
+  int quad = static_cast<int>(warp / static_cast<unsigned>(p.groups));
+  int grp = static_cast<int>(warp % static_cast<unsigned>(p.groups));
+  const int q_groups = (p.q_heads + kRows - 1) / kRows, kv_groups = (p.kv_heads + kRows - 1) / kRows;
+  while (quad < p.quads) {
+    const int64_t tok = static_cast<int64_t>(quad) * kTokPerWarp + (lane >> 3);
+    const bool live = tok < p.n_tokens;
+    const bool is_q = grp < q_groups;
+    const bool is_v = grp >= q_groups + kv_groups;
+    const int row0 = (is_q ? grp : is_v ? grp - q_groups - kv_groups : grp - q_groups) * kRows;   // head of its kind
+    const int rows = min(kRows, (is_q ? p.q_heads : p.kv_heads) - row0);
+    const __half* src = (is_q ? p.q + tok * p.q_tok_stride : (is_v ? p.v + tok * p.v_tok_stride : p.k + tok * p.k_tok_stride)) +
+                        row0 * kD + sub * 8;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    uint4 na = zero, nb = zero;
+    if (live) {
+      na = __ldg(reinterpret_cast<const uint4*>(src));
+      nb = __ldg(reinterpret_cast<const uint4*>(src + kHalf));
+    }
+    auto next_row = [&](int i, uint4& ha, uint4& hb) {   // hands row i out and requests row i + 1
+      ha = na;
+      hb = nb;
+      if (live && i + 1 < rows) {
+        src += kD;
+        na = __ldg(reinterpret_cast<const uint4*>(src));
+        nb = __ldg(reinterpret_cast<const uint4*>(src + kHalf));
       }
-      if (is_q) {
+    };
+    int64_t slot = -1;
+    if (live && !is_q) slot = __ldg(p.slots + tok);
+    const bool slot_ok = slot >= 0 && slot < p.pool_tokens;
+    if (live && !is_q && !slot_ok && sub == 0) set_status(p.status, B200KV_DEV_BAD_SLOT);
+    const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
+    uint8_t* block = p.pool + (slot_ok ? slot / kv4::kPageTok : 0) * p.page_stride +
+                     ((is_v ? p.kv_heads : 0) + row0) * kv4::kBlockBytes;
+    if (is_v) {
+#pragma unroll 1
+      for (int i = 0; i < rows; ++i, block += kv4::kBlockBytes) {
+        uint4 ha, hb;
+        next_row(i, ha, hb);
+        float a[8], b[8];
+        unpack8(ha, a);
+        unpack8(hb, b);
+        store_row(ha, hb, a, b, sub, slot_ok, block, t);
+      }
+    } else {
+      uint32_t c[4], sn[4], neg[4];   // cos, sin and -sin of the token, for all of the warp's rows
+      {
+        uint4 uc = zero, us = zero;
         if (live) {
-          __half* dst = p.q_out + tok * p.q_out_tok_stride + row * kD;
-          *reinterpret_cast<uint4*>(dst + sub * 8) = ua[i];
-          *reinterpret_cast<uint4*>(dst + kHalf + sub * 8) = ub[i];
+          uc = __ldg(reinterpret_cast<const uint4*>(p.cos + tok * p.cs_tok_stride + sub * 8));
+          us = __ldg(reinterpret_cast<const uint4*>(p.sin + tok * p.cs_tok_stride + sub * 8));
+        }
+        words(uc, c);
+        words(us, sn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) neg[i] = sn[i] ^ 0x80008000u;
+      }
+      const __half* weight = is_q ? p.q_weight : p.k_weight;
+      uint32_t wa[4] = {}, wb[4] = {};
+      if (weight != nullptr) {
+        words(__ldg(reinterpret_cast<const uint4*>(weight + sub * 8)), wa);
+        words(__ldg(reinterpret_cast<const uint4*>(weight + kHalf + sub * 8)), wb);
+      }
+      // Products of fp16 numbers are exact in 32 bits, so each rotated element is rounded once there and
+      // once to fp16.
+      auto rotate = [&](const uint32_t (&a)[4], const uint32_t (&b)[4], uint4& ha, uint4& hb) {
+        uint32_t x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = pack_half2(fma_lo(a[i], c[i], fma_lo(b[i], neg[i], 0.f)), fma_hi(a[i], c[i], fma_hi(b[i], neg[i], 0.f)));
+          y[i] = pack_half2(fma_lo(b[i], c[i], fma_lo(a[i], sn[i], 0.f)), fma_hi(b[i], c[i], fma_hi(a[i], sn[i], 0.f)));
+        }
+        ha = make_uint4(x[0], x[1], x[2], x[3]);
+        hb = make_uint4(y[0], y[1], y[2], y[3]);
+      };
+      if (is_q) {
+        __half* dst = p.q_out + tok * p.q_out_tok_stride + row0 * kD + sub * 8;
+#pragma unroll 1
+        for (int i = 0; i < rows; ++i, dst += kD) {
+          uint4 ha, hb;
+          next_row(i, ha, hb);
+          uint32_t a[4], b[4];
+          words(ha, a);
+          words(hb, b);
+          if (weight != nullptr) {
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s0 = fma_lo(a[e], a[e], fma_lo(b[e], b[e], s0));
+              s1 = fma_hi(a[e], a[e], fma_hi(b[e], b[e], s1));
+            }
+            float ss = s0 + s1;
+#pragma unroll
+            for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            const float rrms = rsqrtf(ss * (1.f / kD) + p.eps);
+            norm8(a, rrms, wa);
+            norm8(b, rrms, wb);
+          }
+          rotate(a, b, ha, hb);
+          if (live) {
+            *reinterpret_cast<uint4*>(dst) = ha;
+            *reinterpret_cast<uint4*>(dst + kHalf) = hb;
+          }
         }
       } else {
-        if (kFused && !is_v) {
-          unpack8(ua[i], a);
-          unpack8(ub[i], b);
+#pragma unroll 1
+        for (int i = 0; i < rows; ++i, block += kv4::kBlockBytes) {
+          uint4 ha, hb;
+          next_row(i, ha, hb);
+          uint32_t a[4], b[4];
+          words(ha, a);
+          words(hb, b);
+          if (weight != nullptr) {
+            double ss = 0.;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              ss += (static_cast<double>(fma_lo(a[e], a[e], 0.f)) + static_cast<double>(fma_hi(a[e], a[e], 0.f))) +
+                    (static_cast<double>(fma_lo(b[e], b[e], 0.f)) + static_cast<double>(fma_hi(b[e], b[e], 0.f)));
+#pragma unroll
+            for (int m = 1; m < 8; m <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+            const float rrms = __fdiv_rn(1.f, __fsqrt_rn(static_cast<float>(ss * (1. / kD)) + p.eps));
+            norm8(a, rrms, wa);
+            norm8(b, rrms, wb);
+          }
+          rotate(a, b, ha, hb);
+          float x[8], y[8];
+          unpack8(ha, x);
+          unpack8(hb, y);
+          store_row(ha, hb, x, y, sub, slot_ok, block, t);
         }
-        uint32_t s1, s2;
-        const uint32_t w1 = quantise8(ua[i], a, s1), w2 = quantise8(ub[i], b, s2);   // groups sub / 4 and 2 + sub / 4
-        const uint32_t pw1 = __shfl_xor_sync(0xffffffffu, w1, 4), pw2 = __shfl_xor_sync(0xffffffffu, w2, 4);
-        const uint32_t ps = __shfl_xor_sync(0xffffffffu, s1 | (s2 << 16), 4);
-        if (slot_ok && sub < 4) {
-          uint8_t* block = page + kv_row * kv4::kBlockBytes;
-          *reinterpret_cast<uint4*>(block + kv4::chunk_offset(t, sub)) = make_uint4(w1, pw1, w2, pw2);
-          if (sub == 0)
-            *reinterpret_cast<uint2*>(block + kv4::kScaleOffset + t * kv4::kScaleBytes) =
-                make_uint2(s1 | (ps << 16), s2 | (ps & 0xffff0000u));
-        }
-        if (live && !slot_ok && sub == 0) set_status(p.status, B200KV_DEV_BAD_SLOT);
       }
     }
     quad += p.step_quad;
@@ -359,14 +464,16 @@ inline bool four_rows(int64_t token_groups, int rows, int sms) {
 
 template <bool kFused, int kRows>
 int launch_append_rows(AppendParams p, cudaStream_t stream) {
-  p.groups = (p.rows_per_token + kRows - 1) / kRows;
+  p.groups = kFused ? (p.q_heads + kRows - 1) / kRows + 2 * ((p.kv_heads + kRows - 1) / kRows)
+                    : (p.rows_per_token + kRows - 1) / kRows;
   unsigned blocks = 0;
   const int rc = grid_for(static_cast<int64_t>(p.quads) * p.groups, kCtasPerSm, &blocks);
   if (rc != B200KV_OK) return rc;
   const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
   p.step_quad = static_cast<int>(warps / p.groups);
   p.step_grp = static_cast<int>(warps % p.groups);
-  return launch(kv4_append_kernel<kFused, kRows>, p, blocks, stream);
+  if (kFused) return launch(kv4_prologue_kernel<kRows>, p, blocks, stream);
+  return launch(kv4_append_kernel<kRows>, p, blocks, stream);
 }
 
 template <bool kFused>
