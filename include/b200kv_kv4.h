@@ -94,6 +94,12 @@ int b200kv_stream_capture_id(void* stream, uint64_t* id);
 size_t b200kv_kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim);
 
 /*
+ * Bytes of scratch with which b200kv_kv4_paged_prefill streams chunks of at most max_q_len rows; 0 where
+ * it would not (max_q_len * q_heads / kv_heads above 128, batch above 4096, or bad input).
+ */
+size_t b200kv_kv4_chunk_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads, int head_dim);
+
+/*
  * Paged flash-decoding over a kv4 pool: arguments, limits and meaning as for b200kv_paged_decode, with
  * the pool given as base, pages and page stride.  A token table's entries at page starts must be
  * multiples of 16; one that is not, or a page outside the pool, sets B200KV_DEV_BAD_PAGE and page 0 is
@@ -115,8 +121,13 @@ int b200kv_kv4_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_
 /*
  * Packed causal prefill with history over a kv4 pool: arguments and meaning as for
  * b200kv_paged_prefill (the chunk's own rows are already in the pool), table kinds BLOCK and TOKEN.
- * Lengths, rows and tables may come from the kernel launched immediately before.  A K or V group that
- * reads as NaN reaches the rows that see its token and no others.
+ * Lengths, rows and tables may come from the kernel launched immediately before.  A request whose chunk
+ * is longer than max_q_len is skipped (B200KV_DEV_BAD_LENGTH).  A K or V group that reads as NaN reaches
+ * the rows that see its token and no others.
+ *   workspace  NULL, or scratch of b200kv_kv4_chunk_workspace_bytes() bytes under the rules of the decode
+ *              workspace (the same buffer may serve both): chunks of a few rows -- drafted tokens, the end
+ *              of a prompt -- are then streamed like a decode step instead of filling a small part of
+ *              128-row tiles.  Then q is 16-byte aligned with strides that are multiples of 8
  */
 int b200kv_kv4_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                              const void* pool, int64_t pool_pages, int64_t page_stride_bytes,
@@ -128,6 +139,7 @@ int b200kv_kv4_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride
                              int q_heads, int kv_heads, int head_dim, int page_size,
                              float scale_log2,
                              void* out, int64_t out_stride_t, int64_t out_stride_h,
+                             void* workspace, size_t workspace_bytes,
                              int32_t* status, void* stream);
 
 #ifdef __cplusplus

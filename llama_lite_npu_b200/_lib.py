@@ -125,6 +125,7 @@ _SIGNATURES = {
     ),
     "b200kv_stream_capture_id": (c_int, [c_void_p, c_void_p]),
     "b200kv_kv4_decode_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "b200kv_kv4_chunk_workspace_bytes": (c_size_t, [c_int, c_int64, c_int, c_int, c_int]),
     "b200kv_kv4_paged_decode": (
         c_int,
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,    # q, pool
@@ -138,7 +139,7 @@ _SIGNATURES = {
         [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_int64,
          c_void_p, c_int64, c_int, c_int, c_int64, c_void_p, c_void_p,
          c_void_p, c_void_p, c_int, c_int, c_int64, c_int64,
-         c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_void_p, c_void_p],
+         c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p],
     ),
     # host-side prefix cache (include/b200kv_prefix_cache.h)
     "b200kv_prefix_cache_create": (c_void_p, [c_int, c_int64, c_int64]),

@@ -384,6 +384,10 @@ size_t b200kv_kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, i
   return b200kv::kv4_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim);
 }
 
+size_t b200kv_kv4_chunk_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads, int head_dim) {
+  return b200kv::kv4_chunk_workspace_bytes(batch, max_q_len, q_heads, kv_heads, head_dim);
+}
+
 int b200kv_kv4_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* pool,
                             int64_t pool_pages, int64_t page_stride_bytes, const int32_t* table,
                             int64_t table_row_stride, int table_kind, int table_rows, int64_t table_cols,
@@ -430,8 +434,11 @@ int b200kv_kv4_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride
                              const int32_t* req_ids, const int32_t* q_start, const void* ctx_lens,
                              const void* q_lens, int lens_i64, int batch, int64_t total_q, int64_t max_q_len,
                              int q_heads, int kv_heads, int head_dim, int page_size, float scale_log2, void* out,
-                             int64_t out_stride_t, int64_t out_stride_h, int32_t* status, void* stream) {
+                             int64_t out_stride_t, int64_t out_stride_h, void* workspace, size_t workspace_bytes,
+                             int32_t* status, void* stream) {
   b200kv::Kv4PrefillArgs a{};
+  a.workspace = workspace;
+  a.workspace_bytes = workspace_bytes;
   a.pool = pool;
   a.pool_pages = pool_pages;
   a.page_stride_bytes = page_stride_bytes;

@@ -1,17 +1,19 @@
-// Paged flash-decoding over the 4-bit cache (format: include/b200kv_kv4.h), one launch.
+// Paged flash-decoding over the 4-bit cache (format: include/b200kv_kv4.h), one launch; also the short
+// chunks of a packed prefill, whose few query rows would fill a small part of a tensor-core tile.
 //
-// The page line, its cut into teams and the merge of the partials are those of paged_decode.cu
-// (decode_plan.cuh): a CTA owns one KV head over a contiguous range of pages and serves the head's
-// whole query group from one pass over them.  What differs is a warp's work on a page:
+// Queries are columns: column c of a request is query token c / G and head c % G of a KV head's group of G
+// (a decode step has one token).  A CTA serves ROWS (8 or 16) columns of one KV head in one pass over a
+// contiguous range of pages:
 //
-//   S^T[tok, head] = sum_g s_K[tok, g] * (C_K[tok, d in g] . Q^T[d in g, head])
-//   O^T[d, head]  += C_V^T[d, tok] . (P^T[tok, head] * s_V[tok, g(d)])
+//   S^T[tok, col] = sum_g s_K[tok, g] * (C_K[tok, d in g] . Q^T[d in g, col])
+//   O^T[d, col]  += C_V^T[d, tok] . (P^T[tok, col] * s_V[tok, g(d)])
 //
 // with C the codes minus 8, integers that fp16 holds exactly.  No element is ever multiplied by its
 // scale: K's scales multiply the four partial scores of a token in 32 bits, V's scales go into P,
-// where 16 tokens meet 8 heads instead of 128 elements.  A code costs 9/8 of an instruction (one
+// where 16 tokens meet 8 columns instead of 128 elements.  A code costs 9/8 of an instruction (one
 // logical operation and one packed add per pair, a shift per word) on its way to mma.sync m16n8k16
-// (fp16 in, fp32 accumulate; tokens or head_dim are the M rows, the query heads the N columns).
+// (fp16 in, fp32 accumulate; tokens or head_dim are the M rows, the columns N): tcgen05 would want
+// the codes as fp16 in shared memory first, and 64 rows to work on.
 //
 // P * s_V is an fp16 operand, so its range matters.  P = 2^(score - m) with a reference m that is kept
 // about 2^7 under the running maximum (it cancels between O and the sum of P): P is at most 2^14 and
@@ -19,6 +21,13 @@
 // exceed that.  V scales of 2 and more (values of 14 and more) lower the bound on P accordingly.  A
 // product loses bits only below 2^-14, i.e. where it is 2^-21 of the largest weight times one scale unit;
 // the absolute error of such a token, 2^-25 * 2^-7 * 8 per code, is far under half a step of the output.
+//
+// Scheduling.  All sequences' pages are laid end to end and measured in units (pages, plus kPieceCost per
+// non-empty sequence: ending a piece costs about that many pages of streaming); team i of kv_heads x
+// column-block CTAs takes the i-th equal part.  A part holds tails, whole sequences and heads of sequences
+// ("pieces"); a piece that is a whole sequence yields final rows, any other a partial that the CTA which
+// arrives last combines.  The plan is made by every CTA from the lengths (one load per sequence and two
+// scans), so nothing is synchronised with the host and a captured launch replays with new lengths.
 //
 // A warp streams its own pages: page k of a piece belongs to warp k % 4, two of them make up one step
 // (one wait, one look at the maxima, one request, and twice the independent arithmetic in flight).  Every
@@ -30,8 +39,9 @@
 // entries ahead of use.
 //
 // Bytes per token and KV head: 2 * 72 (a page is 2304 B where fp16 has 8192).
+#include <climits>
+
 #include "common.cuh"
-#include "decode_plan.cuh"
 #include "kv4.cuh"
 #include "launch.h"
 
@@ -39,28 +49,104 @@ namespace b200kv {
 
 namespace {
 
-constexpr int kThreads = kConsumerThreads;
+constexpr int kD = kv4::kHeadDim;
+constexpr int kPS = kv4::kPageTok;
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
 constexpr int kStages = 2;
 constexpr int kPageBytes = 2 * kv4::kBlockBytes;   // K and V block of one page of one head
 constexpr int kPairBytes = 2 * kPageBytes;
-constexpr int kRingBytes = kConsumerWarps * kStages * kPairBytes;
+constexpr int kRingBytes = kWarps * kStages * kPairBytes;
+constexpr int kMinPagesPerTeam = 4;                // a team is not worth launching for fewer pages
+constexpr int kPieceCost = 16;
 // Resident CTAs per SM.  Three of them leave 168 registers, which a step of two pages needs (four spill
 // and were slower: 36.4 against 33.0 us on 32 sequences of 1-4 k tokens, 64/8 heads).
 constexpr int ctas_per_sm(int rows) { return rows == 8 ? 3 : 2; }
-constexpr int kSeqCache = kThreads;                // lengths and table rows kept in shared memory
-constexpr int kDefaultPieceCost = 16;
-static_assert(kPS == kv4::kPageTok && kD == kv4::kHeadDim, "one geometry");
+constexpr size_t kCounterBytes = B200KV_DECODE_COUNTER_BYTES;
+constexpr int64_t kMaxCounters = static_cast<int64_t>(kCounterBytes / sizeof(unsigned));
 
-struct Kv4DecodeParams : DecodePlan {
+struct Kv4Params {
   const __half* q;
-  int64_t q_stride_b, q_stride_h;
+  int64_t q_stride_t, q_stride_h;
   const uint8_t* pool;
-  int64_t pool_pages, page_stride;
+  int pool_pages;
+  int64_t page_stride;
   const int32_t* table;
   int64_t table_row_stride;
-  int table_kind;
+  int table_kind, table_rows;
+  const int32_t* row_ids;
+  // Decode: lens are the sequences' lengths, sequence b has query row b.  Chunk (q_lens != nullptr): lens are the
+  // contexts, request b has query rows q_start[b] .. + q_lens[b], of which the last sees everything.
+  const void* lens;
+  const void* q_lens;
+  const int32_t* q_start;
+  int lens_i64;
+  int batch, kv_heads, group;
+  int blocks;               // column blocks of ROWS columns
+  int max_seq_len;          // decode: bound of the lengths; chunk: positions a table row can name
+  int max_q_len;
+  int64_t total_q;
+  int nteams;
   float scale_log2;
+  float4* part_o;           // [nteams + batch][kv_heads][blocks][8 * NB][32] O^T fragments
+  float2* part_ml;          // [nteams + batch][kv_heads][blocks][ROWS] (m, l)
+  unsigned* piece_ctr;      // [batch][kv_heads][blocks], zero between launches
+  __half* out;
+  int64_t out_stride_t, out_stride_h;
+  int32_t* status;
 };
+
+// What every part of the kernel takes a sequence to be.  A table row that does not exist, or a length or
+// chunk out of bounds, is reported and never turns into an address: a decode length is limited, anything
+// else makes the sequence empty.
+struct Seq {
+  int len, row, ql;
+};
+template <bool kChunk>
+__device__ __forceinline__ Seq seq_of(const Kv4Params& p, int b) {
+  Seq s;
+  s.row = p.row_ids ? __ldg(p.row_ids + b) : b;
+  int64_t len = load_len(p.lens, p.lens_i64, b);
+  bool bad = s.row < 0 || s.row >= p.table_rows || len < 0;
+  int64_t ql = 1;
+  if (kChunk) {
+    ql = load_len(p.q_lens, p.lens_i64, b);
+    const int64_t start = __ldg(p.q_start + b);
+    bad = bad || ql < 0 || ql > p.max_q_len || len > p.max_seq_len || len + ql > p.max_seq_len || start < 0 ||
+          start + ql > p.total_q;
+    len = ql > 0 ? len + ql : 0;
+  }
+  if (bad || len > p.max_seq_len) {
+    set_status(p.status, B200KV_DEV_BAD_LENGTH);
+    len = bad ? 0 : p.max_seq_len;
+  }
+  s.len = static_cast<int>(len);
+  s.ql = static_cast<int>(ql);
+  return s;
+}
+__device__ __forceinline__ int pages_of(int len) { return (len + kPS - 1) / kPS; }
+
+// a * b / c for 0 <= a, b, c < 2^31 (a 64-bit division only where it takes one).
+__device__ __forceinline__ int mul_div(int a, int b, int c) {
+  const uint64_t m = static_cast<uint64_t>(static_cast<uint32_t>(a)) * static_cast<uint32_t>(b);
+  if (m >> 32) return static_cast<int>(m / static_cast<uint32_t>(c));
+  return static_cast<int>(static_cast<uint32_t>(m) / static_cast<uint32_t>(c));
+}
+// Team whose part of `total` units holds unit x.
+__device__ __forceinline__ int team_of(int x, int nteams, int total) {
+  const uint64_t m = static_cast<uint64_t>(x + 1) * static_cast<uint32_t>(nteams) - 1;
+  if (m >> 32) return static_cast<int>(m / static_cast<uint32_t>(total));
+  return static_cast<int>(static_cast<uint32_t>(m) / static_cast<uint32_t>(total));
+}
+
+__device__ __forceinline__ void cta_bar() { __syncthreads(); }
+
+// Programmatic dependent launch: what comes before this call may overlap the tail of the previous kernel
+// and reads launch metadata only (lengths, rows, page table); every thread makes the call on every path.
+__device__ __forceinline__ void pdl_wait_then_trigger() {
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
+}
 
 __device__ __forceinline__ void async_copy16(uint32_t dst, const void* src, uint64_t policy) {
   asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;\n" : : "r"(dst), "l"(src), "l"(policy) : "memory");
@@ -93,64 +179,211 @@ __device__ __forceinline__ uint32_t h2_max(uint32_t a, uint32_t b) {
   return d;
 }
 
-// A piece: the part of one sequence that lies in the team's range.
+// A team's part of the page line.
+struct TeamRange {
+  int b, page, kseq, flat;   // first sequence, its first page, non-empty sequences before it, flat page position
+  int end;                   // flat page position of the end
+  int units_total, nteams;
+  bool any_empty, any;
+};
+struct PlanScratch {
+  int4 sums[kWarps];         // units, non-empty sequences, fewest and most pages of one
+  int2 scan[kWarps];
+  int4 found[2];             // sequence, page, flat position, kseq at the part's begin and end
+};
+// Lengths, rows and query rows of kThreads sequences from `first` on.
+struct SeqCache {
+  int len[kThreads], row[kThreads], ql[kThreads];
+};
+
+// Where is this team's part?  Called by the whole CTA (it holds barriers).
+template <bool kChunk>
+__device__ __forceinline__ TeamRange plan_team_range(const Kv4Params& p, int team, int tid, PlanScratch& sc, SeqCache& cache,
+                                                     int& cache_first) {
+  const int lane = tid & 31, warp = tid >> 5;
+  int units = 0, cnt = 0, lo = INT_MAX, hi = 0, own_np = 0;
+  for (int b = tid; b < p.batch; b += kThreads) {
+    const Seq s = seq_of<kChunk>(p, b);
+    const int np = pages_of(s.len);
+    if (b == tid) {
+      own_np = np;
+      cache.len[tid] = s.len;
+      cache.row[tid] = s.row;
+      cache.ql[tid] = s.ql;
+    }
+    if (np > 0) {
+      units += np + kPieceCost;
+      ++cnt;
+      lo = min(lo, np);
+      hi = max(hi, np);
+    }
+  }
+  units = __reduce_add_sync(0xffffffffu, units);
+  cnt = __reduce_add_sync(0xffffffffu, cnt);
+  lo = __reduce_min_sync(0xffffffffu, lo);
+  hi = __reduce_max_sync(0xffffffffu, hi);
+  if (lane == 0) sc.sums[warp] = make_int4(units, cnt, lo, hi);
+  cta_bar();
+  units = cnt = hi = 0;
+  lo = INT_MAX;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    const int4 v = sc.sums[w];
+    units += v.x;
+    cnt += v.y;
+    lo = min(lo, v.z);
+    hi = max(hi, v.w);
+  }
+  const int pages = units - kPieceCost * cnt;
+  TeamRange r;
+  r.units_total = units;
+  r.any_empty = cnt < p.batch;
+  r.nteams = max(1, min(p.nteams, pages / kMinPagesPerTeam));
+  // Sequences of one length whose count divides into about as many groups as there are teams: one team per
+  // group of whole sequences.  Nothing is then published, counted or combined, at the price of leaving
+  // up to a quarter of the CTA slots empty.
+  if (cnt > 0 && lo == hi) {
+    const int k = (cnt + p.nteams - 1) / p.nteams;
+    const int groups = cnt / k;
+    if (groups * k == cnt && 4 * groups >= 3 * p.nteams) r.nteams = groups;
+  }
+  const bool mine = pages > 0 && team < r.nteams;
+  int x[2] = {0, 0};
+  if (mine) {
+    x[0] = mul_div(team, units, r.nteams);
+    x[1] = mul_div(team + 1, units, r.nteams);
+  }
+  if (tid < 2) sc.found[tid] = make_int4(0, 0, pages, 0);   // x[1] == units: the end of the line
+  cta_bar();
+  if (mine) {
+    int before_u = 0, before_c = 0;    // units and non-empty sequences before this round's
+    for (int base = 0; base < p.batch && before_u <= x[1]; base += kThreads) {
+      const int b = base + tid;
+      const int np = base == 0 ? own_np : (b < p.batch ? pages_of(seq_of<kChunk>(p, b).len) : 0);
+      const int u = np > 0 ? np + kPieceCost : 0;
+      int inc = u;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += o;
+      }
+      const unsigned non_empty = __ballot_sync(0xffffffffu, np > 0);
+      if (lane == 31) sc.scan[warp] = make_int2(inc, __popc(non_empty));
+      cta_bar();
+      int eu = before_u + inc - u, ec = before_c + __popc(non_empty & ((1u << lane) - 1));
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const int2 v = sc.scan[w];
+        if (w < warp) {
+          eu += v.x;
+          ec += v.y;
+        }
+        before_u += v.x;
+        before_c += v.y;
+      }
+#pragma unroll
+      for (int side = 0; side < 2; ++side) {
+        if (u > 0 && eu <= x[side] && x[side] < eu + u) {   // positions in a sequence's extra units are its start
+          const int page = max(0, x[side] - eu - kPieceCost);
+          sc.found[side] = make_int4(b, page, eu - kPieceCost * ec + page, ec);
+        }
+      }
+      cta_bar();
+    }
+  }
+  const int4 f0 = sc.found[0], f1 = sc.found[1];
+  r.b = f0.x;
+  r.page = f0.y;
+  r.flat = f0.z;
+  r.kseq = f0.w;
+  r.end = f1.z;
+  r.any = mine && r.end > r.flat;
+  cache_first = 0;
+  if (p.batch > kThreads && r.any) {   // the cache holds the sequences from this part's first on
+    cta_bar();
+    cache_first = r.b;
+    const int b = r.b + tid;
+    Seq s{0, 0, 0};
+    if (b < p.batch) s = seq_of<kChunk>(p, b);
+    cache.len[tid] = s.len;
+    cache.row[tid] = s.row;
+    cache.ql[tid] = s.ql;
+  }
+  cta_bar();
+  return r;
+}
+
+// Where a CTA stands: its sequences, the end of its part, its column block.
+struct Walk {
+  const SeqCache* cache;
+  int first;                 // sequence of the cache's first entry
+  int end;                   // flat end of the part
+  int col0;                  // first column of the block
+};
+template <bool kChunk>
+__device__ __forceinline__ Seq walk_seq(const Kv4Params& p, const Walk& w, int b) {
+  const int i = b - w.first;
+  if (i < kThreads) return Seq{w.cache->len[i], w.cache->row[i], w.cache->ql[i]};
+  return seq_of<kChunk>(p, b);
+}
+
+// A piece: the part of one sequence that lies in the team's part.
 struct Piece {
-  int b, row, len, np;   // sequence, table row, tokens, pages
-  int begin, end;        // pages [begin, end) of the sequence
-  int64_t flat;          // position of page `begin` on the page line
-  int kseq;              // non-empty sequences before b
+  int b, row, len, ql;
+  int begin, end;            // pages [begin, end) of the sequence
+  int flat;                  // position of page `begin` on the page line
+  int kseq;                  // non-empty sequences before b
   bool valid;
 };
-
-// Lengths and table rows of the sequences from `first` on, from shared memory for the first kSeqCache.
-struct SeqCache {
-  const int* len;
-  const int* row;
-  int first;
-  __device__ __forceinline__ int len_of(const Kv4DecodeParams& p, int b) const {
-    return b - first < kSeqCache ? len[b - first] : seq_len_checked(p, b);
+// The piece that starts at page `page` of sequence pc.b, or the first one after it that has a column for this
+// CTA (a shorter chunk may have none in the block).
+template <bool kChunk>
+__device__ __forceinline__ void settle_piece(const Kv4Params& p, const Walk& w, Piece& pc, int page) {
+  for (;;) {
+    const Seq s = walk_seq<kChunk>(p, w, pc.b);
+    if (s.len > 0) {
+      pc.len = s.len;
+      pc.row = s.row;
+      pc.ql = s.ql;
+      pc.begin = page;
+      pc.end = min(pages_of(s.len), page + (w.end - pc.flat));
+      pc.valid = true;
+      if (!kChunk || s.ql * p.group > w.col0) return;
+      pc.flat += pc.end - pc.begin;
+      ++pc.kseq;
+    }
+    ++pc.b;
+    page = 0;
+    if (pc.flat >= w.end || pc.b >= p.batch) {
+      pc.valid = false;
+      return;
+    }
   }
-  __device__ __forceinline__ int row_of(const Kv4DecodeParams& p, int b) const {
-    return b - first < kSeqCache ? row[b - first] : (p.row_ids ? __ldg(p.row_ids + b) : b);
-  }
-};
-
-__device__ __forceinline__ void enter_piece(const Kv4DecodeParams& p, const SeqCache& seq, int64_t range_end, Piece& pc,
-                                            int b, int first_page) {
-  pc.b = b;
-  pc.len = seq.len_of(p, b);
-  pc.row = seq.row_of(p, b);
-  pc.np = pages_of(pc.len);
-  pc.begin = first_page;
-  const int64_t room = range_end - pc.flat;
-  pc.end = (pc.np - first_page <= room) ? pc.np : first_page + static_cast<int>(room);
-  pc.valid = true;
 }
-__device__ __forceinline__ void next_piece(const Kv4DecodeParams& p, const SeqCache& seq, int64_t range_end, Piece& pc) {
+template <bool kChunk>
+__device__ __forceinline__ void next_piece(const Kv4Params& p, const Walk& w, Piece& pc) {
   pc.flat += pc.end - pc.begin;
   pc.valid = false;
-  if (pc.flat >= range_end) return;
-  int b = pc.b + 1;
-  while (b < p.batch && seq.len_of(p, b) == 0) ++b;
-  if (b >= p.batch) return;   // cannot happen for consistent lengths; stop rather than overrun
   ++pc.kseq;
-  enter_piece(p, seq, range_end, pc, b, 0);
+  ++pc.b;
+  if (pc.flat < w.end && pc.b < p.batch) settle_piece<kChunk>(p, w, pc, 0);
 }
 // Pages of a piece that belong to a warp.
 __device__ __forceinline__ int warp_pages(const Piece& pc, int warp) {
-  return pc.valid ? (pc.end - pc.begin - warp + kConsumerWarps - 1) / kConsumerWarps : 0;
+  return pc.valid ? (pc.end - pc.begin - warp + kWarps - 1) / kWarps : 0;
 }
 
 // The pages a warp requests, in order and two at a time: lane l holds the number of page
 // begin + warp + 4 * (32 * block + l) of the piece; the next block of table entries (of this piece, or
 // the first of the next piece) is already on its way.
+template <bool kChunk>
 struct PageStream {
   Piece pc, nx;
   int m, cnt;            // next page of this warp in pc, and how many it has there
   int32_t ids, ids_next; // page numbers in use; raw table entries of the next block
 
   // Raw table entry -> page number; an entry that names no page is reported and page 0 read instead.
-  __device__ __forceinline__ static int32_t checked(const Kv4DecodeParams& p, int32_t id) {
+  __device__ __forceinline__ static int32_t checked(const Kv4Params& p, int32_t id) {
     int32_t page = id;
     bool ok = true;
     if (p.table_kind == B200KV_TABLE_TOKEN) {
@@ -163,34 +396,34 @@ struct PageStream {
     }
     return page;
   }
-  __device__ __forceinline__ int32_t load_ids(const Kv4DecodeParams& p, const Piece& from, int warp, int lane, int first) const {
-    const int page = from.begin + warp + kConsumerWarps * (first + lane);
+  __device__ __forceinline__ int32_t load_ids(const Kv4Params& p, const Piece& from, int warp, int lane, int first) const {
+    const int page = from.begin + warp + kWarps * (first + lane);
     if (!from.valid || page >= from.end) return 0;
     const int64_t at = p.table_kind == B200KV_TABLE_BLOCK ? page : static_cast<int64_t>(page) * kPS;
     return __ldg(p.table + static_cast<int64_t>(from.row) * p.table_row_stride + at);
   }
-  __device__ __forceinline__ void refill(const Kv4DecodeParams& p, const SeqCache& seq, int64_t range_end, int warp, int lane) {
+  __device__ __forceinline__ void refill(const Kv4Params& p, const Walk& w, int warp, int lane) {
     if (m + 32 < cnt) {
       ids_next = load_ids(p, pc, warp, lane, m + 32);
     } else {
       nx = pc;
       do {
-        next_piece(p, seq, range_end, nx);
+        next_piece<kChunk>(p, w, nx);
       } while (nx.valid && warp_pages(nx, warp) <= 0);   // short pieces have no page for the later warps
       ids_next = load_ids(p, nx, warp, lane, 0);
     }
   }
-  __device__ __forceinline__ void start(const Kv4DecodeParams& p, const SeqCache& seq, int64_t range_end, const Piece& first,
+  __device__ __forceinline__ void start(const Kv4Params& p, const Walk& w, const Piece& first,
                                         int warp, int lane) {
     pc = first;
-    while (pc.valid && warp_pages(pc, warp) <= 0) next_piece(p, seq, range_end, pc);
+    while (pc.valid && warp_pages(pc, warp) <= 0) next_piece<kChunk>(p, w, pc);
     m = 0;
     cnt = warp_pages(pc, warp);
     ids = checked(p, load_ids(p, pc, warp, lane, 0));
-    if (pc.valid) refill(p, seq, range_end, warp, lane);
+    if (pc.valid) refill(p, w, warp, lane);
   }
   __device__ __forceinline__ bool more() const { return pc.valid; }
-  __device__ __forceinline__ void advance(const Kv4DecodeParams& p, const SeqCache& seq, int64_t range_end, int warp, int lane) {
+  __device__ __forceinline__ void advance(const Kv4Params& p, const Walk& w, int warp, int lane) {
     m += 2;
     const bool done = m >= cnt;
     if (!done && (m & 31) != 0) return;
@@ -200,7 +433,7 @@ struct PageStream {
       cnt = warp_pages(pc, warp);
     }
     ids = checked(p, ids_next);
-    if (pc.valid) refill(p, seq, range_end, warp, lane);
+    if (pc.valid) refill(p, w, warp, lane);
   }
 };
 
@@ -249,10 +482,12 @@ __device__ __forceinline__ void page_v_scales(const uint8_t* at, uint32_t (&sv)[
   sv[3][1] = __byte_perm(t1.y, t1.w, 0x7632);
 }
 
-// O^T += V^T (P^T s_V) of 16 tokens.
-template <int NB>
+// O^T += V^T (P^T s_V) of 16 tokens.  kMasked: `seen` has all ones where this lane's column (as a B fragment)
+// sees the token, so that a V scale of NaN reaches no column that does not.
+template <int NB, bool kMasked>
 __device__ __forceinline__ void page_pv(const uint8_t* v_at, uint32_t vsel, const uint32_t (&sv)[4][2],
-                                        const uint32_t (&pb)[NB][2], float (&o)[8][NB][4]) {
+                                        const uint32_t (&pb)[NB][2], const uint32_t (&seen)[NB][2],
+                                        float (&o)[8][NB][4]) {
   const uint4 v0 = *reinterpret_cast<const uint4*>(v_at), v1 = *reinterpret_cast<const uint4*>(v_at + kv4::kRowBytes);
   const uint4 v2 = *reinterpret_cast<const uint4*>(v_at + 8 * kv4::kRowBytes);
   const uint4 v3 = *reinterpret_cast<const uint4*>(v_at + 9 * kv4::kRowBytes);
@@ -265,7 +500,11 @@ __device__ __forceinline__ void page_pv(const uint8_t* v_at, uint32_t vsel, cons
     kv4::unpack_word(__byte_perm(x2[g], x3[g], vsel), b);
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const uint32_t q0 = kv4::h2_mul(pb[nb][0], sv[g][0]), q1 = kv4::h2_mul(pb[nb][1], sv[g][1]);
+      uint32_t q0 = kv4::h2_mul(pb[nb][0], sv[g][0]), q1 = kv4::h2_mul(pb[nb][1], sv[g][1]);
+      if (kMasked) {
+        q0 &= seen[nb][0];
+        q1 &= seen[nb][1];
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float(&acc)[4] = o[2 * g + e][nb];
@@ -298,10 +537,10 @@ __device__ __forceinline__ unsigned atomic_inc_acq_rel(unsigned* ctr, unsigned l
 // memory; every thread then combines 2 * NB of the 16-byte pieces over the warps and writes the final
 // rows (whole sequence) or the partial, in the same fragment order (16-byte accesses without bank
 // conflicts or strides all the way).  A partial is published by one release-acquire count on the
-// (sequence, head) counter, which wraps to zero on the last arrival; the CTA that arrives last
+// (sequence, head, column block) counter, which wraps to zero on the last arrival; the CTA that arrives last
 // combines the partials of all pieces the same way.
-template <int ROWS>
-__device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Piece& pc, bool whole, int team, int head, int tid,
+template <int ROWS, bool kChunk>
+__device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc, bool whole, int team, int head, int blk, int q_row0, int tid,
                                              const float (&o)[8][ROWS / 8][4], const float (&m_ref)[ROWS / 8][2],
                                              const float (&l_run)[ROWS / 8][2], float4* merge_o, float2* merge_ml,
                                              int* note) {
@@ -309,7 +548,7 @@ __device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Pie
   constexpr int kParts = 8 * NB;               // fragments of a warp
   const int lane = tid & 31, warp = tid >> 5;
   const int r = lane >> 2, jq = lane & 3;
-  consumer_bar();   // the previous piece's merge has read the buffers
+  cta_bar();   // the previous piece's merge has read the buffers
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
@@ -324,42 +563,43 @@ __device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Pie
       if (r == 0) merge_ml[warp * ROWS + nb * 8 + 2 * jq + h] = make_float2(m_ref[nb][h], l);
     }
   }
-  consumer_bar();
+  cta_bar();
   // O / l of one fragment (M block j = 2 g + e: elements d0 and d0 + 2, heads 2 jq, 2 jq + 1) -> out
   auto write_out = [&](int nb, int j, const Weighted& w) {
     const int d0 = 32 * (j >> 1) + 8 * (r >> 1) + 4 * (j & 1) + (r & 1);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int hq = nb * 8 + 2 * jq + h;
-      if (hq < p.group) {
-        __half* dst = p.out + static_cast<int64_t>(pc.b) * p.out_stride_b +
-                      (static_cast<int64_t>(head) * p.group + hq) * p.out_stride_h + d0;
+      const int col = blk * ROWS + nb * 8 + 2 * jq + h;
+      if (col < (kChunk ? pc.ql * p.group : p.group)) {
+        const int tok = kChunk ? col / p.group : 0;
+        __half* dst = p.out + static_cast<int64_t>(q_row0 + tok) * p.out_stride_t +
+                      static_cast<int64_t>(head * p.group + col - tok * p.group) * p.out_stride_h + d0;
         dst[0] = __float2half_rn(w.acc[h] / w.l[h]);
         dst[2] = __float2half_rn(w.acc[h + 2] / w.l[h]);
       }
     }
   };
-  const int64_t slot = (static_cast<int64_t>(team) + pc.b) * p.kv_heads + head;
-  float4* part = reinterpret_cast<float4*>(p.part_o) + slot * kParts * 32;
-  float2* part_ml = reinterpret_cast<float2*>(p.part_lse) + slot * ROWS;
+  const int64_t slot = ((static_cast<int64_t>(team) + pc.b) * p.kv_heads + head) * p.blocks + blk;
+  float4* part = p.part_o + slot * kParts * 32;
+  float2* part_ml = p.part_ml + slot * ROWS;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     // (m, l) of the four warps for this lane's two heads
-    float2 ml[kConsumerWarps][2];
+    float2 ml[kWarps][2];
     float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-    for (int w = 0; w < kConsumerWarps; ++w) {
+    for (int w = 0; w < kWarps; ++w) {
       const float4 v = *reinterpret_cast<const float4*>(merge_ml + w * ROWS + nb * 8 + 2 * jq);
       ml[w][0] = make_float2(v.x, v.y);
       ml[w][1] = make_float2(v.z, v.w);
       top[0] = fmaxf(top[0], v.x);
       top[1] = fmaxf(top[1], v.z);
     }
-    float wt[kConsumerWarps][2];
+    float wt[kWarps][2];
     Weighted sum[2];
     float l[2] = {0.f, 0.f};
 #pragma unroll
-    for (int w = 0; w < kConsumerWarps; ++w)
+    for (int w = 0; w < kWarps; ++w)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         // a warp without a page of this piece, or with only NaN scores: its sums enter as they are
@@ -372,7 +612,7 @@ __device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Pie
 #pragma unroll
       for (int i = 0; i < 4; ++i) sum[k].acc[i] = 0.f;
 #pragma unroll
-      for (int w = 0; w < kConsumerWarps; ++w)
+      for (int w = 0; w < kWarps; ++w)
         sum[k].add(merge_o[(w * kParts + nb * 8 + j) * 32 + lane], wt[w][0], wt[w][1]);
       if (whole) {
         sum[k].l[0] = l[0];
@@ -387,15 +627,15 @@ __device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Pie
   }
   if (whole) return;
   const int first_team = note[1], pieces = note[2];   // thread 0 rewrites both when the next piece begins
-  consumer_bar();   // all of the CTA's partial is written; the count below publishes it
+  cta_bar();   // all of the CTA's partial is written; the count below publishes it
   if (tid == 0)
-    note[0] = atomic_inc_acq_rel(p.piece_ctr + static_cast<int64_t>(pc.b) * p.kv_heads + head,
+    note[0] = atomic_inc_acq_rel(p.piece_ctr + (static_cast<int64_t>(pc.b) * p.kv_heads + head) * p.blocks + blk,
                                  static_cast<unsigned>(pieces - 1)) == static_cast<unsigned>(pieces - 1);
-  consumer_bar();
+  cta_bar();
   if (note[0] == 0) return;
   // Last to arrive: the partials of all pieces (this CTA's own among them) lie in neighbouring slots.
-  const int64_t slot0 = (static_cast<int64_t>(first_team) + pc.b) * p.kv_heads + head;
-  const int64_t step = p.kv_heads;
+  const int64_t slot0 = ((static_cast<int64_t>(first_team) + pc.b) * p.kv_heads + head) * p.blocks + blk;
+  const int64_t step = static_cast<int64_t>(p.kv_heads) * p.blocks;
   constexpr int kBatch = 4;                    // partials in flight
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
@@ -412,10 +652,10 @@ __device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Pie
       for (int i = 0; i < kBatch; ++i) {
         if (p0 + i < pieces) {
           const int64_t sl = slot0 + (p0 + i) * step;
-          ml[i] = __ldcg(reinterpret_cast<const float4*>(reinterpret_cast<const float2*>(p.part_lse) + sl * ROWS + nb * 8 + 2 * jq));
+          ml[i] = __ldcg(reinterpret_cast<const float4*>(p.part_ml + sl * ROWS + nb * 8 + 2 * jq));
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            v[i][k] = __ldcg(reinterpret_cast<const float4*>(p.part_o) + (sl * kParts + nb * 8 + 2 * warp + k) * 32 + lane);
+            v[i][k] = __ldcg(p.part_o + (sl * kParts + nb * 8 + 2 * warp + k) * 32 + lane);
         } else {
           ml[i] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
           v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -456,40 +696,42 @@ __device__ __forceinline__ void finish_piece(const Kv4DecodeParams& p, const Pie
   }
 }
 
-template <int ROWS>
-__global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel(Kv4DecodeParams p) {
-  static_assert(ROWS == 8 || ROWS == 16, "query-group heads are padded to 8 or 16");
+// kChunk: query rows come in chunks (p.q_lens); a decode step has one per sequence, and its code none of the
+// arithmetic that several take.
+template <int ROWS, bool kChunk>
+__global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel(Kv4Params p) {
+  static_assert(ROWS == 8 || ROWS == 16, "columns are padded to 8 or 16");
   constexpr int NB = ROWS / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   float4* merge_o = reinterpret_cast<float4*>(smem + kRingBytes);          // [4 warps][8 * NB][32 lanes]
-  float2* merge_ml = reinterpret_cast<float2*>(merge_o + kConsumerWarps * 8 * NB * 32);   // [4][ROWS] (m, l)
-  int* note = reinterpret_cast<int*>(merge_ml + kConsumerWarps * ROWS);    // [0] this CTA merges, [1] first team, [2] pieces
-  int* seq_len_s = note + 4;                                               // [kSeqCache]
-  int* seq_row_s = seq_len_s + kSeqCache;
-  int* scan = reinterpret_cast<int*>(merge_o);
+  float2* merge_ml = reinterpret_cast<float2*>(merge_o + kWarps * 8 * NB * 32);   // [4][ROWS] (m, l)
+  int* note = reinterpret_cast<int*>(merge_ml + kWarps * ROWS);            // [0] this CTA merges, [1] first team, [2] pieces
+  SeqCache& cache = *reinterpret_cast<SeqCache*>(note + 4);
+  PlanScratch& scratch = *reinterpret_cast<PlanScratch*>(merge_o);
 
   const int tid = threadIdx.x;
   const int lane = tid & 31;
   const int warp = tid >> 5;
-  const int team = blockIdx.x / p.kv_heads;
-  const int head = blockIdx.x - team * p.kv_heads;
+  const int unit = kChunk ? blockIdx.x / p.blocks : blockIdx.x;
+  const int blk = kChunk ? blockIdx.x - unit * p.blocks : 0;
+  const int team = unit / p.kv_heads;
+  const int head = unit - team * p.kv_heads;
   const uint8_t* ring = smem + warp * (kStages * kPairBytes);
-  const TeamRange range = plan_team_range(p, team, tid, scan);
-  if (range.any) {
-    const int b = range.start_b + tid;
-    seq_len_s[tid] = b < p.batch ? seq_len_checked(p, b) : 0;
-    seq_row_s[tid] = b < p.batch ? (p.row_ids ? __ldg(p.row_ids + b) : b) : 0;
-  }
-  __syncthreads();
-  const SeqCache seq{seq_len_s, seq_row_s, range.start_b};
+  if (kChunk) pdl_wait_then_trigger();   // a chunk's lengths may come straight from the kernel before
+  Walk walk;
+  const TeamRange range = plan_team_range<kChunk>(p, team, tid, scratch, cache, walk.first);
+  walk.cache = &cache;
+  walk.end = range.end;
+  walk.col0 = blk * ROWS;
   Piece pc;
-  pc.flat = range.begin;
-  pc.kseq = range.start_k;
   pc.valid = false;
-  PageStream st;
+  PageStream<kChunk> st;
   if (range.any) {
-    enter_piece(p, seq, range.end, pc, range.start_b, range.start_page);
-    st.start(p, seq, range.end, pc, warp, lane);
+    pc.b = range.b;
+    pc.flat = range.flat;
+    pc.kseq = range.kseq;
+    settle_piece<kChunk>(p, walk, pc, range.page);
+    st.start(p, walk, pc, warp, lane);
   }
   const uint8_t* k_rows = p.pool + static_cast<int64_t>(head) * kv4::kBlockBytes;
   const int64_t v_from_k = static_cast<int64_t>(p.kv_heads) * kv4::kBlockBytes;
@@ -501,12 +743,12 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
     bulk_prefetch_l2(src + v_from_k, kv4::kBlockBytes);
   }
   pdl_wait_then_trigger();   // q, the pool, the workspace and out belong to earlier kernels until here
-  if (team == 0 && range.any_empty) {
-    // No keys: the output rows are defined as zero, and nobody else writes them.
+  if (!kChunk && team == 0 && range.any_empty) {
+    // No keys: the output rows of a decode step are defined as zero, and nobody else writes them.
     for (int b = 0; b < p.batch; ++b) {
-      if (seq_len_checked(p, b) != 0) continue;
+      if (seq_of<kChunk>(p, b).len != 0) continue;
       for (int g = 0; g < p.group; ++g)
-        p.out[static_cast<int64_t>(b) * p.out_stride_b +
+        p.out[static_cast<int64_t>(b) * p.out_stride_t +
               (static_cast<int64_t>(head) * p.group + g) * p.out_stride_h + tid] = __float2half_rn(0.f);
     }
   }
@@ -537,7 +779,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
         async_copy16(dst + 3584, v1 + 3584, policy);
         async_copy16(dst + 4096, v1 + 4096, policy);
       }
-      st.advance(p, seq, range.end, warp, lane);
+      st.advance(p, walk, warp, lane);
     }
     async_commit();   // an empty group too: the wait below counts groups
   };
@@ -558,14 +800,27 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
     uint32_t qf[NB][8][2];     // Q^T as B fragments
     float o[8][NB][4];         // O^T: 8 M blocks of 16 along head_dim
     float m_ref[NB][2], l_run[NB][2];
+    const int q_row0 = kChunk ? __ldg(p.q_start + pc.b) : pc.b;
+    const int cols = kChunk ? pc.ql * p.group : p.group;
+    const int pos0 = pc.len - (kChunk ? pc.ql : 1);     // position of the first query token: column c sees positions <= pos0 + c / group
+    int lim[NB][2], lim_r[NB];           // of columns 2 jq, 2 jq + 1 (S^T) and r (P^T as B fragment) of each N block
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      const int hq = nb * 8 + r;
-      const __half* qh = p.q + static_cast<int64_t>(pc.b) * p.q_stride_b +
+      lim[nb][0] = lim[nb][1] = lim_r[nb] = pos0;
+      const int col = walk.col0 + nb * 8 + r;
+      int tok = 0, hq = col;
+      if (kChunk) {
+        tok = col / p.group;
+        hq = col - tok * p.group;
+        lim_r[nb] += tok;
+        lim[nb][0] += (walk.col0 + nb * 8 + 2 * jq) / p.group;
+        lim[nb][1] += (walk.col0 + nb * 8 + 2 * jq + 1) / p.group;
+      }
+      const __half* qh = p.q + static_cast<int64_t>(q_row0 + tok) * p.q_stride_t +
                          (static_cast<int64_t>(head) * p.group + hq) * p.q_stride_h + 8 * jq;
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const uint4 v = hq < p.group ? __ldg(reinterpret_cast<const uint4*>(qh + 32 * g)) : make_uint4(0, 0, 0, 0);
+        const uint4 v = col < cols ? __ldg(reinterpret_cast<const uint4*>(qh + 32 * g)) : make_uint4(0, 0, 0, 0);
         qf[nb][2 * g][0] = v.x;
         qf[nb][2 * g][1] = v.y;
         qf[nb][2 * g + 1][0] = v.z;
@@ -580,17 +835,21 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
       for (int nb = 0; nb < NB; ++nb) o[j][nb][0] = o[j][nb][1] = o[j][nb][2] = o[j][nb][3] = 0.f;
     float p_room = 14.f;       // log2 of the largest P allowed: P * (largest V scale) stays under 2^15
     uint32_t sv_lim = 0x4000u; // V scales seen are below this fp16 number (2 to begin with)
-    const bool whole = pc.begin == 0 && pc.end == pc.np;
+    // positions up to here are seen by every column of the block
+    const int all_see = pos0 + (kChunk ? walk.col0 / p.group : 0);
+    const int np = pages_of(pc.len);
+    const bool whole = pc.begin == 0 && pc.end == np;
     const int cnt = warp_pages(pc, warp);
     if (tid == 0 && !whole) {   // the teams that hold a piece of this sequence; read at the end of the piece
-      const int64_t u0 = (pc.flat - pc.begin) + static_cast<int64_t>(p.piece_cost) * (pc.kseq + 1);
-      note[1] = team_of(u0, range.nteams_eff, range.units_total);
-      note[2] = team_of(u0 + pc.np - 1, range.nteams_eff, range.units_total) - note[1] + 1;
+      const int u0 = pc.flat - pc.begin + kPieceCost * (pc.kseq + 1);
+      note[1] = team_of(u0, range.nteams, range.units_total);
+      note[2] = team_of(u0 + np - 1, range.nteams, range.units_total) - note[1] + 1;
     }
 
 #pragma unroll 1
     for (int m = 0; m < cnt; m += 2) {
-      const bool last_step = m + 2 >= cnt;
+      const int page = pc.begin + warp + kWarps * m;      // the step's pages are this one and the fourth after it
+      const bool masked = m + 1 >= cnt || (page + kWarps) * kPS + kPS - 1 > all_see;
       async_wait<kStages - 1>();
       __syncwarp();   // the pair's pieces were copied by all lanes
       const int pair = stage * kPairBytes;
@@ -601,20 +860,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
         page_scores<NB>(k_at + pair + h * kPageBytes, kc_at + pair + h * kPageBytes, qf, p.scale_log2, s[h]);
         page_v_scales(vc_at + pair + h * kPageBytes, sv[h]);
       }
-      if (last_step) {
+      if (masked) {
         // Rows past the length were never written and a missing second page was not loaded: they may
-        // hold anything, NaN scales included.
+        // hold anything, NaN scales included.  Positions past a column's own are not for it.
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int page = pc.begin + warp + kConsumerWarps * (m + h);
-          const int n = m + h < cnt ? pc.len - page * kPS : 0;   // valid tokens, if fewer than 16
+          const int at = m + h < cnt ? (page + kWarps * h) * kPS : INT_MAX - kPS;   // position of the page's first token
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (r >= n) s[h][nb][0] = s[h][nb][1] = -INFINITY;
-            if (r + 8 >= n) s[h][nb][2] = s[h][nb][3] = -INFINITY;
-          }
-          const uint32_t keep0 = (2 * jq < n ? 0xffffu : 0u) | (2 * jq + 1 < n ? 0xffff0000u : 0u);
-          const uint32_t keep1 = (2 * jq + 8 < n ? 0xffffu : 0u) | (2 * jq + 9 < n ? 0xffff0000u : 0u);
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (at + r > lim[nb][i]) s[h][nb][i] = -INFINITY;
+              if (at + r + 8 > lim[nb][i]) s[h][nb][i + 2] = -INFINITY;
+            }
+          const int n = pc.len - at - 2 * jq;
+          const uint32_t keep0 = (0 < n ? 0xffffu : 0u) | (1 < n ? 0xffff0000u : 0u);
+          const uint32_t keep1 = (8 < n ? 0xffffu : 0u) | (9 < n ? 0xffff0000u : 0u);
 #pragma unroll
           for (int g = 0; g < 4; ++g) {
             sv[h][g][0] &= keep0;
@@ -688,33 +949,68 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
         }
       }
 #pragma unroll
-      for (int h = 0; h < 2; ++h) page_pv<NB>(v_at + pair + h * kPageBytes, vsel, sv[h], pb[h], o);
+      for (int h = 0; h < 2; ++h) {
+        uint32_t seen[NB][2];
+        if (kChunk && masked) {
+          const int at = m + h < cnt ? (page + kWarps * h) * kPS + 2 * jq : INT_MAX - kPS;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            const int n = lim_r[nb] - at;
+            seen[nb][0] = (0 <= n ? 0xffffu : 0u) | (1 <= n ? 0xffff0000u : 0u);
+            seen[nb][1] = (8 <= n ? 0xffffu : 0u) | (9 <= n ? 0xffff0000u : 0u);
+          }
+          page_pv<NB, true>(v_at + pair + h * kPageBytes, vsel, sv[h], pb[h], seen, o);
+        } else {
+          page_pv<NB, false>(v_at + pair + h * kPageBytes, vsel, sv[h], pb[h], seen, o);
+        }
+      }
       __syncwarp();   // every lane has read the slot
       request(stage);
       if (++stage == kStages) stage = 0;
     }
 
-    finish_piece<ROWS>(p, pc, whole, team, head, tid, o, m_ref, l_run, merge_o, merge_ml, note);
-    next_piece(p, seq, range.end, pc);
+    finish_piece<ROWS, kChunk>(p, pc, whole, team, head, blk, q_row0, tid, o, m_ref, l_run, merge_o, merge_ml, note);
+    next_piece<kChunk>(p, walk, pc);
   }
 }
 
-inline int rows_for_group(int group) { return group <= 8 ? 8 : 16; }
-inline int max_teams(int sms, int kv_heads, int rows) {
-  const int t = sms * ctas_per_sm(rows) / kv_heads;
-  return t < 1 ? 1 : t;
-}
-inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+inline int64_t align_up(int64_t x, int64_t a) { return (x + a - 1) / a * a; }
 
-template <int ROWS>
-int launch_decode(const Kv4DecodeParams& p, bool programmatic, cudaStream_t stream) {
-  constexpr int smem = kRingBytes + kConsumerWarps * ROWS * kD * 4 + kConsumerWarps * ROWS * 2 * 4 + 4 * 4 +
-                       2 * kSeqCache * 4;
+// How a launch is cut: columns per CTA, column blocks, teams at most.
+struct Shape {
+  int rows, blocks, teams;
+};
+int shape_of(int max_q_len, int q_heads, int kv_heads, Shape* s) {
+  const int sms = device_sm_count();
+  if (sms <= 0) return B200KV_ECUDA;
+  const int cols = max_q_len * (q_heads / kv_heads);
+  s->rows = cols <= 8 ? 8 : 16;
+  s->blocks = (cols + s->rows - 1) / s->rows;
+  const int t = sms * ctas_per_sm(s->rows) / (kv_heads * s->blocks);
+  s->teams = t < 1 ? 1 : t;
+  return B200KV_OK;
+}
+
+// Byte offsets of the workspace's parts: counters, partial outputs, (m, l).
+struct Layout {
+  int64_t ml, total;
+};
+Layout layout_of(const Shape& s, int batch, int kv_heads) {
+  const int64_t slots = (static_cast<int64_t>(s.teams) + batch) * kv_heads * s.blocks;
+  Layout l;
+  l.ml = static_cast<int64_t>(kCounterBytes) + slots * s.rows * kD * 4;
+  l.total = l.ml + align_up(slots * s.rows * 8, 256);
+  return l;
+}
+
+template <int ROWS, bool kChunk>
+int launch_decode(const Kv4Params& p, bool programmatic, cudaStream_t stream) {
+  constexpr int smem = kRingBytes + kWarps * ROWS * kD * 4 + kWarps * ROWS * 2 * 4 + 4 * 4 + static_cast<int>(sizeof(SeqCache));
   static bool attr_done[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return record_cuda_error(cudaGetLastError());
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<ROWS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    cudaError_t e = cudaFuncSetAttribute(kv4_decode_kernel<ROWS, kChunk>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
   }
@@ -722,29 +1018,62 @@ int launch_decode(const Kv4DecodeParams& p, bool programmatic, cudaStream_t stre
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(static_cast<unsigned>(p.nteams * p.kv_heads));
+  cfg.gridDim = dim3(static_cast<unsigned>(p.nteams * p.kv_heads * p.blocks));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = programmatic ? 1 : 0;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<ROWS>, p);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_decode_kernel<ROWS, kChunk>, p);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }
 
+int run_decode(Kv4Params& p, int q_heads, const Shape& s, void* workspace, size_t workspace_bytes, int64_t max_kv_len,
+               bool programmatic, cudaStream_t stream) {
+  if (static_cast<int64_t>(p.batch) * p.kv_heads * s.blocks > kMaxCounters) return B200KV_ETOOLARGE;
+  const int64_t pages_bound = static_cast<int64_t>(p.batch) * ((max_kv_len + kPS - 1) / kPS + kPieceCost);
+  if (pages_bound > INT_MAX) return B200KV_ETOOLARGE;   // the page line is counted in 32 bits
+  const Layout l = layout_of(s, p.batch, p.kv_heads);
+  if (workspace_bytes < static_cast<size_t>(l.total)) return B200KV_EWORKSPACE;
+  // Do not launch more teams than the page bound can feed.
+  int64_t teams = static_cast<int64_t>(p.batch) * ((max_kv_len + kPS - 1) / kPS) / kMinPagesPerTeam;
+  if (teams > s.teams) teams = s.teams;
+  p.nteams = static_cast<int>(teams < 1 ? 1 : teams);
+  p.blocks = s.blocks;
+  p.group = q_heads / p.kv_heads;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  p.piece_ctr = reinterpret_cast<unsigned*>(ws);
+  p.part_o = reinterpret_cast<float4*>(ws + kCounterBytes);
+  p.part_ml = reinterpret_cast<float2*>(ws + l.ml);
+  if (p.q_lens != nullptr)
+    return s.rows == 8 ? launch_decode<8, true>(p, programmatic, stream) : launch_decode<16, true>(p, programmatic, stream);
+  return s.rows == 8 ? launch_decode<8, false>(p, programmatic, stream) : launch_decode<16, false>(p, programmatic, stream);
+}
+
+inline bool misaligned(const void* ptr, uintptr_t al) { return (reinterpret_cast<uintptr_t>(ptr) & (al - 1)) != 0; }
+
+// Columns (query tokens x heads of a group) up to which a chunk is streamed like a decode step.
+constexpr int kChunkColumns = 128;
+
 }  // namespace
 
 size_t kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim) {
-  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || head_dim != kD) return 0;
+  if (batch <= 0 || batch > 4096 || q_heads <= 0 || kv_heads <= 0 || head_dim != kD) return 0;
   if (q_heads % kv_heads != 0 || q_heads / kv_heads > 16) return 0;
   if (static_cast<int64_t>(batch) * kv_heads > kMaxCounters) return 0;
-  const int sms = device_sm_count();
-  if (sms <= 0) return 0;
-  const int rows = rows_for_group(q_heads / kv_heads);
-  const size_t nslots = static_cast<size_t>(max_teams(sms, kv_heads, rows)) + static_cast<size_t>(batch);
-  return kCounterBytes + align_up(nslots * kv_heads * rows * kD * sizeof(float), 256) +
-         align_up(nslots * kv_heads * rows * sizeof(float2), 256);
+  Shape s;
+  if (shape_of(1, q_heads, kv_heads, &s) != B200KV_OK) return 0;
+  return static_cast<size_t>(layout_of(s, batch, kv_heads).total);
+}
+
+size_t kv4_chunk_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads, int head_dim) {
+  if (batch <= 0 || batch > 4096 || q_heads <= 0 || kv_heads <= 0 || max_q_len <= 0 || head_dim != kD) return 0;
+  if (q_heads % kv_heads != 0 || max_q_len * (q_heads / kv_heads) > kChunkColumns) return 0;
+  Shape s;
+  if (shape_of(static_cast<int>(max_q_len), q_heads, kv_heads, &s) != B200KV_OK) return 0;
+  if (static_cast<int64_t>(batch) * kv_heads * s.blocks > kMaxCounters) return 0;
+  return static_cast<size_t>(layout_of(s, batch, kv_heads).total);
 }
 
 int kv4_paged_decode(const Kv4DecodeArgs& a, cudaStream_t stream) {
@@ -754,10 +1083,8 @@ int kv4_paged_decode(const Kv4DecodeArgs& a, cudaStream_t stream) {
   if (a.table_kind != B200KV_TABLE_BLOCK && a.table_kind != B200KV_TABLE_TOKEN) return B200KV_EINVAL;
   if (a.head_dim != kD || a.page_size != kPS) return B200KV_EUNSUPPORTED;
   if (a.q_heads % a.kv_heads != 0) return B200KV_EUNSUPPORTED;
-  const int group = a.q_heads / a.kv_heads;
-  if (group > 16) return B200KV_EUNSUPPORTED;
+  if (a.q_heads / a.kv_heads > 16) return B200KV_EUNSUPPORTED;
   if (a.batch > 4096) return B200KV_ETOOLARGE;
-  if (static_cast<int64_t>(a.batch) * a.kv_heads > kMaxCounters) return B200KV_ETOOLARGE;
   if (a.max_seq_len > (int64_t{1} << 30)) return B200KV_ETOOLARGE;
   if (a.table_rows <= 0 || a.table_cols <= 0 || a.table_row_stride < a.table_cols) return B200KV_EINVAL;
   if (a.row_ids == nullptr && a.batch > a.table_rows) return B200KV_EINVAL;
@@ -765,56 +1092,74 @@ int kv4_paged_decode(const Kv4DecodeArgs& a, cudaStream_t stream) {
   if (a.flags & ~B200KV_DECODE_SERIALIZED) return B200KV_EINVAL;
   int rc = kv4_check_pool(a.pool, a.pool_pages, a.page_stride_bytes, a.kv_heads);
   if (rc != B200KV_OK) return rc;
-  auto mis = [](const void* ptr, uintptr_t al) { return (reinterpret_cast<uintptr_t>(ptr) & (al - 1)) != 0; };
-  if (mis(a.q, 16) || mis(a.out, 8) || mis(a.workspace, 16)) return B200KV_EALIGN;
+  if (misaligned(a.q, 16) || misaligned(a.out, 8) || misaligned(a.workspace, 16)) return B200KV_EALIGN;
   if (a.q_stride_b % 8 != 0 || a.q_stride_h % 8 != 0) return B200KV_EALIGN;
   if (a.out_stride_b % 4 != 0 || a.out_stride_h % 4 != 0) return B200KV_EALIGN;
-  const size_t need = kv4_decode_workspace_bytes(a.batch, a.q_heads, a.kv_heads, a.head_dim);
-  if (need == 0) return B200KV_ECUDA;
-  if (a.workspace_bytes < need) return B200KV_EWORKSPACE;
-
-  const int sms = device_sm_count();
-  const int rows = rows_for_group(group);
-  const int teams_cap = max_teams(sms, a.kv_heads, rows);
-  // Do not launch more teams than the page bound can feed.
-  const int64_t pages_bound = static_cast<int64_t>(a.batch) * ((a.max_seq_len + kPS - 1) / kPS);
-  int64_t teams = pages_bound / kMinPagesPerTeam;
-  if (teams > teams_cap) teams = teams_cap;
-  if (teams < 1) teams = 1;
-
-  Kv4DecodeParams p{};
+  Shape s;
+  rc = shape_of(1, a.q_heads, a.kv_heads, &s);
+  if (rc != B200KV_OK) return rc;
+  Kv4Params p{};
   p.q = static_cast<const __half*>(a.q);
-  p.q_stride_b = a.q_stride_b;
+  p.q_stride_t = a.q_stride_b;
   p.q_stride_h = a.q_stride_h;
   p.pool = static_cast<const uint8_t*>(a.pool);
-  p.pool_pages = a.pool_pages;
+  p.pool_pages = static_cast<int>(a.pool_pages);
   p.page_stride = a.page_stride_bytes;
   p.table = a.table;
   p.table_row_stride = a.table_row_stride;
   p.table_kind = a.table_kind;
   p.table_rows = a.table_rows;
   p.row_ids = a.row_ids;
-  p.seq_lens = a.seq_lens;
-  p.seq_lens_i64 = a.seq_lens_i64;
+  p.lens = a.seq_lens;
+  p.lens_i64 = a.seq_lens_i64;
   p.batch = a.batch;
-  p.q_heads = a.q_heads;
   p.kv_heads = a.kv_heads;
-  p.group = group;
+  p.max_seq_len = static_cast<int>(a.max_seq_len);
+  p.max_q_len = 1;
   p.scale_log2 = a.scale * 1.4426950408889634f;
-  p.max_seq_len = a.max_seq_len;
-  p.nteams = static_cast<int>(teams);
-  p.piece_cost = kDefaultPieceCost;
-  const size_t nslots = static_cast<size_t>(teams_cap) + static_cast<size_t>(a.batch);
-  uint8_t* ws = static_cast<uint8_t*>(a.workspace);
-  p.piece_ctr = reinterpret_cast<unsigned*>(ws);
-  p.part_o = reinterpret_cast<float*>(ws + kCounterBytes);
-  p.part_lse = reinterpret_cast<float*>(ws + kCounterBytes + align_up(nslots * a.kv_heads * rows * kD * sizeof(float), 256));
   p.out = static_cast<__half*>(a.out);
-  p.out_stride_b = a.out_stride_b;
+  p.out_stride_t = a.out_stride_b;
   p.out_stride_h = a.out_stride_h;
   p.status = a.status;
-  const bool programmatic = (a.flags & B200KV_DECODE_SERIALIZED) == 0;
-  return rows == 8 ? launch_decode<8>(p, programmatic, stream) : launch_decode<16>(p, programmatic, stream);
+  return run_decode(p, a.q_heads, s, a.workspace, a.workspace_bytes, a.max_seq_len,
+                    (a.flags & B200KV_DECODE_SERIALIZED) == 0, stream);
+}
+
+// A chunk of at most kChunkColumns columns; the arguments have been checked (kv4_paged_prefill).
+int kv4_paged_chunk(const Kv4PrefillArgs& k, cudaStream_t stream) {
+  const PrefillArgs& a = k.args;
+  if (misaligned(a.q, 16) || a.q_stride_t % 8 != 0 || a.q_stride_h % 8 != 0 || misaligned(k.workspace, 16)) return B200KV_EALIGN;
+  Shape s;
+  const int rc = shape_of(static_cast<int>(a.max_q_len), a.q_heads, a.kv_heads, &s);
+  if (rc != B200KV_OK) return rc;
+  Kv4Params p{};
+  p.q = static_cast<const __half*>(a.q);
+  p.q_stride_t = a.q_stride_t;
+  p.q_stride_h = a.q_stride_h;
+  p.pool = static_cast<const uint8_t*>(k.pool);
+  p.pool_pages = static_cast<int>(k.pool_pages);
+  p.page_stride = k.page_stride_bytes;
+  p.table = a.table;
+  p.table_row_stride = a.table_row_stride;
+  p.table_kind = a.table_kind;
+  p.table_rows = a.table_rows;
+  p.row_ids = a.req_ids;
+  p.lens = a.ctx_lens;
+  p.q_lens = a.q_lens;
+  p.q_start = a.q_start;
+  p.lens_i64 = a.lens_i64;
+  p.batch = a.batch;
+  p.kv_heads = a.kv_heads;
+  const int64_t width = a.table_cols * (a.table_kind == B200KV_TABLE_BLOCK ? kPS : 1);
+  p.max_seq_len = static_cast<int>(width < (1 << 30) ? width : (1 << 30));
+  p.max_q_len = static_cast<int>(a.max_q_len);
+  p.total_q = a.total_q;
+  p.scale_log2 = a.scale_log2;
+  p.out = static_cast<__half*>(a.out);
+  p.out_stride_t = a.out_stride_t;
+  p.out_stride_h = a.out_stride_h;
+  p.status = a.status;
+  return run_decode(p, a.q_heads, s, k.workspace, k.workspace_bytes, p.max_seq_len, true, stream);
 }
 
 }  // namespace b200kv

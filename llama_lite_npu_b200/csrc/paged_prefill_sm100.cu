@@ -215,6 +215,7 @@ struct PrefillParams {
   const uint8_t* pool;
   int64_t pool_pages, page_stride;
   int kv_heads;
+  int64_t max_q_len;
   int one_tile;           // a CTA takes one query tile instead of two
 };
 
@@ -251,9 +252,10 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     cudaTriggerProgrammaticLaunchCompletion();
   };
   const int table_row = p.req_ids ? __ldg(p.req_ids + b) : b;
+  const bool too_long = kKv4 && q_len > static_cast<int64_t>(p.max_q_len);   // more than the launch was sized for
   // A stale length or request id must not become a read outside the table: such a request is
   // reported and skipped.
-  if (q_len < 0 || ctx < 0 || q_len > p.total_q || ctx > p.table_tokens || ctx + q_len > p.table_tokens ||
+  if (too_long || q_len < 0 || ctx < 0 || q_len > p.total_q || ctx > p.table_tokens || ctx + q_len > p.table_tokens ||
       (p.table_kind != B200KV_TABLE_DENSE && (table_row < 0 || table_row >= p.table_rows))) {
     set_status(p.status, B200KV_DEV_BAD_LENGTH);
     leave_early();
@@ -1017,6 +1019,9 @@ int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
   if (a.table_kind == B200KV_TABLE_DENSE) return B200KV_EINVAL;
   rc = kv4_check_pool(k.pool, k.pool_pages, k.page_stride_bytes, a.kv_heads);
   if (rc != B200KV_OK) return rc;
+  // A few query rows over a long context: streamed like a decode step (kv4_decode.cu).
+  if (k.workspace != nullptr && kv4_chunk_workspace_bytes(a.batch, a.max_q_len, a.q_heads, a.kv_heads, a.head_dim) > 0)
+    return kv4_paged_chunk(k, stream);
   CUtensorMap qmap;
   rc = encode_q_tensor_map(&qmap, a.q, a.total_q, a.q_stride_t, a.q_stride_h, a.q_heads);
   if (rc != B200KV_OK) return rc;
@@ -1024,6 +1029,7 @@ int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
   p.pool = static_cast<const uint8_t*>(k.pool);
   p.pool_pages = k.pool_pages;
   p.page_stride = k.page_stride_bytes;
+  p.max_q_len = a.max_q_len;
   // Two query tiles per CTA balance the causal work of many CTAs; where those pairs would leave SMs empty,
   // one tile per CTA spreads a long tile list over twice as many (chunks of 500 on contexts of 9-16 k,
   // 2 requests, 32/4 heads: 520 us paired on 64 CTAs, 273 us as 128).

@@ -854,21 +854,30 @@ def _status_ptr(device_index: int) -> int:
     return st.data_ptr()
 
 
-def kv4_decode_workspace(device_index: int, stream: int, batch: int, q_heads: int, kv_heads: int,
-                         head_dim: int) -> torch.Tensor:
-    """Scratch of :func:`flash_decoding_kv4`: arrival counters (zero between calls) and partials.
+def _kv4_workspace_need(device_index: int, batch: int, max_q_len: int, q_heads: int, kv_heads: int) -> int:
+    """Bytes of scratch of a decode step (``max_q_len`` 0) or a chunk; 0 for a chunk that needs none.
+    The device is current."""
+    key = ("kv4", device_index, batch, max_q_len, q_heads, kv_heads)
+    need = _workspace_need.get(key)
+    if need is None:
+        lib = _lib.lib()
+        if max_q_len:
+            need = lib.b200kv_kv4_chunk_workspace_bytes(batch, max_q_len, q_heads, kv_heads, KV4_HEAD_DIM)
+        else:
+            need = lib.b200kv_kv4_decode_workspace_bytes(batch, q_heads, kv_heads, KV4_HEAD_DIM)
+            if need == 0:
+                raise ValueError("unsupported decode shape: q_heads/kv_heads must be an integer <= 16, batch at most "
+                                 f"4096 and batch * kv_heads at most {DECODE_COUNTER_BYTES // 4}")
+        _workspace_need[key] = need
+    return need
+
+
+def kv4_workspace(device_index: int, stream: int, need: int) -> torch.Tensor:
+    """Scratch of the 4-bit attention operators: arrival counters (zero between calls) and partials.
 
     Eager calls of one stream share one buffer (grown on demand): they follow one another.  A graph under
     capture gets a buffer of its own out of its memory pool, whose counters are cleared by a node of
     the graph, so graphs may be replayed next to each other and next to eager calls."""
-    key = ("kv4", device_index, batch, q_heads, kv_heads, head_dim)
-    need = _workspace_need.get(key)
-    if need is None:
-        need = _lib.lib().b200kv_kv4_decode_workspace_bytes(batch, q_heads, kv_heads, head_dim)
-        if need == 0:
-            raise ValueError("unsupported decode shape: head_dim must be 128, q_heads/kv_heads an integer <= 16 and "
-                             f"batch * kv_heads at most {DECODE_COUNTER_BYTES // 4}")
-        _workspace_need[key] = need
     where = (device_index, stream)
     capture = _capture_of(stream) if _capturing() else 0
     if capture:
@@ -1067,7 +1076,7 @@ def flash_decoding_kv4(
         _debug_check_lengths(b_seq_len, max_len, b_req_idx, tbl_rows, "decode")
     with _on_device(dev):
         stream = _stream(dev)
-        ws = kv4_decode_workspace(dev, stream, batch, q_heads, kv_heads, d)
+        ws = kv4_workspace(dev, stream, _kv4_workspace_need(dev, batch, 0, q_heads, kv_heads))
         rc = _lib.lib().b200kv_kv4_paged_decode(
             q.data_ptr(), q_sb, q_sh, ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols,
             rows_ptr, lens_ptr, b_seq_len.dtype is torch.int64, batch, q_heads, kv_heads, d, int(page_size), float(qk_scale),
@@ -1113,13 +1122,22 @@ def paged_chunk_flash_attention_kv4(
     if _DEBUG:
         width = tbl_cols * (page_size if kind == TABLE_BLOCK else 1)
         _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, tbl_rows, "paged prefill")
-        _debug_check_lengths(q_seq_lens, int(max_q_len), None, 0, "paged prefill chunk")
+        _debug_check_lengths(q_seq_lens, int(max_q_len), None, 0, "paged prefill chunk")   # longer ones are skipped
+    max_q_len = int(max_q_len)
     with _on_device(dev):
+        stream = _stream(dev)
+        # at most 128 columns (rows x heads of a group) are streamed like a decode step, with its scratch
+        need = _kv4_workspace_need(dev, batch, max_q_len, q_heads, kv_heads) if 0 < max_q_len <= 128 else 0
+        ws_ptr, ws_bytes = 0, 0
+        if need:
+            ws = kv4_workspace(dev, stream, need)
+            ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
         rc = _lib.lib().b200kv_kv4_paged_prefill(
             q.data_ptr(), q.stride(0) if total_q > 1 else q_heads * d, q.stride(1) if q_heads > 1 else d,
             ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols, ids_ptr, start_ptr, ctx_ptr,
-            qlen_ptr, q_seq_lens.dtype is torch.int64, batch, total_q, int(max_q_len), q_heads, kv_heads, d,
-            int(page_size), float(sm_scale), output.data_ptr(), q_heads * d, d, _status_ptr(dev), _stream(dev))
+            qlen_ptr, q_seq_lens.dtype is torch.int64, batch, total_q, max_q_len, q_heads, kv_heads, d,
+            int(page_size), float(sm_scale), output.data_ptr(), q_heads * d, d, ws_ptr, ws_bytes, _status_ptr(dev),
+            stream)
     _kv4_done(rc, dev)
     return output
 

@@ -20,7 +20,7 @@ import math
 import pytest
 import torch
 
-from llama_lite_npu_b200 import kernels, workloads as W
+from llama_lite_npu_b200 import _lib, kernels, workloads as W
 from oracle import kv4_oracle as K4
 
 pytestmark = pytest.mark.gpu
@@ -384,6 +384,67 @@ def test_prefill_nan_reaches_only_the_rows_that_see_it():
     assert bool(got[100:150, :2, 64:96].isnan().all()) and not bool(got[100:120, :, :64].isnan().any())
     assert bool(got[120:150, 2:].isnan().all())
     _within(got, want, tol)
+
+
+CHUNK = [   # at most 128 columns (query rows x heads of a group): streamed like a decode step
+    ([40], [1], 8, 1), ([33, 17, 500], [7, 7, 7], 8, 1), ([64, 1, 2000], [4, 1, 2], 16, 1), ([300, 5], [5, 5], 3, 3),
+    ([129, 700], [16, 3], 8, 2), ([90, 1500, 31], [2, 8, 8], 64, 8), ([200, 100], [3, 0], 20, 2), ([4000], [6], 10, 1),
+    ([21, 22, 23, 24] * 40, [1, 2, 3, 4] * 40, 4, 1), ([64], [64], 1, 1),
+]
+
+
+@pytest.mark.parametrize("lens, q_lens, qh, kvh", CHUNK)
+def test_short_chunks(lens, q_lens, qh, kvh):
+    c = Case(sum(lens) + len(lens), lens, qh, kvh, q_lens)
+    want, _, tol = c.want()
+    pool = c.pool.to(DEV)
+    got = c.prefill("block", pool=pool)
+    _within(got, want, tol)
+    _within(c.prefill("token", torch.int32), want, tol)
+    # without a workspace the same call goes through the tensor-core tiles
+    lib, ql = _lib.lib(), torch.tensor(c.q_lens)
+    q, tbl, rows = c.q.to(DEV), c.tables("block"), c.rows.to(DEV)
+    start, ctx, qd = (ql.cumsum(0) - ql).int().to(DEV), (torch.tensor(c.lens) - ql).to(DEV), ql.to(DEV)
+    out = torch.zeros_like(q)
+    need = lib.b200kv_kv4_chunk_workspace_bytes(len(lens), max(q_lens), qh, kvh, 128)
+    assert need > 0
+    args = (q.data_ptr(), q.stride(0), q.stride(1), pool.data_ptr(), pool.shape[0], pool.stride(0), tbl.data_ptr(),
+            tbl.stride(0), 0, tbl.shape[0], tbl.shape[1], rows.data_ptr(), start.data_ptr(), ctx.data_ptr(),
+            qd.data_ptr(), 1, len(lens), q.shape[0], max(q_lens), qh, kvh, 128, 16, SCALE * LOG2E, out.data_ptr(),
+            out.stride(0), out.stride(1))
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.b200kv_kv4_paged_prefill(*args, 0, 0, kernels.status_tensor(0).data_ptr(), stream) == 0
+    _within(out, want, tol)
+    # and one that is too small is refused
+    assert lib.b200kv_kv4_paged_prefill(*args, pool.data_ptr(), need - 1, None, stream) == 4
+
+
+def test_short_chunk_nan_reaches_only_the_rows_that_see_it():
+    c = Case(63, [150, 90], 8, 2, [8, 8])
+    x = _randn(64, (150, 4, 128))
+    x[146, 2, 70] = float("nan")        # V of head 0, group 2, at the chunk's row 4
+    x[148, 1, 0] = float("inf")         # K of head 1 at row 6
+    K4.append(x, c.slots[0], c.pool)
+    c.values[0] = K4.rows_of(c.pool, c.slots[0])
+    want, _, tol = c.want()
+    got = c.prefill().cpu()
+    assert not bool(got[:4].isnan().any()) and not bool(got[8:].isnan().any())
+    assert bool(got[4:8, :4, 64:96].isnan().all()) and not bool(got[4:6, :, :64].isnan().any())
+    assert bool(got[6:8, 4:].isnan().all())
+    _within(got, want, tol)
+
+
+@pytest.mark.parametrize("max_q", [4, 200])
+def test_a_chunk_longer_than_stated_is_skipped(max_q):
+    c = Case(65, [300, 300], 8, 1, [max_q // 2, max_q + 1])
+    want, _, tol = c.want()
+    ql = torch.tensor(c.q_lens)
+    got = kernels.paged_chunk_flash_attention_kv4(
+        c.q.to(DEV), c.pool.to(DEV), SCALE * LOG2E, c.tables("block"), c.rows.to(DEV), (ql.cumsum(0) - ql).int().to(DEV),
+        (torch.tensor(c.lens) - ql).to(DEV), ql.to(DEV), max_q, table_kind="block")
+    with pytest.raises(RuntimeError, match="length"):
+        kernels.check_status(0)
+    _within(got[: max_q // 2], want[: max_q // 2], tol[: max_q // 2])
 
 
 def test_prefill_skips_a_request_the_table_cannot_hold():

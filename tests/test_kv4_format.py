@@ -142,7 +142,7 @@ def test_prefill_refusals(built_lib, kw, code):
     a.update(kw)
     assert built_lib.b200kv_kv4_paged_prefill(
         a["q"], 1024, 128, a["pool"], a["pages"], 2 * 4 * 1152, a["table"], 10, a["kind"], 2, 10, A, A, A, A, 0,
-        a["batch"], a["total"], a["maxq"], a["qh"], 4, 128, a["ps"], 0.1, A, a["os"], 128, None, None) == code
+        a["batch"], a["total"], a["maxq"], a["qh"], 4, 128, a["ps"], 0.1, A, a["os"], 128, None, 0, None, None) == code
 
 
 def test_capture_id_wants_a_place_for_the_answer(built_lib):
