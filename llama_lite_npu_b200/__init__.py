@@ -2,7 +2,8 @@
 ``kv_engine`` / paged-attention modules.
 
 * :mod:`.kernels` — ``update_kv_buffer``, ``flash_decoding``,
-  ``paged_chunk_flash_attention``, ``flash_attention2_no_pad`` (CUDA, via libb200kv.so)
+  ``paged_chunk_flash_attention``, ``flash_attention2_no_pad`` (CUDA, via libb200kv.so), and the same
+  over a 4-bit cache (``*_kv4``)
 * :mod:`.paged_attention` — ``PagedKVCacheManager``, ``PagedReqTokensManager``
 * :mod:`.kv_engine` — refcounts, prefix cache, prefill packer and chunk planner
 """
@@ -19,10 +20,17 @@ from .kv_engine import (  # noqa: F401
 )
 from .paged_attention import PagedKVCacheManager, PagedReqTokensManager  # noqa: F401
 from .kernels import (  # noqa: F401
+    empty_kv4_buffer,
     flash_attention2_no_pad,
     flash_decoding,
+    flash_decoding_kv4,
+    fused_qk_norm_rope_append_kv4,
+    gather_kv_buffer_kv4,
     paged_chunk_flash_attention,
+    paged_chunk_flash_attention_kv4,
     update_kv_buffer,
+    update_kv_buffer_kv4,
+    update_kv_buffer_kv4_split,
     update_kv_buffer_split,
 )
 

@@ -69,18 +69,24 @@ class PendingAdvance:
 
 
 class PagedKVExecutor:
-    """Owns the page pool, the request tables, the prefix caches and ``atten_info``."""
+    """Owns the page pool, the request tables, the prefix caches and ``atten_info``.
+
+    ``kv_format="kv4"`` keeps the cache in 4 bits (``PagedKVCacheManager``): the attention call
+    sequences then append through the quantising operators and read through the ``*_kv4`` ones;
+    everything else — requests, pages, prefix sharing, metadata, graphs — is the same."""
 
     def __init__(self, num_layers: int, num_kv_heads: int, head_dim: int, num_pages: int,
                  max_requests: int, max_seq_len: int, page_size: int = 16,
                  dtype: torch.dtype = torch.float16, device: str = "cuda:0",
-                 prefix_cache_entries: int = 128, prefix_cache_block_entries: int = 4096):
+                 prefix_cache_entries: int = 128, prefix_cache_block_entries: int = 4096,
+                 kv_format: str = "fp16"):
         self.device = device
+        self.kv_format = kv_format
         self.page_size = page_size
         self.num_kv_heads = num_kv_heads
         self.use_paged_attn = True
         self.kv_mem_manager = PagedKVCacheManager(num_layers, num_kv_heads, head_dim, num_pages,
-                                                  page_size, dtype, device)
+                                                  page_size, dtype, device, kv_format)
         self.req_tokens_manager = PagedReqTokensManager(max_requests, max_seq_len,
                                                         self.kv_mem_manager, device)
         self.atten_info = AttentionInfo()
@@ -367,16 +373,40 @@ class PagedKVExecutor:
         same computation with zero history."""
         from . import kernels
 
-        info, kh = self.atten_info, self.num_kv_heads
+        info = self.atten_info
         pool = info.kv_buffer[layer_index]
-        kernels.update_kv_buffer_split(xk, xv, info.cur_select_index, pool)
+        if self.kv_format == "kv4":
+            kernels.update_kv_buffer_kv4_split(xk, xv, info.cur_select_index, pool)
+        else:
+            kernels.update_kv_buffer_split(xk, xv, info.cur_select_index, pool)
+        return self._attend_context(xq, pool, qk_scale)
+
+    def _attend_context(self, xq, pool, qk_scale: float) -> torch.Tensor:
+        """Attention of the active prefill batch over a pool that holds its rows already."""
+        from . import kernels
+
+        info, kh = self.atten_info, self.num_kv_heads
         if info.is_paged_chunk_prefill:
             ctx, qlen, max_q = info.chunk_context_len, info.chunk_q_seq_len, info.max_actual_q_seq_len
         else:
             ctx, qlen, max_q = torch.zeros_like(info.b_seq_len), info.b_seq_len, info.max_actual_seq_len
+        if self.kv_format == "kv4":
+            return kernels.paged_chunk_flash_attention_kv4(
+                xq, pool, qk_scale, info.b_req_block_table, info.b_req_idx, info.b_start_loc, ctx, qlen, max_q,
+                table_kind="block")
         return kernels.paged_chunk_flash_attention(
             xq, pool[:, :kh, :], pool[:, kh:, :], qk_scale, info.b_req_block_table, info.b_req_idx,
             info.b_start_loc, ctx, qlen, max_q, table_kind="block")
+
+    def _attend_token_kv4(self, xq, pool, qk_scale: float) -> torch.Tensor:
+        """Decode attention of the active batch over a 4-bit pool whose append was the launch before: that
+        launch has waited for whatever produced the step's metadata, so this one may start early."""
+        from . import kernels
+
+        info = self.atten_info
+        return kernels.flash_decoding_kv4(
+            xq, pool, qk_scale, info.b_req_block_table, info.b_seq_len, info.max_actual_seq_len,
+            b_req_idx=info.b_req_idx, table_kind="block")
 
     def token_forward(self, xq, xk, xv, layer_index: int, qk_scale: float) -> torch.Tensor:
         """Decode attention of one layer: append the new token's K/V, then attend.  Table rows are
@@ -384,6 +414,10 @@ class PagedKVExecutor:
         from . import kernels
 
         info = self.atten_info
+        if self.kv_format == "kv4":
+            pool = info.kv_buffer[layer_index]
+            kernels.update_kv_buffer_kv4_split(xk, xv, info.cur_select_index, pool)
+            return self._attend_token_kv4(xq, pool, qk_scale)
         # one launch: append + decode.  The first layer's launch may directly follow the kernel or
         # copy that produced the step's lengths, so it gives up its overlap with its predecessor.
         return kernels.append_flash_decoding_split(
@@ -403,6 +437,10 @@ class PagedKVExecutor:
 
         info, kh = self.atten_info, self.num_kv_heads
         pool = info.kv_buffer[layer_index]
+        if self.kv_format == "kv4":
+            kernels.fused_qk_norm_rope_append_kv4(xq, xkv, q_norm_weight, k_norm_weight, eps, cos, sin,
+                                                  info.cur_select_index, pool)
+            return self._attend_token_kv4(xq, pool, qk_scale)
         kernels.fused_qk_norm_rope_append(xq, xkv, q_norm_weight, k_norm_weight, eps, cos, sin,
                                           info.cur_select_index, pool)
         return kernels.flash_decoding(
@@ -415,14 +453,8 @@ class PagedKVExecutor:
         ``qk_scale`` is the softmax scale times log2(e) as for ``context_forward``."""
         from . import kernels
 
-        info, kh = self.atten_info, self.num_kv_heads
+        info = self.atten_info
         pool = info.kv_buffer[layer_index]
-        kernels.fused_qk_norm_rope_append(xq, xkv, q_norm_weight, k_norm_weight, eps, cos, sin,
-                                          info.cur_select_index, pool)
-        if info.is_paged_chunk_prefill:
-            ctx, qlen, max_q = info.chunk_context_len, info.chunk_q_seq_len, info.max_actual_q_seq_len
-        else:
-            ctx, qlen, max_q = torch.zeros_like(info.b_seq_len), info.b_seq_len, info.max_actual_seq_len
-        return kernels.paged_chunk_flash_attention(
-            xq, pool[:, :kh, :], pool[:, kh:, :], qk_scale, info.b_req_block_table, info.b_req_idx,
-            info.b_start_loc, ctx, qlen, max_q, table_kind="block")
+        append = kernels.fused_qk_norm_rope_append_kv4 if self.kv_format == "kv4" else kernels.fused_qk_norm_rope_append
+        append(xq, xkv, q_norm_weight, k_norm_weight, eps, cos, sin, info.cur_select_index, pool)
+        return self._attend_context(xq, pool, qk_scale)

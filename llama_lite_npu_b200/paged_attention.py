@@ -28,10 +28,16 @@ from typing import List, Optional, Tuple
 import numpy as np
 import torch
 
+from .kernels import KV4_HEAD_DIM, KV4_PAGE_SIZE, empty_kv4_buffer
+
 
 class PagedKVCacheManager:
     """Fixed-size page pool: one ``[num_pages*page_size, 2*kv_heads, head_dim]`` tensor per
-    layer (K heads first, then V heads, inside a token row) plus host refcounts."""
+    layer (K heads first, then V heads, inside a token row) plus host refcounts.
+
+    ``kv_format="kv4"`` makes the layers' tensors 4-bit pools (``kernels.empty_kv4_buffer``:
+    uint8 ``[num_pages, 2*kv_heads, 1152]``, 9/32 of the bytes) with the same pages and slots; the
+    ``*_kv4`` operators work on them."""
 
     def __init__(
         self,
@@ -42,7 +48,14 @@ class PagedKVCacheManager:
         page_size: int = 16,
         dtype: torch.dtype = torch.float16,
         device: str = "cuda:0",
+        kv_format: str = "fp16",
     ):
+        if kv_format not in ("fp16", "kv4"):
+            raise ValueError(f"kv_format must be 'fp16' or 'kv4' (got {kv_format!r})")
+        if kv_format == "kv4" and (head_dim != KV4_HEAD_DIM or page_size != KV4_PAGE_SIZE):
+            raise ValueError(f"a 4-bit pool has head_dim {KV4_HEAD_DIM} and pages of {KV4_PAGE_SIZE} tokens "
+                             f"(got {head_dim} and {page_size})")
+        self.kv_format = kv_format
         self.num_layers = num_layers
         self.num_kv_heads = num_kv_heads
         self.head_dim = head_dim
@@ -53,10 +66,13 @@ class PagedKVCacheManager:
 
         self.max_tokens = num_pages * page_size
         self.max_num_tokens = self.max_tokens
-        self.gpu_kv_buffer = [
-            torch.empty((self.max_tokens, 2 * num_kv_heads, head_dim), dtype=dtype, device=device)
-            for _ in range(num_layers)
-        ]
+        if kv_format == "kv4":
+            self.gpu_kv_buffer = [empty_kv4_buffer(num_pages, num_kv_heads, device) for _ in range(num_layers)]
+        else:
+            self.gpu_kv_buffer = [
+                torch.empty((self.max_tokens, 2 * num_kv_heads, head_dim), dtype=dtype, device=device)
+                for _ in range(num_layers)
+            ]
 
         # Ownership is scheduler metadata and stays on the host.
         self.page_free = torch.ones(num_pages, dtype=torch.bool, device="cpu")
