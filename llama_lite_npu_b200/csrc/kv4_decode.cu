@@ -32,8 +32,8 @@
 // A warp streams its own pages: page k of a piece belongs to warp k % 4, two of them make up one step
 // (one wait, one look at the maxima, one request, and twice the independent arithmetic in flight).  Every
 // warp keeps a ring of kStages page pairs (2 x (K block + V block), 4608 bytes) that its own lanes fill with
-// 16-byte asynchronous copies, nine per lane and pair, as soon as the slot has been read (bulk copies by
-// one lane cost three times the instructions here: their operands are uniform registers).  No producer
+// 16-byte asynchronous copies, nine per lane and pair, as soon as the slot has been read (bulk copies, and
+// cache hints, cost several times the instructions here: their operands are uniform registers).  No producer
 // warp, no barrier in the steady state; the blocks are stored in the order in which the lanes read
 // them (conflict-free 16-byte shared loads).  The page table is read 32 entries at a time, one block of
 // entries ahead of use.
@@ -59,6 +59,7 @@ constexpr int kPairBytes = 2 * kPageBytes;
 constexpr int kRingBytes = kWarps * kStages * kPairBytes;
 constexpr int kMinPagesPerTeam = 4;                // a team is not worth launching for fewer pages
 constexpr int kPieceCost = 16;
+constexpr float kNoScore = -3.0e38f;               // the reference of sums over no token; finite, so that differences are
 // Resident CTAs per SM.  Three of them leave 168 registers, which a step of two pages needs (four spill
 // and were slower: 36.4 against 33.0 us on 32 sequences of 1-4 k tokens, 64/8 heads).
 constexpr int ctas_per_sm(int rows) { return rows == 8 ? 3 : 2; }
@@ -148,8 +149,8 @@ __device__ __forceinline__ void pdl_wait_then_trigger() {
   cudaTriggerProgrammaticLaunchCompletion();
 }
 
-__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src, uint64_t policy) {
-  asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;\n" : : "r"(dst), "l"(src), "l"(policy) : "memory");
+__device__ __forceinline__ void async_copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" : : "r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void async_commit() { asm volatile("cp.async.commit_group;\n" : : : "memory"); }
 template <int N>
@@ -440,7 +441,7 @@ struct PageStream {
 // S^T of 16 tokens: k_at and c_at are this lane's chunk of token r and that token's scales.
 template <int NB>
 __device__ __forceinline__ void page_scores(const uint8_t* k_at, const uint8_t* c_at, const uint32_t (&qf)[NB][8][2],
-                                            float scale, float (&s)[NB][4]) {
+                                            float (&s)[NB][4]) {
   const uint4 k0 = *reinterpret_cast<const uint4*>(k_at), k1 = *reinterpret_cast<const uint4*>(k_at + 8 * kv4::kRowBytes);
   const uint2 c0 = *reinterpret_cast<const uint2*>(c_at), c1 = *reinterpret_cast<const uint2*>(c_at + 8 * kv4::kScaleBytes);
   const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
@@ -463,10 +464,6 @@ __device__ __forceinline__ void page_scores(const uint8_t* k_at, const uint8_t* 
       }
     }
   }
-#pragma unroll
-  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[nb][i] *= scale;
 }
 
 // V scales of tokens 2jq, 2jq+1 | 2jq+8, 2jq+9 as fp16 pairs per group.
@@ -560,7 +557,7 @@ __device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc
       l += __shfl_xor_sync(0xffffffffu, l, 4);
       l += __shfl_xor_sync(0xffffffffu, l, 8);
       l += __shfl_xor_sync(0xffffffffu, l, 16);
-      if (r == 0) merge_ml[warp * ROWS + nb * 8 + 2 * jq + h] = make_float2(m_ref[nb][h], l);
+      if (r == 0) merge_ml[warp * ROWS + nb * 8 + 2 * jq + h] = make_float2(l == 0.f ? kNoScore : m_ref[nb][h], l);
     }
   }
   cta_bar();
@@ -586,7 +583,7 @@ __device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc
   for (int nb = 0; nb < NB; ++nb) {
     // (m, l) of the four warps for this lane's two heads
     float2 ml[kWarps][2];
-    float top[2] = {-INFINITY, -INFINITY};
+    float top[2] = {kNoScore, kNoScore};
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float4 v = *reinterpret_cast<const float4*>(merge_ml + w * ROWS + nb * 8 + 2 * jq);
@@ -602,8 +599,7 @@ __device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc
     for (int w = 0; w < kWarps; ++w)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        // a warp without a page of this piece, or with only NaN scores: its sums enter as they are
-        wt[w][h] = ml[w][h].x == -INFINITY ? 1.f : fast_exp2(ml[w][h].x - top[h]);
+        wt[w][h] = fast_exp2(ml[w][h].x - top[h]);
         l[h] += wt[w][h] * ml[w][h].y;
       }
 #pragma unroll
@@ -640,7 +636,7 @@ __device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     Weighted sum[2];
-    float top[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    float top[2] = {kNoScore, kNoScore}, l[2] = {0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < 2; ++k)
 #pragma unroll
@@ -657,7 +653,7 @@ __device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc
           for (int k = 0; k < 2; ++k)
             v[i][k] = __ldcg(p.part_o + (sl * kParts + nb * 8 + 2 * warp + k) * 32 + lane);
         } else {
-          ml[i] = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+          ml[i] = make_float4(kNoScore, 0.f, kNoScore, 0.f);
           v[i][0] = v[i][1] = make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
@@ -670,7 +666,7 @@ __device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc
       float re[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        re[h] = was[h] == -INFINITY ? 1.f : fast_exp2(was[h] - top[h]);
+        re[h] = fast_exp2(was[h] - top[h]);
         l[h] *= re[h];
       }
 #pragma unroll
@@ -679,8 +675,7 @@ __device__ __forceinline__ void finish_piece(const Kv4Params& p, const Piece& pc
         for (int i = 0; i < 4; ++i) sum[k].acc[i] *= re[i & 1];
 #pragma unroll
       for (int i = 0; i < kBatch; ++i) {
-        const float w0 = ml[i].x == -INFINITY ? 1.f : fast_exp2(ml[i].x - top[0]);
-        const float w1 = ml[i].z == -INFINITY ? 1.f : fast_exp2(ml[i].z - top[1]);
+        const float w0 = fast_exp2(ml[i].x - top[0]), w1 = fast_exp2(ml[i].z - top[1]);
         l[0] += w0 * ml[i].y;
         l[1] += w1 * ml[i].w;
 #pragma unroll
@@ -754,30 +749,22 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
   }
   if (!range.any) return;
 
-  const uint64_t policy = l2_evict_first_policy();
-  // The next two pages into ring slot `stage`: 288 16-byte pieces, piece i * 32 + lane by this lane; 72
-  // pieces are a block, the blocks are K and V of the first page, K and V of the second.
-  const uint32_t ring_dst = smem_u32(ring) + lane * 16;
+  // The next two pages into ring slot `stage`.  The pair is four blocks (K and V of the first page, K and V of
+  // the second); eight lanes copy a block, each of them every eighth of its 72 16-byte pieces, so that a lane
+  // has one address.
+  const int my_block = lane >> 3;
+  const uint8_t* my_rows = k_rows + ((my_block & 1) ? v_from_k : 0) + (lane & 7) * 16;
+  const uint32_t my_dst = smem_u32(ring) + my_block * kv4::kBlockBytes + (lane & 7) * 16;
+  const uint32_t page_stride = static_cast<uint32_t>(p.page_stride);   // the host refuses strides of 2^31 and more
   auto request = [&](int stage) {
     if (st.more()) {
       const bool two = st.cnt - st.m >= 2;
-      const int32_t id0 = __shfl_sync(0xffffffffu, st.ids, st.m & 31);
-      const int32_t id1 = __shfl_sync(0xffffffffu, st.ids, (st.m & 31) + 1);
-      const uint8_t* k0 = k_rows + id0 * p.page_stride + lane * 16;
-      const uint8_t* v0 = k0 + v_from_k - kv4::kBlockBytes;
-      const uint8_t* k1 = k_rows + id1 * p.page_stride + lane * 16 - 2 * kv4::kBlockBytes;
-      const uint8_t* v1 = k1 + v_from_k - kv4::kBlockBytes;
-      const uint32_t dst = ring_dst + stage * kPairBytes;
-      async_copy16(dst, k0, policy);
-      async_copy16(dst + 512, k0 + 512, policy);
-      async_copy16(dst + 1024, (lane < 8 ? k0 : v0) + 1024, policy);
-      async_copy16(dst + 1536, v0 + 1536, policy);
-      if (two || lane < 16) async_copy16(dst + 2048, (lane < 16 ? v0 : k1) + 2048, policy);
-      if (two) {
-        async_copy16(dst + 2560, k1 + 2560, policy);
-        async_copy16(dst + 3072, (lane < 24 ? k1 : v1) + 3072, policy);
-        async_copy16(dst + 3584, v1 + 3584, policy);
-        async_copy16(dst + 4096, v1 + 4096, policy);
+      const int32_t id = __shfl_sync(0xffffffffu, st.ids, (st.m & 31) + (my_block >> 1));
+      if (two || my_block < 2) {
+        const uint8_t* src = my_rows + static_cast<uint64_t>(static_cast<uint32_t>(id)) * page_stride;
+        const uint32_t dst = my_dst + stage * kPairBytes;
+#pragma unroll
+        for (int i = 0; i < kv4::kBlockBytes / 128; ++i) async_copy16(dst + i * 128, src + i * 128);
       }
       st.advance(p, walk, warp, lane);
     }
@@ -826,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
         qf[nb][2 * g + 1][0] = v.z;
         qf[nb][2 * g + 1][1] = v.w;
       }
-      m_ref[nb][0] = m_ref[nb][1] = -INFINITY;
+      m_ref[nb][0] = m_ref[nb][1] = 0.f;
       l_run[nb][0] = l_run[nb][1] = 0.f;
     }
 #pragma unroll
@@ -857,9 +844,16 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
       uint32_t sv[2][4][2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        page_scores<NB>(k_at + pair + h * kPageBytes, kc_at + pair + h * kPageBytes, qf, p.scale_log2, s[h]);
+        page_scores<NB>(k_at + pair + h * kPageBytes, kc_at + pair + h * kPageBytes, qf, s[h]);
         page_v_scales(vc_at + pair + h * kPageBytes, sv[h]);
       }
+      // scores relative to the reference, in the log2 domain
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[h][nb][i] = fmaf(s[h][nb][i], p.scale_log2, -m_ref[nb][i & 1]);
       if (masked) {
         // Rows past the length were never written and a missing second page was not loaded: they may
         // hold anything, NaN scales included.  Positions past a column's own are not for it.
@@ -889,13 +883,14 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int g = 0; g < 4; ++g) any_sv |= sv[h][g][0] | sv[h][g][1];
-      bool grow = ((any_sv + (0x8000u - sv_lim) * 0x10001u) & 0x80008000u) != 0;
+      // (The first step of a piece always goes there: it sets the reference.)
+      bool grow = m == 0 || ((any_sv + (0x8000u - sv_lim) * 0x10001u) & 0x80008000u) != 0;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           const float top = fmaxf(fmaxf(s[0][nb][i], s[0][nb][i + 2]), fmaxf(s[1][nb][i], s[1][nb][i + 2]));
-          grow |= top > m_ref[nb][i] + p_room;
+          grow |= top > p_room;
         }
       if (__any_sync(0xffffffffu, grow)) {
         uint32_t top2 = 0;
@@ -921,10 +916,17 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
             // the largest weight so far becomes 2^(p_room - 7), unless the reference is higher already
-            const float m_new = fmaxf(m_ref[nb][i], mx - (p_room - 7.f));
-            const float alpha = m_ref[nb][i] == -INFINITY ? 0.f : fast_exp2(m_ref[nb][i] - m_new);
-            m_ref[nb][i] = m_new;
+            float up = mx - (p_room - 7.f);
+            if (m == 0) up = mx > -INFINITY ? up : 0.f;   // nothing seen: nothing will be, positions only grow
+            else up = fmaxf(0.f, up);
+            const float alpha = m == 0 ? 0.f : fast_exp2(-up);
+            m_ref[nb][i] += up;
             l_run[nb][i] *= alpha;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              s[h][nb][i] -= up;
+              s[h][nb][i + 2] -= up;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               o[j][nb][i] *= alpha;
@@ -936,12 +938,10 @@ __global__ void __launch_bounds__(kThreads, ctas_per_sm(ROWS)) kv4_decode_kernel
       uint32_t pb[2][NB][2];
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        const float m0 = m_ref[nb][0] == -INFINITY ? 0.f : m_ref[nb][0];
-        const float m1 = m_ref[nb][1] == -INFINITY ? 0.f : m_ref[nb][1];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const float p0 = fast_exp2(s[h][nb][0] - m0), p1 = fast_exp2(s[h][nb][1] - m1);
-          const float p2 = fast_exp2(s[h][nb][2] - m0), p3 = fast_exp2(s[h][nb][3] - m1);
+          const float p0 = fast_exp2(s[h][nb][0]), p1 = fast_exp2(s[h][nb][1]);
+          const float p2 = fast_exp2(s[h][nb][2]), p3 = fast_exp2(s[h][nb][3]);
           l_run[nb][0] += p0 + p2;
           l_run[nb][1] += p1 + p3;
           pb[h][nb][0] = movmatrix_trans(pack_half2(p0, p1));
