@@ -637,10 +637,8 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     Item nxt = next_item(cur);
     int32_t id_nxt = raw_id(nxt);
     for (int n = 0, sl = 0, par = 1;; ++n) {
-      if (n >= kSlots && !mbar_wait_bounded(bar_empty + 8 * sl, par)) {
-        set_status(p.status, B200KV_DEV_WAIT_TIMEOUT);
-        break;
-      }
+      // The next item is opened before the slot is waited for: from a free slot to a full one only the
+      // conversion itself passes.
       if (nxt.np > 0) locate(nxt, id_nxt);
       const Item after = nxt.np > 0 ? next_item(nxt) : nxt;
       id_nxt = raw_id(after);     // in flight while this item is converted
@@ -661,6 +659,10 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
             if ((scales[u].y & 0x7c000000u) == 0x7c000000u) { scales[u].y &= 0xffffu; atomicMin(nan_pos + 3, pos); }
           }
         }
+      }
+      if (n >= kSlots && !mbar_wait_bounded(bar_empty + 8 * sl, par)) {
+        set_status(p.status, B200KV_DEV_WAIT_TIMEOUT);
+        break;
       }
       const uint32_t dst = dst_row + sl * kTileBytes;
 #pragma unroll
