@@ -807,8 +807,8 @@ def _table_arg(tbl: torch.Tensor, table_kind: str, dev: int):
 
 def _ints_arg(t: torch.Tensor, name: str, n: int, dev: int, wide: bool) -> int:
     """Pointer of a contiguous 1-D tensor of ``n`` int32 (or, where ``wide``, int64) values."""
-    if (t.dtype is not torch.int32 and not (wide and t.dtype is torch.int64)) or t.dim() != 1 \
-            or t.shape[0] != n or not t.is_contiguous():
+    dtype = t.dtype
+    if (dtype is not torch.int32 and not (wide and dtype is torch.int64)) or t.shape != (n,) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous 1-D {'int32 or int64' if wide else 'int32'} tensor of {n} values")
     if t.get_device() != dev:
         raise _off_device(name, t, dev)
@@ -830,6 +830,7 @@ def _rows_arg(t: torch.Tensor, name: str, heads: int, n: int, dev: int):
     return t.data_ptr(), s0 if n > 1 else heads * KV4_HEAD_DIM
 
 
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
 _capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing") else \
     torch.cuda.is_current_stream_capturing
 
@@ -918,7 +919,7 @@ def update_kv_buffer_kv4(KV_Values: torch.Tensor, Select_Index: torch.Tensor, KV
         return
     if _DEBUG:
         _debug_check_append(KV_Values, slots, pages * KV4_PAGE_SIZE)
-    with _on_device(dev):
+    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
         rc = _lib.lib().b200kv_kv4_append(k_ptr, k_ptr + kvh * KV4_HEAD_DIM * 2, n, stride, stride, slots.data_ptr(),
                                           ptr, pages, page_stride, kvh, KV4_HEAD_DIM, _status_ptr(dev), _stream(dev))
     _kv4_done(rc, dev)
@@ -936,7 +937,7 @@ def update_kv_buffer_kv4_split(xk: torch.Tensor, xv: torch.Tensor, Select_Index:
         return
     if _DEBUG:
         _debug_check_append(torch.cat([xk[:n], xv[:n]], dim=1), slots, pages * KV4_PAGE_SIZE)
-    with _on_device(dev):
+    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
         rc = _lib.lib().b200kv_kv4_append(k_ptr, v_ptr, n, k_stride, v_stride, slots.data_ptr(), ptr, pages, page_stride,
                                           kvh, KV4_HEAD_DIM, _status_ptr(dev), _stream(dev))
     _kv4_done(rc, dev)
@@ -991,7 +992,7 @@ def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_we
         return out
     if _DEBUG:
         _debug_check_append(xkv, slots, pages * KV4_PAGE_SIZE)
-    with _on_device(dev):
+    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
         rc = _lib.lib().b200kv_kv4_qk_norm_rope_append(
             q_ptr, out_ptr, q_stride, out_stride, xkv.data_ptr(), xkv.stride(0) if n > 1 else row,
             0 if q_norm_weight is None else q_norm_weight.data_ptr(),
@@ -1010,7 +1011,7 @@ def gather_kv_buffer_kv4(KV4_Buffer: torch.Tensor, Select_Index: torch.Tensor,
     slots = _slots_arg(Select_Index, dev)
     n, d = slots.shape[0], KV4_HEAD_DIM
     if out is None:
-        out = torch.empty((n, 2 * kvh, d), dtype=torch.float16, device=slots.device)
+        out = torch.empty(n, 2 * kvh, d, dtype=torch.float16, device=slots.device)
         out_ptr, out_stride = out.data_ptr(), 2 * kvh * d
     else:
         out_ptr, out_stride = _rows_arg(out, "out", 2 * kvh, n, dev)
@@ -1018,7 +1019,7 @@ def gather_kv_buffer_kv4(KV4_Buffer: torch.Tensor, Select_Index: torch.Tensor,
             raise ValueError(f"out must hold {n} rows")
     if n == 0:
         return out
-    with _on_device(dev):
+    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
         rc = _lib.lib().b200kv_kv4_gather(ptr, pages, page_stride, slots.data_ptr(), n, out_ptr, out_stride, kvh, d,
                                           _status_ptr(dev), _stream(dev))
     _kv4_done(rc, dev)
@@ -1062,7 +1063,7 @@ def flash_decoding_kv4(
     if not 0 <= max_len <= tbl_cols * (page_size if kind == TABLE_BLOCK else 1):
         raise ValueError("max_actual_seq_len exceeds the table width")
     if out is None:
-        out = torch.empty((batch, q_heads, d), dtype=torch.float16, device=q.device)
+        out = torch.empty(batch, q_heads, d, dtype=torch.float16, device=q.device)
         out_sb, out_sh = q_heads * d, d
     else:
         out_sb, out_sh, out_sd = out.stride() if out.dim() == 3 else (0, 0, 0)
@@ -1074,7 +1075,7 @@ def flash_decoding_kv4(
         return out
     if _DEBUG:
         _debug_check_lengths(b_seq_len, max_len, b_req_idx, tbl_rows, "decode")
-    with _on_device(dev):
+    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
         stream = _stream(dev)
         ws = kv4_workspace(dev, stream, _kv4_workspace_need(dev, batch, 0, q_heads, kv_heads))
         rc = _lib.lib().b200kv_kv4_paged_decode(
@@ -1116,7 +1117,7 @@ def paged_chunk_flash_attention_kv4(
     ids_ptr = _ints_arg(req_ids, "req_ids", batch, dev, False)
     start_ptr = _ints_arg(q_start_loc, "q_start_loc", batch, dev, False)
     total_q, q_heads, d = q.shape
-    output = torch.empty((total_q, q_heads, d), dtype=torch.float16, device=q.device)
+    output = torch.empty(total_q, q_heads, d, dtype=torch.float16, device=q.device)
     if total_q == 0 or q_heads == 0 or batch == 0:
         return output
     if _DEBUG:
@@ -1124,7 +1125,7 @@ def paged_chunk_flash_attention_kv4(
         _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, tbl_rows, "paged prefill")
         _debug_check_lengths(q_seq_lens, int(max_q_len), None, 0, "paged prefill chunk")   # longer ones are skipped
     max_q_len = int(max_q_len)
-    with _on_device(dev):
+    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
         stream = _stream(dev)
         # at most 128 columns (rows x heads of a group) are streamed like a decode step, with its scratch
         need = _kv4_workspace_need(dev, batch, max_q_len, q_heads, kv_heads) if 0 < max_q_len <= 128 else 0
