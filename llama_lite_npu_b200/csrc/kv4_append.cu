@@ -36,6 +36,11 @@ constexpr int kThreads = 256;
 constexpr int kD = kv4::kHeadDim;
 constexpr int kHalf = kD / 2;
 constexpr int kTokPerWarp = 4;
+// CTAs per SM that a grid is capped at; warps stride above it.  The copies balance best in many short CTAs
+// (4 / 8 / 32 / unlimited per SM: 124 / 123 / 119 / 122 us for 65 536 tokens appended and read back), the
+// fused form, whose warps set up more, in the four that are resident (64.6 / 64.9 / 66.3 / 66.9 us for 8205).
+constexpr int kCopyCtas = 32;
+constexpr int kPrologueCtas = 4;
 constexpr float kMaxScale = 9352.f;   // 7 * 9352 = 65464 is a value fp16 can hold after rounding
 
 struct AppendParams {
@@ -99,58 +104,74 @@ __device__ __forceinline__ void norm8(uint32_t (&x)[4], float rrms, const uint32
     x[i] = kv4::h2_mul(pack_half2(f.x * rrms, f.y * rrms), w[i]);
   }
 }
-__device__ __forceinline__ uint32_t h2_abs_max_nan(uint32_t a, uint32_t b) {   // of non-negative a; b taken absolute
+__device__ __forceinline__ uint32_t h2_max_nan(uint32_t a, uint32_t b) {
   uint32_t d;
-  asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b & 0x7fff7fffu));
+  asm("max.NaN.f16x2 %0, %1, %2;\n" : "=r"(d) : "r"(a), "r"(b));
   return d;
 }
-
-// One group's share of a lane: its 8 elements (fp16 in `h`, 32-bit in `x`) -> a word of codes; the scale
-// (fp16 bits) is the same in the four lanes of the group.  Called by whole warps.
-__device__ __forceinline__ uint32_t quantise8(const uint4& h, const float (&x)[8], uint32_t& scale_bits) {
-  uint32_t m = h2_abs_max_nan(h2_abs_max_nan(h2_abs_max_nan(h.x & 0x7fff7fffu, h.y), h.z), h.w);
-  m = h2_abs_max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = h2_abs_max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const float2 mf = __half22float2(*reinterpret_cast<const __half2*>(&m));
-  const float amax = fmaxf(mf.x, mf.y);
-  const bool fine = mf.x <= 65504.f && mf.y <= 65504.f;   // false for infinities and NaN
-  const __half sh = __float2half_rn(fminf(amax * (1.f / 7.f), kMaxScale));
-  const float s = __half2float(sh);
-  const float inv = s > 0.f ? __frcp_rn(s) : 0.f;
-  // floor(x / s + 8.5) is 1 .. 15 when s is a normal number (|x| / s <= 7 (1 + 2^-11)); only a subnormal s,
-  // rounded coarsely, can be exceeded by more, and then the sum is limited first.
-  float t[8];
-#pragma unroll
-  for (int n = 0; n < 8; ++n) t[n] = fmaf(x[n], inv, 8.5f + 1.f / 16384.f);
-  if (s < 6.104e-5f) {
-#pragma unroll
-    for (int n = 0; n < 8; ++n) t[n] = fminf(fmaxf(t[n], 0.f), 15.5f);
-  }
-  // Adding 2^23 rounding down leaves the floor in the low bits of 0x4B000000; the eight of them are shifted
-  // into place and added up, and the constant parts taken off (all but two are shifted out).
-  uint32_t word = 0u - 0x4B000000u - (0x4B000000u << 4);
-#pragma unroll
-  for (int n = 0; n < 8; ++n) {
-    const int shift = 4 * ((n >> 1) + 4 * (n & 1));
-    word += __float_as_uint(__fadd_rd(t[n], 8388608.f)) << shift;
-  }
-  scale_bits = fine ? static_cast<uint32_t>(__half_as_ushort(sh)) : 0x7E00u;   // NaN: never read as a number
-  return fine ? word : 0x88888888u;
+__device__ __forceinline__ uint32_t h2_abs(uint32_t a) { return a & 0x7fff7fffu; }
+__device__ __forceinline__ uint32_t abs_max8(const uint4& h) {
+  return h2_max_nan(h2_max_nan(h2_abs(h.x), h2_abs(h.y)), h2_max_nan(h2_abs(h.z), h2_abs(h.w)));
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));
+  return y;
 }
 
-// The codes and scales of four rows (eight lanes each) of one head row to their places: lane `sub` of a row
-// holds the words of groups sub / 4 and 2 + sub / 4, lane sub ^ 4 the others of the same chunk.
+// Floors of t[0..7] (1 .. 15) as the nibbles of a word.  Adding 2^23 rounding down leaves a floor in the low bits of
+// 0x4B000000; the eight are shifted into place and added up, and the constant parts taken off (all but two
+// are shifted out).
+__device__ __forceinline__ uint32_t pack_floors(const float (&t)[8]) {
+  uint32_t word = 0u - 0x4B000000u - (0x4B000000u << 4);
+#pragma unroll
+  for (int n = 0; n < 8; ++n)
+    word += __float_as_uint(__fadd_rd(t[n], 8388608.f)) << (4 * ((n >> 1) + 4 * (n & 1)));
+  return word;
+}
+
+// One head row of four tokens, eight lanes each: this lane's 8 + 8 elements (fp16 in ha and hb, 32-bit in a and
+// b) are quantised and stored.  Lane `sub` of a row owns the words of groups sub / 4 and 2 + sub / 4; lane
+// sub ^ 4 has the others of the same chunk.  Called by whole warps; nothing is stored where slot_ok is
+// false.
 __device__ __forceinline__ void store_row(const uint4& ha, const uint4& hb, const float (&a)[8], const float (&b)[8],
                                           int sub, bool slot_ok, uint8_t* block, int t) {
-  uint32_t s1, s2;
-  const uint32_t w1 = quantise8(ha, a, s1), w2 = quantise8(hb, b, s2);
+  // the largest magnitudes of both groups travel as one pair through the four lanes of a group
+  const uint32_t ma = abs_max8(ha), mb = abs_max8(hb);
+  uint32_t m = h2_max_nan(__byte_perm(ma, mb, 0x5410), __byte_perm(ma, mb, 0x7632));
+  m = h2_max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = h2_max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+  const float2 top = __half22float2(*reinterpret_cast<const __half2*>(&m));
+  const bool fine1 = top.x <= 65504.f, fine2 = top.y <= 65504.f;   // false for infinities and NaN
+  const __half2 sh = __floats2half2_rn(fminf(top.x * (1.f / 7.f), kMaxScale), fminf(top.y * (1.f / 7.f), kMaxScale));
+  const float2 s = __half22float2(sh);
+  const float inv1 = s.x > 0.f ? rcp_approx(s.x) : 0.f, inv2 = s.y > 0.f ? rcp_approx(s.y) : 0.f;
+  float t1[8], t2[8];
+#pragma unroll
+  for (int n = 0; n < 8; ++n) {
+    t1[n] = fmaf(a[n], inv1, 8.5f + 1.f / 16384.f);
+    t2[n] = fmaf(b[n], inv2, 8.5f + 1.f / 16384.f);
+  }
+  // floor(x / s + 8.5) is 1 .. 15 when s is a normal number (|x| / s <= 7 (1 + 2^-11)); only a subnormal s,
+  // rounded coarsely, can be exceeded by more, and then the sum is limited first.
+  if (__any_sync(0xffffffffu, fminf(s.x, s.y) < 6.104e-5f)) {
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+      t1[n] = fminf(fmaxf(t1[n], 0.f), 15.5f);
+      t2[n] = fminf(fmaxf(t2[n], 0.f), 15.5f);
+    }
+  }
+  const uint32_t w1 = fine1 ? pack_floors(t1) : 0x88888888u, w2 = fine2 ? pack_floors(t2) : 0x88888888u;
+  uint32_t sc = *reinterpret_cast<const uint32_t*>(&sh);   // a scale of NaN is never read as a number
+  if (!fine1) sc = (sc & 0xffff0000u) | 0x7E00u;
+  if (!fine2) sc = (sc & 0xffffu) | 0x7E000000u;
   const uint32_t pw1 = __shfl_xor_sync(0xffffffffu, w1, 4), pw2 = __shfl_xor_sync(0xffffffffu, w2, 4);
-  const uint32_t ps = __shfl_xor_sync(0xffffffffu, s1 | (s2 << 16), 4);
+  const uint32_t ps = __shfl_xor_sync(0xffffffffu, sc, 4);
   if (slot_ok && sub < 4) {
     *reinterpret_cast<uint4*>(block + kv4::chunk_offset(t, sub)) = make_uint4(w1, pw1, w2, pw2);
     if (sub == 0)
       *reinterpret_cast<uint2*>(block + kv4::kScaleOffset + t * kv4::kScaleBytes) =
-          make_uint2(s1 | (ps << 16), s2 | (ps & 0xffff0000u));
+          make_uint2(__byte_perm(sc, ps, 0x5410), __byte_perm(sc, ps, 0x7632));
   }
 }
 
@@ -167,20 +188,19 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendParams p) {
     const int64_t tok = static_cast<int64_t>(quad) * kTokPerWarp + (lane >> 3);
     const bool live = tok < p.n_tokens;
     const int row0 = grp * kRows;
+    const int64_t src_tok = live ? tok : p.n_tokens - 1;   // lanes past the last token load it again and store nothing
     uint4 ua[kRows], ub[kRows];
-    int64_t slot = -1;
 #pragma unroll
     for (int i = 0; i < kRows; ++i) {
-      ua[i] = ub[i] = make_uint4(0, 0, 0, 0);
       const int row = row0 + i;   // K heads, then V heads
-      if (live && row < p.rows_per_token) {
-        const __half* src = row >= p.kv_heads ? p.v + tok * p.v_tok_stride + (row - p.kv_heads) * kD
-                                              : p.k + tok * p.k_tok_stride + row * kD;
-        ua[i] = __ldg(reinterpret_cast<const uint4*>(src + sub * 8));
-        ub[i] = __ldg(reinterpret_cast<const uint4*>(src + kHalf + sub * 8));
+      if (row < p.rows_per_token) {
+        const __half* src = (row >= p.kv_heads ? p.v + src_tok * p.v_tok_stride + (row - p.kv_heads) * kD
+                                               : p.k + src_tok * p.k_tok_stride + row * kD) + sub * 8;
+        ua[i] = __ldg(reinterpret_cast<const uint4*>(src));
+        ub[i] = __ldg(reinterpret_cast<const uint4*>(src + kHalf));
       }
     }
-    if (live) slot = __ldg(p.slots + tok);
+    const int64_t slot = live ? __ldg(p.slots + src_tok) : -1;
     const bool slot_ok = slot >= 0 && slot < p.pool_tokens;
     if (live && !slot_ok && sub == 0) set_status(p.status, B200KV_DEV_BAD_SLOT);
     const int t = static_cast<int>(slot & (kv4::kPageTok - 1));
@@ -206,7 +226,7 @@ __global__ void __launch_bounds__(kThreads) kv4_append_kernel(AppendParams p) {
 // of its own and the loops are not unrolled: the kernel has to stay inside the instruction cache), and
 // the next row is on its way while one is worked on.
 template <int kRows>
-__global__ void __launch_bounds__(kThreads, 4) kv4_prologue_kernel(AppendParams p) {
+__global__ void __launch_bounds__(kThreads, kPrologueCtas) kv4_prologue_kernel(AppendParams p) {
   cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
   const int lane = threadIdx.x & 31;
@@ -453,8 +473,6 @@ int launch(Kernel kernel, const Params& p, unsigned blocks, cudaStream_t stream)
   return check_launch();
 }
 
-constexpr int kCtasPerSm = 8;
-
 // Rows per warp: four when that still gives every SM this many warps, one otherwise (a decode step's few
 // tokens: 3.8 against 4.3 us for four tokens of 16 + 16 rows and their read-back).
 constexpr int kWarpsForFour = 16;
@@ -467,7 +485,7 @@ int launch_append_rows(AppendParams p, cudaStream_t stream) {
   p.groups = kFused ? (p.q_heads + kRows - 1) / kRows + 2 * ((p.kv_heads + kRows - 1) / kRows)
                     : (p.rows_per_token + kRows - 1) / kRows;
   unsigned blocks = 0;
-  const int rc = grid_for(static_cast<int64_t>(p.quads) * p.groups, kCtasPerSm, &blocks);
+  const int rc = grid_for(static_cast<int64_t>(p.quads) * p.groups, kFused ? kPrologueCtas : kCopyCtas, &blocks);
   if (rc != B200KV_OK) return rc;
   const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
   p.step_quad = static_cast<int>(warps / p.groups);
@@ -490,7 +508,7 @@ template <int kRows>
 int launch_gather(GatherParams p, cudaStream_t stream) {
   p.groups = (p.rows + kRows - 1) / kRows;
   unsigned blocks = 0;
-  const int rc = grid_for(static_cast<int64_t>(p.octets) * p.groups, kCtasPerSm, &blocks);
+  const int rc = grid_for(static_cast<int64_t>(p.octets) * p.groups, kCopyCtas, &blocks);
   if (rc != B200KV_OK) return rc;
   const int64_t warps = static_cast<int64_t>(blocks) * (kThreads / 32);
   p.step_octet = static_cast<int>(warps / p.groups);
