@@ -473,8 +473,9 @@ int launch(Kernel kernel, const Params& p, unsigned blocks, cudaStream_t stream)
   return check_launch();
 }
 
-// Rows per warp: four when that still gives every SM this many warps, one otherwise (a decode step's few
-// tokens: 3.8 against 4.3 us for four tokens of 16 + 16 rows and their read-back).
+// Rows per warp: four when that still gives every SM this many warps, one otherwise.  One / four rows, us, 64/8
+// heads: append of 32 tokens 1.6 / 2.7, 4096 5.8 / 6.1, 32 768 38.2 / 36.4; read-back of 32 1.6 / 2.5, 32 768
+// 28.8 / 28.4; fused append of 256 3.7 / 5.2, 1024 9.2 / 9.4, 8192 64.1 / 54.0.
 constexpr int kWarpsForFour = 16;
 inline bool four_rows(int64_t token_groups, int rows, int sms) {
   return token_groups * ((rows + 3) / 4) >= static_cast<int64_t>(sms) * kWarpsForFour;
