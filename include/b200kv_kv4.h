@@ -123,7 +123,7 @@ int b200kv_kv4_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_
  * b200kv_paged_prefill (the chunk's own rows are already in the pool), table kinds BLOCK and TOKEN.
  * Lengths, rows and tables may come from the kernel launched immediately before.  A request whose chunk
  * is longer than max_q_len is skipped (B200KV_DEV_BAD_LENGTH).  A K or V group that reads as NaN reaches
- * the rows that see its token and no others.
+ * the rows that see its token and no others.  scale_log2 is positive and finite.
  *   workspace  NULL, or scratch of b200kv_kv4_chunk_workspace_bytes() bytes under the rules of the decode
  *              workspace (the same buffer may serve both): chunks of a few rows -- drafted tokens, the end
  *              of a prompt -- are then streamed like a decode step instead of filling a small part of

@@ -49,6 +49,7 @@
 //
 // Every wait is an mbarrier try-wait bounded by ~2 s of %globaltimer; a wait that runs out sets
 // B200KV_DEV_WAIT_TIMEOUT, and every warp still reaches the common exit where TMEM is freed.
+#include <cfloat>
 #include <climits>
 
 #include "common.cuh"
@@ -1019,6 +1020,7 @@ int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
   int rc = check_prefill(a, &nothing);
   if (rc != B200KV_OK || nothing) return rc;
   if (a.table_kind == B200KV_TABLE_DENSE) return B200KV_EINVAL;
+  if (!(a.scale_log2 > 0.f && a.scale_log2 <= FLT_MAX)) return B200KV_EINVAL;   // the tiles take the maximum of raw scores
   rc = kv4_check_pool(k.pool, k.pool_pages, k.page_stride_bytes, a.kv_heads);
   if (rc != B200KV_OK) return rc;
   // A few query rows over a long context: streamed like a decode step (kv4_decode.cu).

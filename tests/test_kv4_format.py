@@ -147,3 +147,11 @@ def test_prefill_refusals(built_lib, kw, code):
 
 def test_capture_id_wants_a_place_for_the_answer(built_lib):
     assert built_lib.b200kv_stream_capture_id(None, None) == EINVAL
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.1, float("nan"), float("inf")])
+@pytest.mark.parametrize("ws", [None, A])
+def test_prefill_refuses_a_scale_that_is_not_positive(built_lib, scale, ws):
+    assert built_lib.b200kv_kv4_paged_prefill(
+        A, 1024, 128, A, 8, 2 * 4 * 1152, A, 10, 0, 2, 10, A, A, A, A, 0, 2, 8, 4, 8, 4, 128, 16, scale, A, 1024, 128, ws,
+        0, None, None) == EINVAL
