@@ -856,29 +856,37 @@ def _status_ptr(device_index: int) -> int:
 
 
 def _kv4_workspace_need(device_index: int, batch: int, max_q_len: int, q_heads: int, kv_heads: int) -> int:
-    """Bytes of scratch of a decode step (``max_q_len`` 0) or a chunk; 0 for a chunk that needs none.
-    The device is current."""
+    """Bytes of scratch of a decode step (``max_q_len`` 0) or a chunk; 0 for a chunk that needs none."""
     key = ("kv4", device_index, batch, max_q_len, q_heads, kv_heads)
     need = _workspace_need.get(key)
     if need is None:
         lib = _lib.lib()
-        if max_q_len:
-            need = lib.b200kv_kv4_chunk_workspace_bytes(batch, max_q_len, q_heads, kv_heads, KV4_HEAD_DIM)
-        else:
-            need = lib.b200kv_kv4_decode_workspace_bytes(batch, q_heads, kv_heads, KV4_HEAD_DIM)
-            if need == 0:
-                raise ValueError("unsupported decode shape: q_heads/kv_heads must be an integer <= 16, batch at most "
-                                 f"4096 and batch * kv_heads at most {DECODE_COUNTER_BYTES // 4}")
+        with _on_device(device_index):
+            if max_q_len:
+                need = lib.b200kv_kv4_chunk_workspace_bytes(batch, max_q_len, q_heads, kv_heads, KV4_HEAD_DIM)
+            else:
+                need = lib.b200kv_kv4_decode_workspace_bytes(batch, q_heads, kv_heads, KV4_HEAD_DIM)
+        if need == 0 and not max_q_len:
+            raise ValueError("unsupported decode shape: q_heads/kv_heads must be an integer <= 16, batch at most "
+                             f"4096 and batch * kv_heads at most {DECODE_COUNTER_BYTES // 4}")
         _workspace_need[key] = need
     return need
 
 
-def kv4_workspace(device_index: int, stream: int, need: int) -> torch.Tensor:
-    """Scratch of the 4-bit attention operators: arrival counters (zero between calls) and partials.
+def kv4_workspace(device_index: int, batch: int, max_q_len: int, q_heads: int, kv_heads: int) -> Optional[torch.Tensor]:
+    """Scratch of a decode step (``max_q_len`` 0) or a chunk on the device's current stream: arrival counters
+    (zero between calls) and partials.  None for a chunk that needs none.
 
     Eager calls of one stream share one buffer (grown on demand): they follow one another.  A graph under
     capture gets a buffer of its own out of its memory pool, whose counters are cleared by a node of
     the graph, so graphs may be replayed next to each other and next to eager calls."""
+    need = _kv4_workspace_need(device_index, batch, max_q_len, q_heads, kv_heads)
+    if need == 0:
+        return None
+    if _current_device() != device_index:
+        with torch.cuda.device(device_index):
+            return kv4_workspace(device_index, batch, max_q_len, q_heads, kv_heads)
+    stream = _stream(device_index)
     where = (device_index, stream)
     capture = _capture_of(stream) if _capturing() else 0
     if capture:
@@ -898,7 +906,23 @@ def kv4_workspace(device_index: int, stream: int, need: int) -> torch.Tensor:
     return ws
 
 
-def _kv4_done(rc: int, dev: int) -> None:
+# The launches as calls with packed arguments: (op, pack, number of words).
+_KV4_APPEND = (0, *_lib.kv4_packer("b200kv_kv4_append"))
+_KV4_PROLOGUE = (1, *_lib.kv4_packer("b200kv_kv4_qk_norm_rope_append"))
+_KV4_GATHER = (2, *_lib.kv4_packer("b200kv_kv4_gather"))
+_KV4_DECODE = (3, *_lib.kv4_packer("b200kv_kv4_paged_decode"))
+_KV4_PREFILL = (4, *_lib.kv4_packer("b200kv_kv4_paged_prefill"))
+
+
+def _kv4_call(call: tuple, dev: int, *args) -> None:
+    """Launch on ``dev``'s current stream; ``args`` are all but the last two (status word and stream)."""
+    op, pack, n = call
+    words = pack(*args, _status_ptr(dev), _stream(dev))
+    if _current_device() == dev:
+        rc = _lib.lib().b200kv_kv4_call(op, words, n)
+    else:
+        with torch.cuda.device(dev):
+            rc = _lib.lib().b200kv_kv4_call(op, words, n)
     if rc != 0:
         _lib.check(rc)
     if _DEBUG:
@@ -919,10 +943,8 @@ def update_kv_buffer_kv4(KV_Values: torch.Tensor, Select_Index: torch.Tensor, KV
         return
     if _DEBUG:
         _debug_check_append(KV_Values, slots, pages * KV4_PAGE_SIZE)
-    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
-        rc = _lib.lib().b200kv_kv4_append(k_ptr, k_ptr + kvh * KV4_HEAD_DIM * 2, n, stride, stride, slots.data_ptr(),
-                                          ptr, pages, page_stride, kvh, KV4_HEAD_DIM, _status_ptr(dev), _stream(dev))
-    _kv4_done(rc, dev)
+    _kv4_call(_KV4_APPEND, dev, k_ptr, k_ptr + kvh * KV4_HEAD_DIM * 2, n, stride, stride, slots.data_ptr(), ptr, pages,
+              page_stride, kvh, KV4_HEAD_DIM)
 
 
 def update_kv_buffer_kv4_split(xk: torch.Tensor, xv: torch.Tensor, Select_Index: torch.Tensor,
@@ -937,10 +959,8 @@ def update_kv_buffer_kv4_split(xk: torch.Tensor, xv: torch.Tensor, Select_Index:
         return
     if _DEBUG:
         _debug_check_append(torch.cat([xk[:n], xv[:n]], dim=1), slots, pages * KV4_PAGE_SIZE)
-    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
-        rc = _lib.lib().b200kv_kv4_append(k_ptr, v_ptr, n, k_stride, v_stride, slots.data_ptr(), ptr, pages, page_stride,
-                                          kvh, KV4_HEAD_DIM, _status_ptr(dev), _stream(dev))
-    _kv4_done(rc, dev)
+    _kv4_call(_KV4_APPEND, dev, k_ptr, v_ptr, n, k_stride, v_stride, slots.data_ptr(), ptr, pages, page_stride, kvh,
+              KV4_HEAD_DIM)
 
 
 def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
@@ -992,14 +1012,10 @@ def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_we
         return out
     if _DEBUG:
         _debug_check_append(xkv, slots, pages * KV4_PAGE_SIZE)
-    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
-        rc = _lib.lib().b200kv_kv4_qk_norm_rope_append(
-            q_ptr, out_ptr, q_stride, out_stride, xkv.data_ptr(), xkv.stride(0) if n > 1 else row,
-            0 if q_norm_weight is None else q_norm_weight.data_ptr(),
-            0 if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps),
-            cos.data_ptr(), sin.data_ptr(), cos.stride(0) if n > 1 else d, slots.data_ptr(),
-            ptr, pages, page_stride, n, qh, kvh, d, _status_ptr(dev), _stream(dev))
-    _kv4_done(rc, dev)
+    _kv4_call(_KV4_PROLOGUE, dev, q_ptr, out_ptr, q_stride, out_stride, xkv.data_ptr(), xkv.stride(0) if n > 1 else row,
+              0 if q_norm_weight is None else q_norm_weight.data_ptr(),
+              0 if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(),
+              cos.stride(0) if n > 1 else d, slots.data_ptr(), ptr, pages, page_stride, n, qh, kvh, d)
     return out
 
 
@@ -1019,10 +1035,7 @@ def gather_kv_buffer_kv4(KV4_Buffer: torch.Tensor, Select_Index: torch.Tensor,
             raise ValueError(f"out must hold {n} rows")
     if n == 0:
         return out
-    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
-        rc = _lib.lib().b200kv_kv4_gather(ptr, pages, page_stride, slots.data_ptr(), n, out_ptr, out_stride, kvh, d,
-                                          _status_ptr(dev), _stream(dev))
-    _kv4_done(rc, dev)
+    _kv4_call(_KV4_GATHER, dev, ptr, pages, page_stride, slots.data_ptr(), n, out_ptr, out_stride, kvh, d)
     return out
 
 
@@ -1063,7 +1076,7 @@ def flash_decoding_kv4(
     if not 0 <= max_len <= tbl_cols * (page_size if kind == TABLE_BLOCK else 1):
         raise ValueError("max_actual_seq_len exceeds the table width")
     if out is None:
-        out = torch.empty(batch, q_heads, d, dtype=torch.float16, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(batch, q_heads, d, dtype=torch.float16, device=q.device)
         out_sb, out_sh = q_heads * d, d
     else:
         out_sb, out_sh, out_sd = out.stride() if out.dim() == 3 else (0, 0, 0)
@@ -1075,15 +1088,11 @@ def flash_decoding_kv4(
         return out
     if _DEBUG:
         _debug_check_lengths(b_seq_len, max_len, b_req_idx, tbl_rows, "decode")
-    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
-        stream = _stream(dev)
-        ws = kv4_workspace(dev, stream, _kv4_workspace_need(dev, batch, 0, q_heads, kv_heads))
-        rc = _lib.lib().b200kv_kv4_paged_decode(
-            q.data_ptr(), q_sb, q_sh, ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols,
-            rows_ptr, lens_ptr, b_seq_len.dtype is torch.int64, batch, q_heads, kv_heads, d, int(page_size), float(qk_scale),
-            max_len, ws.data_ptr(), ws.numel(), out.data_ptr(), out_sb, out_sh,
-            DECODE_SERIALIZED if metadata_fresh else 0, _status_ptr(dev), stream)
-    _kv4_done(rc, dev)
+    ws = kv4_workspace(dev, batch, 0, q_heads, kv_heads)
+    _kv4_call(_KV4_DECODE, dev, q.data_ptr(), q_sb, q_sh, ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows,
+              tbl_cols, rows_ptr, lens_ptr, b_seq_len.dtype is torch.int64, batch, q_heads, kv_heads, d, int(page_size),
+              float(qk_scale), max_len, ws.data_ptr(), ws.numel(), out.data_ptr(), out_sb, out_sh,
+              DECODE_SERIALIZED if metadata_fresh else 0)
     return out
 
 
@@ -1117,7 +1126,7 @@ def paged_chunk_flash_attention_kv4(
     ids_ptr = _ints_arg(req_ids, "req_ids", batch, dev, False)
     start_ptr = _ints_arg(q_start_loc, "q_start_loc", batch, dev, False)
     total_q, q_heads, d = q.shape
-    output = torch.empty(total_q, q_heads, d, dtype=torch.float16, device=q.device)
+    output = torch.empty_like(q) if q.is_contiguous() else torch.empty(total_q, q_heads, d, dtype=torch.float16, device=q.device)
     if total_q == 0 or q_heads == 0 or batch == 0:
         return output
     if _DEBUG:
@@ -1125,21 +1134,12 @@ def paged_chunk_flash_attention_kv4(
         _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, tbl_rows, "paged prefill")
         _debug_check_lengths(q_seq_lens, int(max_q_len), None, 0, "paged prefill chunk")   # longer ones are skipped
     max_q_len = int(max_q_len)
-    with _NO_SWITCH if _current_device() == dev else torch.cuda.device(dev):
-        stream = _stream(dev)
-        # at most 128 columns (rows x heads of a group) are streamed like a decode step, with its scratch
-        need = _kv4_workspace_need(dev, batch, max_q_len, q_heads, kv_heads) if 0 < max_q_len <= 128 else 0
-        ws_ptr, ws_bytes = 0, 0
-        if need:
-            ws = kv4_workspace(dev, stream, need)
-            ws_ptr, ws_bytes = ws.data_ptr(), ws.numel()
-        rc = _lib.lib().b200kv_kv4_paged_prefill(
-            q.data_ptr(), q.stride(0) if total_q > 1 else q_heads * d, q.stride(1) if q_heads > 1 else d,
-            ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols, ids_ptr, start_ptr, ctx_ptr,
-            qlen_ptr, q_seq_lens.dtype is torch.int64, batch, total_q, max_q_len, q_heads, kv_heads, d,
-            int(page_size), float(sm_scale), output.data_ptr(), q_heads * d, d, ws_ptr, ws_bytes, _status_ptr(dev),
-            stream)
-    _kv4_done(rc, dev)
+    # at most 128 columns (rows x heads of a group) are streamed like a decode step, with its scratch
+    ws = kv4_workspace(dev, batch, max_q_len, q_heads, kv_heads) if 0 < max_q_len <= 128 else None
+    _kv4_call(_KV4_PREFILL, dev, q.data_ptr(), q.stride(0) if total_q > 1 else q_heads * d, q.stride(1) if q_heads > 1 else d,
+              ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols, ids_ptr, start_ptr, ctx_ptr, qlen_ptr,
+              q_seq_lens.dtype is torch.int64, batch, total_q, max_q_len, q_heads, kv_heads, d, int(page_size), float(sm_scale),
+              output.data_ptr(), q_heads * d, d, 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
     return output
 
 
