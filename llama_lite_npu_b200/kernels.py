@@ -797,12 +797,13 @@ def _table_arg(tbl: torch.Tensor, table_kind: str, dev: int):
     kind = _TABLE_KINDS.get(table_kind, -1)
     if kind != TABLE_BLOCK and kind != TABLE_TOKEN:
         raise ValueError("the 4-bit operators take a 'token' or 'block' table")
-    if tbl.dtype is not torch.int32 or tbl.dim() != 2 or tbl.stride(1) != 1:
+    strides = tbl.stride()
+    if tbl.dtype is not torch.int32 or len(strides) != 2 or strides[1] != 1:
         raise ValueError("the table must be a 2-D int32 tensor contiguous along its last dimension")
     if tbl.get_device() != dev:
         raise _off_device("the table", tbl, dev)
     rows, cols = tbl.shape
-    return tbl.data_ptr(), tbl.stride(0) if rows > 1 else cols, kind, rows, cols
+    return tbl.data_ptr(), strides[0] if rows > 1 else cols, kind, rows, cols
 
 
 def _ints_arg(t: torch.Tensor, name: str, n: int, dev: int, wide: bool) -> int:
@@ -985,17 +986,18 @@ def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_we
     row = 2 * kvh * d
     if xkv.dim() == 3 and xkv.shape[1:] == (2 * kvh, d):
         xkv = xkv.reshape(n, row) if xkv.shape[0] == n else xkv
-    if xkv.dtype is not torch.float16 or xkv.dim() != 2 or xkv.shape != (n, row) or xkv.stride(1) != 1:
+    kv_strides = xkv.stride()
+    if xkv.dtype is not torch.float16 or xkv.shape != (n, row) or kv_strides[1] != 1:
         raise ValueError("xkv must be [n, 2*kv_heads*head_dim] float16, contiguous rows")
     if xkv.get_device() != dev:
         raise _off_device("xkv", xkv, dev)
     if cos.dim() != 2 or sin.dim() != 2:
         cos, sin = cos.reshape(-1, cos.shape[-1]), sin.reshape(-1, sin.shape[-1])
-    width = cos.shape[1]
+    (rows, width), (cs_stride, cos_step), (sin_stride, sin_step) = cos.shape, cos.stride(), sin.stride()
     if cos.dtype is not torch.float16 or sin.dtype is not torch.float16:
         raise ValueError("cos and sin must be float16")
-    if cos.shape != (n, width) or sin.shape != (n, width) or (width != d and width != d // 2) \
-            or cos.stride(1) != 1 or sin.stride(1) != 1 or (n > 1 and cos.stride(0) != sin.stride(0)):
+    if rows != n or sin.shape != cos.shape or (width != d and width != d // 2) or cos_step != 1 or sin_step != 1 \
+            or (n > 1 and cs_stride != sin_stride):
         raise ValueError("cos and sin must be one row of head_dim (or head_dim/2) per token with equal strides")
     if cos.get_device() != dev or sin.get_device() != dev:
         raise _off_device("cos and sin", cos if cos.get_device() != dev else sin, dev)
@@ -1012,10 +1014,10 @@ def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_we
         return out
     if _DEBUG:
         _debug_check_append(xkv, slots, pages * KV4_PAGE_SIZE)
-    _kv4_call(_KV4_PROLOGUE, dev, q_ptr, out_ptr, q_stride, out_stride, xkv.data_ptr(), xkv.stride(0) if n > 1 else row,
+    _kv4_call(_KV4_PROLOGUE, dev, q_ptr, out_ptr, q_stride, out_stride, xkv.data_ptr(), kv_strides[0] if n > 1 else row,
               0 if q_norm_weight is None else q_norm_weight.data_ptr(),
               0 if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(),
-              cos.stride(0) if n > 1 else d, slots.data_ptr(), ptr, pages, page_stride, n, qh, kvh, d)
+              cs_stride if n > 1 else d, slots.data_ptr(), ptr, pages, page_stride, n, qh, kvh, d)
     return out
 
 
