@@ -94,8 +94,9 @@ int b200kv_stream_capture_id(void* stream, uint64_t* id);
 size_t b200kv_kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head_dim);
 
 /*
- * Bytes of scratch with which b200kv_kv4_paged_prefill streams chunks of at most max_q_len rows; 0 where
- * it would not (max_q_len * q_heads / kv_heads above 128, batch above 4096, or bad input).
+ * Bytes of scratch that b200kv_kv4_paged_prefill can use for chunks of at most max_q_len rows on the CURRENT
+ * device; 0 where it has no use for any (many long chunks), or on bad input.  Above 128 rows only the
+ * number of 128-row tiles matters.
  */
 size_t b200kv_kv4_chunk_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads, int head_dim);
 
@@ -125,9 +126,10 @@ int b200kv_kv4_paged_decode(const void* q, int64_t q_stride_b, int64_t q_stride_
  * is longer than max_q_len is skipped (B200KV_DEV_BAD_LENGTH).  A K or V group that reads as NaN reaches
  * the rows that see its token and no others.  scale_log2 is positive and finite.
  *   workspace  NULL, or scratch of b200kv_kv4_chunk_workspace_bytes() bytes under the rules of the decode
- *              workspace (the same buffer may serve both): chunks of a few rows -- drafted tokens, the end
- *              of a prompt -- are then streamed like a decode step instead of filling a small part of
- *              128-row tiles.  Then q is 16-byte aligned with strides that are multiples of 8
+ *              workspace (the same buffer may serve both).  With it chunks of a few rows -- drafted tokens,
+ *              the end of a prompt -- are streamed like a decode step instead of filling a small part of
+ *              128-row tiles (then q is 16-byte aligned with strides that are multiples of 8), and where
+ *              the query tiles leave most SMs empty their keys are cut into parts that are joined at the end
  */
 int b200kv_kv4_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride_h,
                              const void* pool, int64_t pool_pages, int64_t page_stride_bytes,

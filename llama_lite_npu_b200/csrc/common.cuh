@@ -58,6 +58,14 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   return *reinterpret_cast<uint32_t*>(&h);
 }
 
+// Count an arrival (0 .. limit, wrapping): what the CTA wrote before (and joined with a barrier) is published by
+// it, and what earlier arrivals published is seen after it.
+__device__ __forceinline__ unsigned atomic_inc_acq_rel(unsigned* ctr, unsigned limit) {
+  unsigned old;
+  asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;\n" : "=r"(old) : "l"(ctr), "r"(limit) : "memory");
+  return old;
+}
+
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x));

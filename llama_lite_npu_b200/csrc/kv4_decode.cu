@@ -525,12 +525,6 @@ struct Weighted {
   }
 };
 
-__device__ __forceinline__ unsigned atomic_inc_acq_rel(unsigned* ctr, unsigned limit) {
-  unsigned old;
-  asm volatile("atom.acq_rel.gpu.global.inc.u32 %0, [%1], %2;\n" : "=r"(old) : "l"(ctr), "r"(limit) : "memory");
-  return old;
-}
-
 // The end of a piece.  The four warps put their O^T fragments, as they are, and their (m, l) into shared
 // memory; every thread then combines 2 * NB of the 16-byte pieces over the warps and writes the final
 // rows (whole sequence) or the partial, in the same fragment order (16-byte accesses without bank
@@ -1077,12 +1071,20 @@ size_t kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head
   return static_cast<size_t>(layout_of(s, batch, kv_heads).total);
 }
 
+// Does a chunk of at most max_q_len rows go through this file's kernel (given a workspace)?
+bool kv4_streams_chunk(int batch, int64_t max_q_len, int q_heads, int kv_heads) {
+  if (batch > 4096 || max_q_len * (q_heads / kv_heads) > kChunkColumns) return false;
+  Shape s;
+  return shape_of(static_cast<int>(max_q_len), q_heads, kv_heads, &s) == B200KV_OK &&
+         static_cast<int64_t>(batch) * kv_heads * s.blocks <= kMaxCounters;
+}
+
 size_t kv4_chunk_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads, int head_dim) {
-  if (batch <= 0 || batch > 4096 || q_heads <= 0 || kv_heads <= 0 || max_q_len <= 0 || head_dim != kD) return 0;
-  if (q_heads % kv_heads != 0 || max_q_len * (q_heads / kv_heads) > kChunkColumns) return 0;
+  if (batch <= 0 || q_heads <= 0 || kv_heads <= 0 || max_q_len <= 0 || head_dim != kD) return 0;
+  if (batch > 65535 || max_q_len > (int64_t{1} << 31) - 1 || q_heads % kv_heads != 0) return 0;
+  if (!kv4_streams_chunk(batch, max_q_len, q_heads, kv_heads)) return kv4_split_workspace_bytes(batch, max_q_len, q_heads, kv_heads);
   Shape s;
   if (shape_of(static_cast<int>(max_q_len), q_heads, kv_heads, &s) != B200KV_OK) return 0;
-  if (static_cast<int64_t>(batch) * kv_heads * s.blocks > kMaxCounters) return 0;
   return static_cast<size_t>(layout_of(s, batch, kv_heads).total);
 }
 

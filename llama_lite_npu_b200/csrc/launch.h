@@ -184,10 +184,12 @@ struct Kv4PrefillArgs {
   PrefillArgs args;   // k_base, v_base, kv strides and pool_tokens unused
   const void* pool;
   int64_t pool_pages, page_stride_bytes;
-  void* workspace;    // short chunks only (kv4_chunk_workspace_bytes > 0)
+  void* workspace;    // of kv4_chunk_workspace_bytes; may be null
   size_t workspace_bytes;
 };
 size_t kv4_chunk_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads, int head_dim);
+size_t kv4_split_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads);
+bool kv4_streams_chunk(int batch, int64_t max_q_len, int q_heads, int kv_heads);
 int kv4_paged_chunk(const Kv4PrefillArgs& a, cudaStream_t stream);
 int kv4_paged_prefill(const Kv4PrefillArgs& a, cudaStream_t stream);
 int wait_selftest(uint64_t limit_ns, int32_t* result, int32_t* status, cudaStream_t stream);

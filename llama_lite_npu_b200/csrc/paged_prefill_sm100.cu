@@ -38,7 +38,8 @@
 // in the reference (:166, :220), output fp16.  Tensor-bound:
 // flops = 4 * 128 * sum over (query, visible key) pairs, per query head.
 //
-// Over a 4-bit cache (kKv4, include/b200kv_kv4.h) the same pipeline runs with a fourth warpgroup: its four
+// Over a 4-bit cache (kKv4, include/b200kv_kv4.h) a launch of few query tiles cuts their keys into parts, one CTA
+// each, that the CTA which arrives last joins; and the same pipeline runs with a fourth warpgroup: its four
 // warps read the blocks of codes and scales straight from the pool, one ring item ahead of use in
 // registers, turn them into fp16 (code - 8) * scale, and store each word of codes as one 16-byte piece of
 // the K or V tile where the copies would have put it (72 bytes read per row instead of 256).  The
@@ -88,6 +89,11 @@ constexpr int kTmemCols = 512;
 constexpr int kTmemS = 0;                      // S_0 at 0, S_1 at 128
 constexpr int kTmemO = 256;                    // O_0 at 256, O_1 at 384
 constexpr int kBarBytes = 256;
+// Parts of a query tile's keys (4-bit pool): at most kMaxSplits, of at least kMinSplitTiles key tiles.  Joining
+// costs about 7 us, three key tiles, so fewer than two such parts are left whole (cut in two / whole, us:
+// 5 key tiles 25.6 / 20.1, 17-20 tiles 29.9 / 45.7; in four, 13 tiles 26.4 / 34.4; in nine, 95 tiles 55.9 / 210).
+constexpr int kMaxSplits = 16;
+constexpr int kMinSplitTiles = 4;
 constexpr int kSmemBytes = kGroups * (kQBytes + kPBytes) + kSlots * kTileBytes + kBarBytes;
 
 // tcgen05 instruction descriptor, kind::f16: fp16 A/B, fp32 accumulate.
@@ -218,9 +224,67 @@ struct PrefillParams {
   int kv_heads;
   int64_t max_q_len;
   int one_tile;           // a CTA takes one query tile instead of two
+  int splits;             // kSplit: parts that a query tile's keys may be cut into
+  unsigned* part_ctr;     // [batch][tiles_m][q_heads], zero between launches
+  float4* part_o;         // [batch][tiles_m][splits][q_heads][32 column quads][128 rows]
+  float2* part_ml;        // [batch][tiles_m][splits][q_heads][128 rows] (m, l)
+  int4* part_nan;         // [batch][tiles_m][splits][q_heads]
 };
 
-template <bool kKv4>
+// The end of a part of a query tile's keys: O, m and l of the row this thread owns go to the part's slot, the
+// group of 128 threads counts itself in, and the group that arrives last joins all parts, in their order, into
+// ov and l_run (true).  A slot is laid out [quad of columns][row], so that a warp's accesses are 512 contiguous
+// bytes.  A row that sees no key of a part has m = -infinity and l = 0 there.
+__device__ __forceinline__ bool join_parts(const PrefillParams& p, int64_t tile, int split, int pieces, int head, int row,
+                                           int barrier, int* nan_pos, int* merge, float m, float& l_run,
+                                           uint32_t (&ov)[kD / 32][32]) {
+  const int64_t slot0 = tile * p.splits * p.q_heads + head;
+  const int64_t slot = slot0 + static_cast<int64_t>(split) * p.q_heads;
+  float4* o = p.part_o + slot * (kD / 4) * kBM + row;
+#pragma unroll
+  for (int c = 0; c < kD / 4; ++c) {
+    const uint32_t* v = ov[c >> 3] + 4 * (c & 7);
+    __stcg(o + c * kBM, make_float4(__uint_as_float(v[0]), __uint_as_float(v[1]), __uint_as_float(v[2]), __uint_as_float(v[3])));
+  }
+  __stcg(p.part_ml + slot * kBM + row, make_float2(m, l_run));
+  if (row == 0) __stcg(p.part_nan + slot, make_int4(nan_pos[0], nan_pos[1], nan_pos[2], nan_pos[3]));
+  asm volatile("bar.sync %0, %1;\n" ::"r"(barrier), "n"(kGroupWarps * 32) : "memory");
+  if (row == 0) {
+    const unsigned last = static_cast<unsigned>(pieces - 1);
+    *merge = atomic_inc_acq_rel(p.part_ctr + tile * p.q_heads + head, last) == last;
+  }
+  asm volatile("bar.sync %0, %1;\n" ::"r"(barrier), "n"(kGroupWarps * 32) : "memory");
+  if (*merge == 0) return false;
+  float top = -INFINITY;
+  for (int i = 0; i < pieces; ++i) top = fmaxf(top, __ldcg(p.part_ml + (slot0 + static_cast<int64_t>(i) * p.q_heads) * kBM + row).x);
+  l_run = 0.f;
+#pragma unroll
+  for (int c = 0; c < kD; ++c) ov[c >> 5][c & 31] = 0u;
+#pragma unroll 1
+  for (int i = 0; i < pieces; ++i) {
+    const int64_t at = slot0 + static_cast<int64_t>(i) * p.q_heads;
+    const float2 ml = __ldcg(p.part_ml + at * kBM + row);
+    const float w = fast_exp2(ml.x - top);
+    l_run += w * ml.y;
+    const float4* src = p.part_o + at * (kD / 4) * kBM + row;
+#pragma unroll
+    for (int c = 0; c < kD / 4; ++c) {
+      const float4 v = __ldcg(src + c * kBM);
+      uint32_t* a = ov[c >> 3] + 4 * (c & 7);
+      a[0] = __float_as_uint(fmaf(w, v.x, __uint_as_float(a[0])));
+      a[1] = __float_as_uint(fmaf(w, v.y, __uint_as_float(a[1])));
+      a[2] = __float_as_uint(fmaf(w, v.z, __uint_as_float(a[2])));
+      a[3] = __float_as_uint(fmaf(w, v.w, __uint_as_float(a[3])));
+    }
+    if (row < 4) atomicMin(nan_pos + row, __ldcg(reinterpret_cast<const int*>(p.part_nan + at) + row));
+  }
+  return true;
+}
+
+// kSplit (4-bit pool): a CTA takes a part of one query tile's keys.  It is a kernel of its own because the joining
+// costs registers that the main loop needs: as one kernel 8 packed prompts of up to 2 k take 350 us instead of
+// 340, two chunks of 500 on 9-16 k 276 instead of 265.
+template <bool kKv4, bool kSplit>
 __global__ void __launch_bounds__(threads_of(kKv4), 1)
 paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
                      const __grid_constant__ CUtensorMap kmap, const __grid_constant__ CUtensorMap vmap) {
@@ -242,7 +306,8 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
   // A CTA takes up to TWO query tiles of its request, one after the other: tile t_b-1-k (many key
   // tiles) and tile k (few), so every CTA of a request does about the same work, and the second
   // tile's Q / K / V loads, barrier set-up and TMEM are already there when the first one drains.
-  const int pair_k = static_cast<int>(blockIdx.y);
+  const int split = kSplit ? static_cast<int>(blockIdx.y) / p.tiles_m : 0;
+  const int pair_k = static_cast<int>(blockIdx.y) - (kSplit ? split * p.tiles_m : 0);
   const int b = blockIdx.z;
   const int64_t q_len = load_len(p.q_lens, p.lens_i64, b);
   const int64_t ctx = load_len(p.ctx_lens, p.lens_i64, b);
@@ -263,7 +328,7 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     return;
   }
   const int t_b = static_cast<int>((q_len + kBM - 1) / kBM);   // query tiles of the request
-  const bool one_tile = kKv4 && p.one_tile;
+  const bool one_tile = kSplit || (kKv4 && p.one_tile);
   if (one_tile ? pair_k >= t_b : pair_k > t_b - 1 - pair_k) {   // also q_len == 0
     leave_early();
     return;
@@ -278,6 +343,7 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     int64_t n_pages;
     int n_tiles;       // 128-key tiles
   };
+  int tile0 = 0, pieces = 1;         // first key tile of this CTA's part, and how many parts there are
   auto work_of = [&](int w) {
     Work k;
     k.row0 = static_cast<int64_t>(w == 0 ? t_b - 1 - pair_k : pair_k) * kBM;
@@ -286,11 +352,22 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     k.kv_len = ctx + k.row0 + k.rows;
     k.n_tiles = static_cast<int>((k.kv_len + kBN - 1) / kBN);
     k.n_pages = (k.kv_len + kPS - 1) / kPS;
+    if (kSplit) {                   // this CTA's part of the key tiles
+      const int part = k.n_tiles < 2 * kMinSplitTiles ? k.n_tiles : max((k.n_tiles + p.splits - 1) / p.splits, kMinSplitTiles);
+      pieces = (k.n_tiles + part - 1) / part;
+      tile0 = split * part;
+      k.n_tiles = min(part, k.n_tiles - tile0);
+      k.n_pages -= static_cast<int64_t>(tile0) * kTilePages;
+    }
     return k;
   };
   const Work work0 = work_of(0), work1 = work_of(n_work - 1);
   if (work0.q_tok0 < 0 || work0.q_tok0 + work0.rows > p.total_q || work1.q_tok0 < 0) {
     set_status(p.status, B200KV_DEV_BAD_LENGTH);
+    leave_early();
+    return;
+  }
+  if (kSplit && split >= pieces) {   // fewer key tiles than parts
     leave_early();
     return;
   }
@@ -310,7 +387,8 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
   const uint32_t bar_qfree = bar_sfree + 8 * kGroups;       // every S of a query tile has completed
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + (bar_qfree + 8 - sm_q));
   int* nan_pos = reinterpret_cast<int*>(tmem_slot + 2);    // [4] first position whose V group reads as NaN
-  static_assert(8 + 2 * 8 * kSlots + 4 * 8 * kGroups + 8 + 8 + 16 <= kBarBytes, "barrier area too small");
+  int* merges = nan_pos + 4;                               // [kGroups] this CTA joins the parts
+  static_assert(8 + 2 * 8 * kSlots + 4 * 8 * kGroups + 8 + 8 + 16 + 4 * kGroups <= kBarBytes, "barrier area too small");
   if ((sm_q & 1023u) != 0) {  // swizzled boxes and UMMA descriptors assume 1024-byte alignment
     set_status(p.status, B200KV_DEV_BAD_PAGE);
     leave_early();
@@ -571,7 +649,7 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     const uint32_t page_stride = static_cast<uint32_t>(p.page_stride);   // the host refuses strides of 2^31 and more
     const int pool_pages = static_cast<int>(p.pool_pages);
     const bool by_token = p.table_kind == B200KV_TABLE_TOKEN;
-    const int32_t* trow = p.table + static_cast<int64_t>(table_row) * p.table_row_stride + (by_token ? lane * kPS : lane);
+    const int32_t* trow = p.table + static_cast<int64_t>(table_row) * p.table_row_stride + (by_token ? kPS : 1) * (lane + static_cast<int64_t>(tile0) * kTilePages);
     const uint32_t dst_row = sm_ring + (c >> 1) * kHalfPage + tp * 128;
     const uint32_t piece0 = static_cast<uint32_t>((j ^ (tp & 7)) << 4), piece1 = static_cast<uint32_t>(((4 + j) ^ (tp & 7)) << 4);
     // One ring item: K or V of key tile `tile` of query tile w; pages 0 .. np - 1 of it exist.
@@ -653,7 +731,7 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
 #pragma unroll
           for (int u = 0; u < kUnits; ++u) {
             if ((c >> 1) + 2 * u >= cur.np) continue;
-            const int pos = cur.tile * kBN + ((c >> 1) + 2 * u) * kPS + tp;
+            const int pos = (tile0 + cur.tile) * kBN + ((c >> 1) + 2 * u) * kPS + tp;
             if ((scales[u].x & 0x7c00u) == 0x7c00u) { scales[u].x &= 0xffff0000u; atomicMin(nan_pos + 0, pos); }
             if ((scales[u].x & 0x7c000000u) == 0x7c000000u) { scales[u].x &= 0xffffu; atomicMin(nan_pos + 1, pos); }
             if ((scales[u].y & 0x7c00u) == 0x7c00u) { scales[u].y &= 0xffff0000u; atomicMin(nan_pos + 2, pos); }
@@ -730,7 +808,7 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
       const uint32_t par = (tile_base + j) & 1;            // phase of the per-key-tile barriers
       if (!mbar_wait_bounded(b_sfull, par)) { ok = false; break; }
       tc_fence_after();
-      const int64_t key0 = static_cast<int64_t>(j) * kBN;
+      const int64_t key0 = static_cast<int64_t>(tile0 + j) * kBN;
       // Only tiles that reach past the first row's diagonal need the causal mask (warp-uniform).
       const bool need_mask = key0 + kBN - 1 > ctx + row0;
       const int lim = static_cast<int>(q_pos - key0 < kBN ? q_pos - key0 : kBN);  // keys c <= lim visible
@@ -843,7 +921,6 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
     if (ok && !mbar_wait_bounded(b_pvfull, (tile_base + n_tiles - 1) & 1)) ok = false;
     {
       tc_fence_after();
-      const float inv = 1.f / l_run;
       const int rows = wk.rows;
       // O / l -> fp16, staged through the group's (now idle) P buffer so that the global stores are
       // whole 256-byte rows: written straight from the registers, a warp's 16-byte stores would
@@ -854,6 +931,13 @@ paged_prefill_kernel(PrefillParams p, const __grid_constant__ CUtensorMap qmap,
 #pragma unroll
       for (int q4 = 0; q4 < kD / 32; ++q4) tmem_ld32(tmem_o + q4 * 32, ov[q4]);   // warp-collective, all in flight
       tmem_ld_wait();
+      if (kSplit && pieces > 1 &&
+          !join_parts(p, static_cast<int64_t>(b) * p.tiles_m + pair_k, split, pieces, head0 + g, row, 2 + g, nan_pos,
+                      merges + g, m_used, l_run, ov)) {
+        tc_fence_before();
+        break;     // another CTA writes these rows
+      }
+      const float inv = 1.f / l_run;
 #pragma unroll
       for (int q4 = 0; q4 < kD / 32; ++q4) {
 #pragma unroll
@@ -965,14 +1049,14 @@ PrefillParams common_params(const PrefillArgs& a) {
   return p;
 }
 
-template <bool kKv4>
+template <bool kKv4, bool kSplit>
 int launch_prefill(const PrefillParams& p, const CUtensorMap& qmap, const CUtensorMap& kmap, const CUtensorMap& vmap,
                    cudaStream_t stream) {
   static bool attr_done[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return record_cuda_error(cudaGetLastError());
   if (dev < 0 || dev >= 64 || !attr_done[dev]) {
-    cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<kKv4>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<kKv4, kSplit>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                          kSmemBytes);
     if (e != cudaSuccess) return record_cuda_error(e);
     if (dev >= 0 && dev < 64) attr_done[dev] = true;
@@ -983,13 +1067,14 @@ int launch_prefill(const PrefillParams& p, const CUtensorMap& qmap, const CUtens
   cudaLaunchConfig_t cfg{};
   // x: (KV head, pair of query heads of its group), adjacent so a group's CTAs share K/V in L2.
   cfg.gridDim = dim3(static_cast<unsigned>(p.kv_heads * ((p.group + 1) / 2)),
-                     static_cast<unsigned>(p.one_tile ? p.tiles_m : (p.tiles_m + 1) / 2), static_cast<unsigned>(p.batch));
+                     static_cast<unsigned>(kSplit ? p.tiles_m * p.splits : p.one_tile ? p.tiles_m : (p.tiles_m + 1) / 2),
+                     static_cast<unsigned>(p.batch));
   cfg.blockDim = dim3(threads_of(kKv4));
   cfg.dynamicSmemBytes = kSmemBytes;
   cfg.stream = stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<kKv4>, p, qmap, kmap, vmap);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prefill_kernel<kKv4, kSplit>, p, qmap, kmap, vmap);
   if (e != cudaSuccess) return record_cuda_error(e);
   return check_launch();
 }
@@ -1011,7 +1096,38 @@ int paged_prefill(const PrefillArgs& a, cudaStream_t stream) {
   rc = cached_kv_tensor_map(&vmap, a.v_base, a.pool_tokens, a.kv_tok_stride, a.kv_head_stride,
                             a.kv_heads, kD, kPS);
   if (rc != B200KV_OK) return rc;
-  return launch_prefill<false>(common_params(a), qmap, kmap, vmap, stream);
+  return launch_prefill<false, false>(common_params(a), qmap, kmap, vmap, stream);
+}
+
+// Query tiles of a launch (one per pair of heads), and the parts that their keys may be cut into where the tiles
+// leave most SMs empty: as many as fill them once (chunk of 500 on 12 k, 32/4 heads, 64 tiles in two parts
+// 125 us, whole 218).  Where the tiles fill more than half of the SMs, finer parts would even out the last wave, but
+// a CTA's start and the joining (17 us together) cost what that gives.
+int64_t query_tiles(int batch, int64_t max_q_len, int q_heads, int kv_heads) {
+  return static_cast<int64_t>(batch) * kv_heads * ((q_heads / kv_heads + 1) / 2) * ((max_q_len + kBM - 1) / kBM);
+}
+int splits_of(int64_t tiles, int sms) {
+  const int64_t s = tiles > 0 ? sms / tiles : 1;
+  return static_cast<int>(s < 1 ? 1 : s > kMaxSplits ? kMaxSplits : s);
+}
+struct SplitLayout {
+  int64_t ml, nan, total;   // byte offsets behind the counters and the partial outputs
+};
+SplitLayout split_layout(int batch, int64_t tiles_m, int splits, int q_heads) {
+  const int64_t slots = static_cast<int64_t>(batch) * tiles_m * splits * q_heads;
+  SplitLayout l;
+  l.ml = static_cast<int64_t>(B200KV_DECODE_COUNTER_BYTES) + slots * kBM * kD * 4;
+  l.nan = l.ml + slots * kBM * 8;
+  l.total = l.nan + slots * 16;
+  return l;
+}
+
+size_t kv4_split_workspace_bytes(int batch, int64_t max_q_len, int q_heads, int kv_heads) {
+  const int sms = device_sm_count();
+  if (sms <= 0) return 0;
+  const int splits = splits_of(query_tiles(batch, max_q_len, q_heads, kv_heads), sms);
+  if (splits <= 1) return 0;
+  return static_cast<size_t>(split_layout(batch, (max_q_len + kBM - 1) / kBM, splits, q_heads).total);
 }
 
 int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
@@ -1024,8 +1140,7 @@ int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
   rc = kv4_check_pool(k.pool, k.pool_pages, k.page_stride_bytes, a.kv_heads);
   if (rc != B200KV_OK) return rc;
   // A few query rows over a long context: streamed like a decode step (kv4_decode.cu).
-  if (k.workspace != nullptr && kv4_chunk_workspace_bytes(a.batch, a.max_q_len, a.q_heads, a.kv_heads, a.head_dim) > 0)
-    return kv4_paged_chunk(k, stream);
+  if (k.workspace != nullptr && kv4_streams_chunk(a.batch, a.max_q_len, a.q_heads, a.kv_heads)) return kv4_paged_chunk(k, stream);
   CUtensorMap qmap;
   rc = encode_q_tensor_map(&qmap, a.q, a.total_q, a.q_stride_t, a.q_stride_h, a.q_heads);
   if (rc != B200KV_OK) return rc;
@@ -1041,7 +1156,17 @@ int kv4_paged_prefill(const Kv4PrefillArgs& k, cudaStream_t stream) {
   if (sms <= 0) return B200KV_ECUDA;
   const int64_t paired = static_cast<int64_t>(a.kv_heads) * ((p.group + 1) / 2) * ((p.tiles_m + 1) / 2) * a.batch;
   p.one_tile = paired < sms && p.tiles_m <= 65535;
-  return launch_prefill<true>(p, qmap, qmap, qmap, stream);
+  p.splits = splits_of(query_tiles(a.batch, a.max_q_len, a.q_heads, a.kv_heads), sms);
+  if (k.workspace == nullptr || p.splits <= 1) return launch_prefill<true, false>(p, qmap, qmap, qmap, stream);
+  if ((reinterpret_cast<uintptr_t>(k.workspace) & 15u) != 0) return B200KV_EALIGN;
+  const SplitLayout l = split_layout(a.batch, p.tiles_m, p.splits, a.q_heads);
+  if (k.workspace_bytes < static_cast<size_t>(l.total)) return B200KV_EWORKSPACE;
+  uint8_t* ws = static_cast<uint8_t*>(k.workspace);
+  p.part_ctr = reinterpret_cast<unsigned*>(ws);
+  p.part_o = reinterpret_cast<float4*>(ws + B200KV_DECODE_COUNTER_BYTES);
+  p.part_ml = reinterpret_cast<float2*>(ws + l.ml);
+  p.part_nan = reinterpret_cast<int4*>(ws + l.nan);
+  return launch_prefill<true, true>(p, qmap, qmap, qmap, stream);
 }
 
 }  // namespace b200kv

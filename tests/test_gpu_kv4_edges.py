@@ -417,3 +417,78 @@ def test_prefill_refuses_scales_that_are_not_positive():
             kernels.paged_chunk_flash_attention_kv4(
                 c.q.to(DEV), c.pool.to(DEV), scale, c.tables("block"), c.rows.to(DEV), torch.zeros(1, dtype=torch.int32, device=DEV),
                 torch.zeros(1, dtype=torch.int64, device=DEV), torch.tensor([20], device=DEV), 20, table_kind="block")
+
+
+SPLIT = [   # few query tiles: their keys are cut into parts
+    ([3000], [200], 2, 1), ([2500, 100], [130, 100], 16, 2), ([1700, 33, 600], [150, 33, 130], 3, 1), ([700], [300], 1, 1),
+    ([2049], [129], 5, 1), ([513, 512], [257, 129], 1, 1), ([4000, 1], [140, 1], 8, 1), ([1300], [129], 8, 8),
+]
+
+
+@pytest.mark.parametrize("lens, q_lens, qh, kvh", SPLIT)
+def test_keys_of_a_few_query_tiles_are_cut_into_parts(lens, q_lens, qh, kvh):
+    c = Case(sum(lens) + qh, lens, qh, kvh, q_lens)
+    want, _, tol = c.want()
+    assert _lib.lib().b200kv_kv4_chunk_workspace_bytes(len(lens), max(q_lens), qh, kvh, 128) > 1 << 18
+    got = c.prefill("block").clone()
+    _within(got, want, tol)
+    for _ in range(3):                        # the order in which parts arrive does not matter
+        assert torch.equal(c.prefill("token", torch.int32), got)
+    assert not any(bool(ws[: kernels.DECODE_COUNTER_BYTES].any()) for ws in kernels._kv4_workspace.values())
+
+
+def test_cut_keys_nan_reaches_only_the_rows_that_see_it():
+    c = Case(91, [2000, 800], 4, 2, [150, 130])
+    x = _randn(92, (2000, 4, 128))
+    x[1900, 2, 70] = float("nan")       # V of head 0, group 2, seen by rows 50 on
+    x[1960, 1, 0] = float("inf")        # K of head 1
+    x[1870, 3, 5] = float("-inf")       # V of head 1, group 0, seen by rows 20 on
+    K4.append(x, c.slots[0], c.pool)
+    c.values[0] = K4.rows_of(c.pool, c.slots[0])
+    want, _, tol = c.want()
+    got = c.prefill().cpu()
+    assert bool(got[50:150, :2, 64:96].isnan().all()) and not bool(got[:50, :2].isnan().any())
+    assert bool(got[110:150, 2:].isnan().all()) and bool(got[20:150, 2:, :32].isnan().all())
+    assert not bool(got[:20].isnan().any()) and not bool(got[150:].isnan().any())
+    _within(got, want, tol)
+
+
+def test_cut_keys_value_ranges_and_unwritten_places():
+    for gain_k, gain_v in ((15.0, 1.0), (1.0, 2000.0), (1.0, 1e-5)):
+        c = Case(93, [1500, 31], 4, 1, [140, 31], gain_k=gain_k, gain_v=gain_v)
+        want, _, tol = c.want()
+        _within(c.prefill(), want, tol)
+    fill = torch.full_like(c.pool, 0xF0)
+    fill.view(torch.int16)[..., 512:] = GARBAGE[1]
+    for s in c.slots:
+        _take(fill, c.pool, s)
+    _within(c.prefill(pool=fill.to(DEV)), want, tol)
+
+
+def test_cut_keys_in_graphs_and_on_two_streams():
+    a, b = Case(95, [3000], 8, 1, [200]), Case(96, [1500, 900], 4, 2, [130, 260])
+    want = [c.prefill().clone() for c in (a, b)]
+    calls = []
+    for c in (a, b):
+        ql = torch.tensor(c.q_lens)
+        args = (c.q.to(DEV), c.pool.to(DEV), SCALE * LOG2E, c.tables("block"), c.rows.to(DEV), (ql.cumsum(0) - ql).int().to(DEV),
+                (torch.tensor(c.lens) - ql).to(DEV), ql.to(DEV), max(c.q_lens))
+        calls.append(lambda args=args: kernels.paged_chunk_flash_attention_kv4(*args, table_kind="block"))
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for call in calls:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append([call() for _ in range(2)])
+        graphs.append(g)
+    streams = torch.cuda.Stream(), torch.cuda.Stream()
+    for _ in range(5):
+        eager = []
+        for i in (0, 1):
+            with torch.cuda.stream(streams[i]):
+                graphs[i].replay()
+                eager.append(calls[i]())
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            for o in outs[i] + [eager[i]]:
+                assert torch.equal(o, want[i])
