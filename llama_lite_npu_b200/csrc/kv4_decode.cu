@@ -1054,11 +1054,17 @@ int run_decode(Kv4Params& p, int q_heads, const Shape& s, void* workspace, size_
 
 inline bool misaligned(const void* ptr, uintptr_t al) { return (reinterpret_cast<uintptr_t>(ptr) & (al - 1)) != 0; }
 
-// Columns (query tokens x heads of a group) up to which a chunk is streamed like a decode step.  Streaming costs a
-// pass per 16 columns, the 128-row tiles the same whatever part of them is filled.  Streamed / tiles, us: 8 requests
-// on contexts of 1-4 k, 64/8 heads, 64 columns 42 / 132, 128 columns 80 / 134; 32 such requests, 128 columns
-// 290 / 427 (twice as many columns cost twice the passes, i.e. about the tiles' time or more).
+// A chunk is streamed like a decode step when it has at most kChunkRows rows, and at most kChunkColumns columns (rows
+// x heads of a group) or at most kChunkWork columns over all KV heads and requests.  Streaming costs a pass over
+// the keys per 16 columns; the 128-row tiles cost the same whatever part of them is filled, but have few CTAs to
+// spread over when there are few heads and requests.  Streamed / tiles, us, contexts of 2 k and 12 k:
+//   128 columns: 1 request, 32/4 heads 13.7 / 27.8 and 26.8 / 54.6; 4 requests, 64/8 heads 30.3 / 42.1 and 141 / 211
+//   256 columns: 1 request, 32/4 heads 16.7 / 27.8 and 43.6 / 55.2; 4 requests, 64/8 heads 56.5 / 42.4 and 278 / 213
+//   1024 columns in all, contexts of 1 k and 12 k: 1 request, 8/1 heads 14.1 / 23.9 and 45.0 / 54.8; 2048: 2 requests
+//   18.0 / 24.9 and 79.3 / 60.2
+constexpr int kChunkRows = 128;
 constexpr int kChunkColumns = 128;
+constexpr int kChunkWork = 1024;
 
 }  // namespace
 
@@ -1073,7 +1079,9 @@ size_t kv4_decode_workspace_bytes(int batch, int q_heads, int kv_heads, int head
 
 // Does a chunk of at most max_q_len rows go through this file's kernel (given a workspace)?
 bool kv4_streams_chunk(int batch, int64_t max_q_len, int q_heads, int kv_heads) {
-  if (batch > 4096 || max_q_len * (q_heads / kv_heads) > kChunkColumns) return false;
+  if (batch > 4096 || max_q_len > kChunkRows) return false;
+  const int64_t cols = max_q_len * (q_heads / kv_heads);
+  if (cols > kChunkColumns && cols * kv_heads * batch > kChunkWork) return false;
   Shape s;
   return shape_of(static_cast<int>(max_q_len), q_heads, kv_heads, &s) == B200KV_OK &&
          static_cast<int64_t>(batch) * kv_heads * s.blocks <= kMaxCounters;
@@ -1137,7 +1145,7 @@ int kv4_paged_decode(const Kv4DecodeArgs& a, cudaStream_t stream) {
                     (a.flags & B200KV_DECODE_SERIALIZED) == 0, stream);
 }
 
-// A chunk of at most kChunkColumns columns; the arguments have been checked (kv4_paged_prefill).
+// A chunk that is streamed (kv4_streams_chunk); the arguments have been checked (kv4_paged_prefill).
 int kv4_paged_chunk(const Kv4PrefillArgs& k, cudaStream_t stream) {
   const PrefillArgs& a = k.args;
   if (misaligned(a.q, 16) || a.q_stride_t % 8 != 0 || a.q_stride_h % 8 != 0 || misaligned(k.workspace, 16)) return B200KV_EALIGN;

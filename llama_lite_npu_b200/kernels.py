@@ -1136,8 +1136,8 @@ def paged_chunk_flash_attention_kv4(
         _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, tbl_rows, "paged prefill")
         _debug_check_lengths(q_seq_lens, int(max_q_len), None, 0, "paged prefill chunk")   # longer ones are skipped
     max_q_len = int(max_q_len)
-    # Scratch: chunks of at most 128 columns (rows x heads of a group) are streamed like a decode step, and the keys
-    # of a few query tiles are cut into parts.  Beyond 128 rows only their number of 128-row tiles counts.
+    # Scratch: chunks of few rows and heads are streamed like a decode step, and the keys of a few query tiles are cut
+    # into parts.  Beyond 128 rows only their number of 128-row tiles counts.
     rows = max_q_len if max_q_len <= 128 else (max_q_len + 127) // 128 * 128
     ws = kv4_workspace(dev, batch, rows, q_heads, kv_heads) if rows > 0 else None
     _kv4_call(_KV4_PREFILL, dev, q.data_ptr(), q.stride(0) if total_q > 1 else q_heads * d, q.stride(1) if q_heads > 1 else d,

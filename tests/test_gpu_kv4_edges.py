@@ -492,3 +492,13 @@ def test_cut_keys_in_graphs_and_on_two_streams():
         for i in (0, 1):
             for o in outs[i] + [eager[i]]:
                 assert torch.equal(o, want[i])
+
+
+@pytest.mark.parametrize("lens, q_lens, qh, kvh", [   # more than 128 columns, few heads and requests: streamed; the last two are not
+    ([500], [40], 8, 1), ([300, 61], [60, 7], 4, 1), ([900], [128], 8, 1), ([77, 3], [32, 3], 16, 2), ([1000, 41, 5], [85, 30, 1], 4, 1),
+    ([900], [129], 8, 1), ([400, 300], [65, 64], 8, 1)])
+def test_chunks_of_many_columns_on_few_heads(lens, q_lens, qh, kvh):
+    c = Case(sum(lens) + qh, lens, qh, kvh, q_lens)
+    want, _, tol = c.want()
+    _within(c.prefill("block"), want, tol)
+    _within(c.prefill("token", torch.int32), want, tol)
