@@ -38,7 +38,10 @@
 // them (conflict-free 16-byte shared loads).  The page table is read 32 entries at a time, one block of
 // entries ahead of use.
 //
-// Bytes per token and KV head: 2 * 72 (a page is 2304 B where fp16 has 8192).
+// Bytes per token and KV head: 2 * 72 (a page is 2304 B where fp16 has 8192).  32 sequences of 1-4 k tokens, 64/8
+// heads: 25.9 us = 3.68 TB/s where the fp16 cache takes 57.9; 48 sequences of up to 16 k 34.2 us (fp16 76.9).  Half of the
+// rate of a copy: a step's chain (wait, unpack, two products, exponentials) over the 12 warps of an SM bounds it, issue
+// slots are 52 % busy, and leaving out the unpacking (22.9 us), V (21.7) or K (21.1) shortens it little.
 #include <climits>
 #include <cmath>
 
@@ -61,8 +64,8 @@ constexpr int kRingBytes = kWarps * kStages * kPairBytes;
 constexpr int kMinPagesPerTeam = 4;                // a team is not worth launching for fewer pages
 constexpr int kPieceCost = 16;
 constexpr float kNoScore = -3.0e38f;               // the reference of sums over no token; finite, so that differences are
-// Resident CTAs per SM.  Three of them leave 168 registers, which a step of two pages needs (four spill
-// and were slower: 36.4 against 33.0 us on 32 sequences of 1-4 k tokens, 64/8 heads).
+// Resident CTAs per SM.  Three of them leave 168 registers, which a step of two pages needs (32 sequences of 1-4 k
+// tokens, 64/8 heads, us: four, with spills, 31.0; three 25.9; two with 184 registers 26.6).
 constexpr int ctas_per_sm(int rows) { return rows == 8 ? 3 : 2; }
 constexpr size_t kCounterBytes = B200KV_DECODE_COUNTER_BYTES;
 constexpr int64_t kMaxCounters = static_cast<int64_t>(kCounterBytes / sizeof(unsigned));

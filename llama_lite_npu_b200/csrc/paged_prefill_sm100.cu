@@ -38,15 +38,17 @@
 // in the reference (:166, :220), output fp16.  Tensor-bound:
 // flops = 4 * 128 * sum over (query, visible key) pairs, per query head.
 //
-// Over a 4-bit cache (kKv4, include/b200kv_kv4.h) a launch of few query tiles cuts their keys into parts, one CTA
-// each, that the CTA which arrives last joins; and the same pipeline runs with a fourth warpgroup: its four
+// Over a 4-bit cache (kKv4, include/b200kv_kv4.h) the same pipeline runs with a fourth warpgroup: its four
 // warps read the blocks of codes and scales straight from the pool, one ring item ahead of use in
 // registers, turn them into fp16 (code - 8) * scale, and store each word of codes as one 16-byte piece of
-// the K or V tile where the copies would have put it (72 bytes read per row instead of 256).  The
-// registers are split 168 for the softmax warps, 88 for the rest.  A group of V whose
-// scale is NaN must reach only the rows that see its token, and 0 * NaN would reach all: such groups
-// are stored as zeros, the first such position of each group is kept, and the read-out writes NaN from
-// that position on.
+// the K or V tile where the copies would have put it (72 bytes read per row instead of 256).  That product
+// is rounded once, to fp16 (a code has 4 bits and a scale 11; the tensor core takes 11): half a step, as the
+// fp16 cache's own rounding of K and V.  The registers are split 168 for the softmax warps, 88 for the rest.
+// A group of V whose scale is NaN must reach only the rows that see its token, and 0 * NaN would reach
+// all: such groups are stored as zeros, the first such position of each group is kept, and the read-out writes
+// NaN from that position on.  A launch of few query tiles cuts their keys into parts, one CTA each, that the
+// CTA which arrives last joins.  8 packed prompts of up to 2 k, 64/8 heads: 339 us = 626 TFLOP/s of 1645 (the fp16
+// cache 293); two chunks of 500 on 9-16 k, 32/4 heads, 266 us = 663 TFLOP/s (fp16, which pairs its tiles, 477).
 //
 // Every wait is an mbarrier try-wait bounded by ~2 s of %globaltimer; a wait that runs out sets
 // B200KV_DEV_WAIT_TIMEOUT, and every warp still reaches the common exit where TMEM is freed.
@@ -168,31 +170,7 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void tmem_ld_wait() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
 
-// Packed fp32 pairs (sm_100 f32x2 arithmetic) and the 3-input maximum.
-__device__ __forceinline__ uint64_t pack_u32x2(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ uint64_t pack_f32x2(float lo, float hi) {
-  return pack_u32x2(__float_as_uint(lo), __float_as_uint(hi));
-}
-__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& lo, float& hi) {
-  uint32_t a, b;
-  asm("mov.b64 {%0, %1}, %2;\n" : "=r"(a), "=r"(b) : "l"(v));
-  lo = __uint_as_float(a);
-  hi = __uint_as_float(b);
-}
-__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
+// The 3-input maximum.
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;\n" : "=f"(d) : "f"(a), "f"(b), "f"(c));
