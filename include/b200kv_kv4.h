@@ -144,19 +144,6 @@ int b200kv_kv4_paged_prefill(const void* q, int64_t q_stride_t, int64_t q_stride
                              void* workspace, size_t workspace_bytes,
                              int32_t* status, void* stream);
 
-/*
- * One of the five launches above with its n arguments as an array of 64-bit words in the order of its
- * parameters: pointers and integers as they are, a float as the bits of a double.  For callers to whom every
- * argument of a foreign call costs time (from Python 27 arguments take 2.7 us, packing them and passing the
- * array 0.7).  A wrong op or n, or a word outside an int parameter's range, is B200KV_EINVAL.
- */
-#define B200KV_KV4_OP_APPEND 0
-#define B200KV_KV4_OP_QK_NORM_ROPE_APPEND 1
-#define B200KV_KV4_OP_GATHER 2
-#define B200KV_KV4_OP_PAGED_DECODE 3
-#define B200KV_KV4_OP_PAGED_PREFILL 4
-int b200kv_kv4_call(int op, const int64_t* words, int n);
-
 #ifdef __cplusplus
 }
 #endif

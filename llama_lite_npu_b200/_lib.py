@@ -1,4 +1,5 @@
-"""ctypes binding of libb200kv.so — the only route from Python to the CUDA kernels.
+"""ctypes binding of libb200kv.so — the only route from Python to the CUDA kernels (the 4-bit operators'
+extension module, csrc/kv4_python.c, is given the entry points' addresses from here).
 
 There is deliberately no fallback: if the shared library is missing or a symbol
 cannot be resolved, importing this module's :func:`lib` raises, and every
@@ -8,7 +9,6 @@ operator in :mod:`llama_lite_npu_b200.kernels` fails with it.
 from __future__ import annotations
 
 import ctypes
-import struct
 from ctypes import c_char_p, c_float, c_int, c_int32, c_int64, c_size_t, c_uint64, c_void_p
 from pathlib import Path
 
@@ -142,7 +142,6 @@ _SIGNATURES = {
          c_void_p, c_void_p, c_int, c_int, c_int64, c_int64,
          c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int64, c_void_p, c_size_t, c_void_p, c_void_p],
     ),
-    "b200kv_kv4_call": (c_int, [c_int, c_char_p, c_int]),   # packed words, see kv4_packer
     # host-side prefix cache (include/b200kv_prefix_cache.h)
     "b200kv_prefix_cache_create": (c_void_p, [c_int, c_int64, c_int64]),
     "b200kv_prefix_cache_destroy": (None, [c_void_p]),
@@ -177,13 +176,6 @@ _SIGNATURES = {
 }
 
 EXPORTED_SYMBOLS = tuple(_SIGNATURES)
-
-
-def kv4_packer(name: str):
-    """``(pack, number of words)`` for ``b200kv_kv4_call``: packs the arguments of entry point ``name``."""
-    argtypes = _SIGNATURES[name][1]
-    return struct.Struct("=" + "".join("d" if t is c_float else "q" for t in argtypes)).pack, len(argtypes)
-
 
 _lib = None
 

@@ -12,6 +12,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -19,6 +20,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = PKG_DIR.parent / "include"
 LIB_PATH = PKG_DIR / "libb200kv.so"
 STAMP_PATH = PKG_DIR / "libb200kv.stamp"
+NATIVE_PATH = PKG_DIR / "_kv4_native.so"        # CPython extension: argument checks of the 4-bit operators
 
 SOURCES = (
     "b200kv_capi.cu",
@@ -53,19 +55,21 @@ def _find_nvcc() -> str:
 def _source_digest() -> str:
     h = hashlib.sha256()
     files = (sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h"))
-             + sorted(CSRC.glob("*.cpp")))
+             + sorted(CSRC.glob("*.cpp")) + sorted(CSRC.glob("*.c")))
     files += sorted(INCLUDE.glob("*.h"))
     for f in files:
         h.update(f.name.encode())
         h.update(f.read_bytes())
     h.update(" ".join(NVCC_FLAGS).encode())
+    h.update(sysconfig.get_paths()["include"].encode())
     return h.hexdigest()
 
 
 def build_library(force: bool = False, verbose: bool = False) -> Path:
-    """Compile every CUDA source into ``libb200kv.so``; skip when sources are unchanged."""
+    """Compile every CUDA source into ``libb200kv.so``, and the extension module beside it; skip when sources are
+    unchanged."""
     digest = _source_digest()
-    if not force and LIB_PATH.exists() and STAMP_PATH.exists():
+    if not force and LIB_PATH.exists() and NATIVE_PATH.exists() and STAMP_PATH.exists():
         if STAMP_PATH.read_text().strip() == digest:
             return LIB_PATH
     nvcc = _find_nvcc()
@@ -94,6 +98,12 @@ def build_library(force: bool = False, verbose: bool = False) -> Path:
     if res.returncode != 0:
         sys.stderr.write(res.stdout)
         raise RuntimeError("linking libb200kv.so failed")
+    native = ["gcc", "-O2", "-std=gnu11", "-shared", "-fPIC", f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
+              str(CSRC / "kv4_python.c"), "-o", str(NATIVE_PATH)]
+    res = subprocess.run(native, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
+    if res.returncode != 0:
+        sys.stderr.write(res.stdout)
+        raise RuntimeError("building _kv4_native.so failed")
     STAMP_PATH.write_text(digest)
     if verbose:
         sys.stdout.write("\n".join(log))

@@ -1,11 +1,8 @@
 // extern "C" surface of libb200kv.so: argument marshalling only, see include/b200kv.h.
 #include <cuda_runtime.h>
 
-#include <climits>
 #include <cstdio>
 #include <cstring>
-#include <type_traits>
-#include <utility>
 
 #include "b200kv.h"
 #include "b200kv_kv4.h"
@@ -23,37 +20,6 @@ int record_cuda_error(cudaError_t e) {
                 cudaGetErrorString(e));
   return B200KV_ECUDA;
 }
-
-namespace {
-
-// Calls with the arguments in an array of 64-bit words: is a word within the parameter's type, and what is it?
-template <typename T>
-bool word_fits(int64_t w) {
-  return !std::is_same<T, int>::value || (w >= INT_MIN && w <= INT_MAX);
-}
-template <typename T>
-T word_as(int64_t w) {
-  if constexpr (std::is_pointer<T>::value) {
-    return reinterpret_cast<T>(static_cast<uintptr_t>(w));
-  } else if constexpr (std::is_floating_point<T>::value) {
-    double d;
-    std::memcpy(&d, &w, sizeof(d));
-    return static_cast<T>(d);
-  } else {
-    return static_cast<T>(w);
-  }
-}
-template <typename... A, size_t... I>
-int call_words(int (*fn)(A...), const int64_t* w, int n, std::index_sequence<I...>) {
-  if (n != static_cast<int>(sizeof...(A)) || !(word_fits<A>(w[I]) && ...)) return B200KV_EINVAL;
-  return fn(word_as<A>(w[I])...);
-}
-template <typename... A>
-int call_words(int (*fn)(A...), const int64_t* w, int n) {
-  return call_words(fn, w, n, std::index_sequence_for<A...>());
-}
-
-}  // namespace
 
 int check_launch() { return record_cuda_error(cudaGetLastError()); }
 
@@ -401,18 +367,6 @@ int b200kv_kv4_gather(const void* pool, int64_t pool_pages, int64_t page_stride_
                       void* stream) {
   return b200kv::kv4_gather(pool, pool_pages, page_stride_bytes, slots, n, out, out_tok_stride, kv_heads, head_dim,
                             status, static_cast<cudaStream_t>(stream));
-}
-
-int b200kv_kv4_call(int op, const int64_t* words, int n) {
-  if (words == nullptr) return B200KV_EINVAL;
-  switch (op) {
-    case B200KV_KV4_OP_APPEND: return b200kv::call_words(b200kv_kv4_append, words, n);
-    case B200KV_KV4_OP_QK_NORM_ROPE_APPEND: return b200kv::call_words(b200kv_kv4_qk_norm_rope_append, words, n);
-    case B200KV_KV4_OP_GATHER: return b200kv::call_words(b200kv_kv4_gather, words, n);
-    case B200KV_KV4_OP_PAGED_DECODE: return b200kv::call_words(b200kv_kv4_paged_decode, words, n);
-    case B200KV_KV4_OP_PAGED_PREFILL: return b200kv::call_words(b200kv_kv4_paged_prefill, words, n);
-    default: return B200KV_EINVAL;
-  }
 }
 
 int b200kv_stream_capture_id(void* stream, uint64_t* id) {

@@ -4,8 +4,8 @@ and called from ``Attention.context_forward`` / ``token_forward``,
 ``lite_llama/models/qwen3.py:20-75``).
 
 Every function validates its tensors on the host, then makes exactly one call
-into ``libb200kv.so`` through ctypes with raw device pointers and the current
-CUDA stream.  PyTorch is used for memory (outputs, the split-KV workspace) and
+into ``libb200kv.so`` through ctypes (the 4-bit operators: through the extension module
+``_kv4_native``) with raw device pointers and the current CUDA stream.  PyTorch is used for memory (outputs, the split-KV workspace) and
 streams only.  There is no CPU path: tensors must live on a CUDA device and the
 shared library must be present.
 
@@ -45,6 +45,7 @@ _workspace: dict[int, torch.Tensor] = {}
 _retired_workspaces: list[torch.Tensor] = []
 _kv4_workspace: dict[tuple, torch.Tensor] = {}       # (device, stream) -> eager calls
 _kv4_graph_workspace: dict[tuple, tuple] = {}        # (device, stream) -> (capture id, tensor)
+_kv4_need: dict[tuple, int] = {}                     # shape -> bytes of scratch
 
 
 def _device_index(t: torch.Tensor) -> int:
@@ -759,90 +760,49 @@ def empty_kv4_buffer(num_pages: int, kv_heads: int, device="cuda:0") -> torch.Te
     return torch.empty((int(num_pages), 2 * int(kv_heads), KV4_BLOCK_BYTES), dtype=torch.uint8, device=device)
 
 
-def _kv4_pool(t: torch.Tensor):
-    """``(device index, pointer, pages, page stride in bytes, kv_heads)`` of a 4-bit pool.
-
-    These operators run once per layer and step, and their kernels take a few microseconds: each
-    tensor attribute is read once and nothing is formatted unless it is raised."""
-    dev = t.get_device()
-    if dev < 0:
-        _device_index(t)     # raises
-    if t.dtype is not torch.uint8 or t.dim() != 3:
-        raise ValueError(f"KV4_Buffer must be uint8 [num_pages, 2*kv_heads, {KV4_BLOCK_BYTES}]")
-    pages, rows, block = t.shape
-    s0, s1, s2 = t.stride()
-    if block != KV4_BLOCK_BYTES or rows == 0 or rows & 1:
-        raise ValueError(f"KV4_Buffer must be uint8 [num_pages, 2*kv_heads, {KV4_BLOCK_BYTES}]")
-    if s2 != 1 or s1 != KV4_BLOCK_BYTES:
-        raise ValueError("KV4_Buffer must be contiguous inside a page")
-    if pages <= 1:          # the stride of a dimension of one may be anything
-        s0 = max(s0, rows * KV4_BLOCK_BYTES)
-    return dev, t.data_ptr(), pages, s0, rows >> 1
-
-
-def _off_device(name: str, t: torch.Tensor, dev: int) -> ValueError:
-    return ValueError(f"{name} must be on the pool's device cuda:{dev} (got {t.device})")
-
-
-def _slots_arg(slots: torch.Tensor, dev: int) -> torch.Tensor:
-    if slots.dtype is not torch.int32 or slots.dim() != 1:
-        raise ValueError("Select_Index must be a 1-D int32 tensor")
-    if slots.get_device() != dev:
-        raise _off_device("Select_Index", slots, dev)
-    return slots if slots.is_contiguous() else slots.contiguous()
-
-
-def _table_arg(tbl: torch.Tensor, table_kind: str, dev: int):
-    """``(pointer, row stride, kind, rows, columns)`` of a page or token table."""
-    kind = _TABLE_KINDS.get(table_kind, -1)
-    if kind != TABLE_BLOCK and kind != TABLE_TOKEN:
-        raise ValueError("the 4-bit operators take a 'token' or 'block' table")
-    strides = tbl.stride()
-    if tbl.dtype is not torch.int32 or len(strides) != 2 or strides[1] != 1:
-        raise ValueError("the table must be a 2-D int32 tensor contiguous along its last dimension")
-    if tbl.get_device() != dev:
-        raise _off_device("the table", tbl, dev)
-    rows, cols = tbl.shape
-    return tbl.data_ptr(), strides[0] if rows > 1 else cols, kind, rows, cols
-
-
-def _ints_arg(t: torch.Tensor, name: str, n: int, dev: int, wide: bool) -> int:
-    """Pointer of a contiguous 1-D tensor of ``n`` int32 (or, where ``wide``, int64) values."""
-    dtype = t.dtype
-    if (dtype is not torch.int32 and not (wide and dtype is torch.int64)) or t.shape != (n,) or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous 1-D {'int32 or int64' if wide else 'int32'} tensor of {n} values")
-    if t.get_device() != dev:
-        raise _off_device(name, t, dev)
-    return t.data_ptr()
-
-
-def _rows_arg(t: torch.Tensor, name: str, heads: int, n: int, dev: int):
-    """``(pointer, token stride)`` of fp16 head rows ``[>= n, heads, 128]``, contiguous inside a token."""
-    if t.dtype is not torch.float16 or t.dim() != 3:
-        raise ValueError(f"{name} must be float16 [tokens, {heads}, {KV4_HEAD_DIM}]")
-    m, h, d = t.shape
-    s0, s1, s2 = t.stride()
-    if h != heads or d != KV4_HEAD_DIM or m < n:
-        raise ValueError(f"{name} must be float16 [{n} or more, {heads}, {KV4_HEAD_DIM}] (got {tuple(t.shape)})")
-    if s2 != 1 or (s1 != KV4_HEAD_DIM and heads > 1):
-        raise ValueError(f"{name} must be contiguous inside a token")
-    if t.get_device() != dev:
-        raise _off_device(name, t, dev)
-    return t.data_ptr(), s0 if n > 1 else heads * KV4_HEAD_DIM
-
-
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_capturing = torch._C._cuda_isCurrentStreamCapturing if hasattr(torch._C, "_cuda_isCurrentStreamCapturing") else \
-    torch.cuda.is_current_stream_capturing
 
 
-def _capture_of(stream: int) -> int:
-    """Identifier of the graph capture the stream records, 0 for none."""
-    found = _ctypes.c_uint64(0)
-    rc = _lib.lib().b200kv_stream_capture_id(stream, _ctypes.addressof(found))
-    if rc != 0:
-        _lib.check(rc)
-    return found.value
+def _kv4_parts() -> dict:
+    """What the extension module works with: torch's objects, this module's, and the library's entry points."""
+    lib = _lib.lib()
+    entry = lambda f: _ctypes.cast(f, _ctypes.c_void_p).value  # noqa: E731
+    return {
+        "float16": torch.float16, "int32": torch.int32, "int64": torch.int64, "uint8": torch.uint8,
+        "empty": torch.empty, "empty_like": torch.empty_like, "current_device": _current_device,
+        "raw_stream": _raw_stream or _stream, "status": _status, "status_ptr": _status_ptr,
+        "workspace": _kv4_scratch, "on_device": _kv4_on_device, "refuse_cpu": _device_index, "check": _lib.check,
+        "append": entry(lib.b200kv_kv4_append), "prologue": entry(lib.b200kv_kv4_qk_norm_rope_append),
+        "gather": entry(lib.b200kv_kv4_gather), "decode": entry(lib.b200kv_kv4_paged_decode),
+        "prefill": entry(lib.b200kv_kv4_paged_prefill), "capture_id": entry(lib.b200kv_stream_capture_id)}
+
+
+class _Kv4Native:
+    """Stands in for the extension module until the first call, which loads and connects it."""
+
+    def __getattr__(self, name: str):
+        global _kv4
+        parts = _kv4_parts()
+        try:
+            from . import _kv4_native as module
+        except ImportError as e:
+            raise ImportError("llama_lite_npu_b200/_kv4_native.so not found: build it with "
+                              "`python -m llama_lite_npu_b200.build`") from e
+        module.setup(parts)
+        _kv4 = module
+        return getattr(module, name)
+
+
+# The checks and launches of the 4-bit operators (csrc/kv4_python.c).  A call reads about thirty tensor attributes and
+# its kernel takes a few microseconds.  Host time per call, us, with the checks in Python and the launch through
+# ctypes / here: decode 13.3 / 7.2, append 6.8 / 3.8, read-back 8.4 / 5.5.
+_kv4 = _Kv4Native()
+
+
+def _kv4_on_device(device_index: int, name: str, *args):
+    """The native call again with the tensors' device made current."""
+    with torch.cuda.device(device_index):
+        return getattr(_kv4, name)(*args)
 
 
 def _status_ptr(device_index: int) -> int:
@@ -850,46 +810,36 @@ def _status_ptr(device_index: int) -> int:
     zero-fill would become part of the graph)."""
     st = _status.get(device_index)
     if st is None:
-        if _capturing():
+        if torch.cuda.is_current_stream_capturing():
             return 0
         st = status_tensor(device_index)
     return st.data_ptr()
 
 
-def _kv4_workspace_need(device_index: int, batch: int, max_q_len: int, q_heads: int, kv_heads: int) -> int:
-    """Bytes of scratch of a decode step (``max_q_len`` 0) or a chunk; 0 for a chunk that needs none."""
-    key = ("kv4", device_index, batch, max_q_len, q_heads, kv_heads)
-    need = _workspace_need.get(key)
-    if need is None:
-        lib = _lib.lib()
-        with _on_device(device_index):
-            if max_q_len:
-                need = lib.b200kv_kv4_chunk_workspace_bytes(batch, max_q_len, q_heads, kv_heads, KV4_HEAD_DIM)
-            else:
-                need = lib.b200kv_kv4_decode_workspace_bytes(batch, q_heads, kv_heads, KV4_HEAD_DIM)
-        if need == 0 and not max_q_len:
-            raise ValueError("unsupported decode shape: q_heads/kv_heads must be an integer <= 16, batch at most "
-                             f"4096 and batch * kv_heads at most {DECODE_COUNTER_BYTES // 4}")
-        _workspace_need[key] = need
-    return need
-
-
-def kv4_workspace(device_index: int, batch: int, max_q_len: int, q_heads: int, kv_heads: int) -> Optional[torch.Tensor]:
-    """Scratch of a decode step (``max_q_len`` 0) or a chunk on the device's current stream: arrival counters
+def _kv4_scratch(device_index: int, stream: int, capture: int, batch: int, max_q_len: int, q_heads: int,
+                 kv_heads: int) -> Optional[torch.Tensor]:
+    """Scratch of a decode step (``max_q_len`` 0) or a chunk on the (current) device's stream: arrival counters
     (zero between calls) and partials.  None for a chunk that needs none.
 
     Eager calls of one stream share one buffer (grown on demand): they follow one another.  A graph under
-    capture gets a buffer of its own out of its memory pool, whose counters are cleared by a node of
-    the graph, so graphs may be replayed next to each other and next to eager calls."""
-    need = _kv4_workspace_need(device_index, batch, max_q_len, q_heads, kv_heads)
+    capture (``capture`` names it, 0 for none) gets a buffer of its own out of its memory pool, whose
+    counters are cleared by a node of the graph, so graphs may be replayed next to each other and next to
+    eager calls."""
+    key = (device_index, batch, max_q_len, q_heads, kv_heads)
+    need = _kv4_need.get(key)
+    if need is None:
+        lib = _lib.lib()
+        if max_q_len:
+            need = lib.b200kv_kv4_chunk_workspace_bytes(batch, max_q_len, q_heads, kv_heads, KV4_HEAD_DIM)
+        else:
+            need = lib.b200kv_kv4_decode_workspace_bytes(batch, q_heads, kv_heads, KV4_HEAD_DIM)
+            if need == 0:
+                raise ValueError("unsupported decode shape: q_heads/kv_heads must be an integer <= 16, batch at most "
+                                 f"4096 and batch * kv_heads at most {DECODE_COUNTER_BYTES // 4}")
+        _kv4_need[key] = need
     if need == 0:
         return None
-    if _current_device() != device_index:
-        with torch.cuda.device(device_index):
-            return kv4_workspace(device_index, batch, max_q_len, q_heads, kv_heads)
-    stream = _stream(device_index)
     where = (device_index, stream)
-    capture = _capture_of(stream) if _capturing() else 0
     if capture:
         held = _kv4_graph_workspace.get(where)
         if held is not None and held[0] == capture and held[1].numel() >= need:
@@ -907,61 +857,30 @@ def kv4_workspace(device_index: int, batch: int, max_q_len: int, q_heads: int, k
     return ws
 
 
-# The launches as calls with packed arguments: (op, pack, number of words).
-_KV4_APPEND = (0, *_lib.kv4_packer("b200kv_kv4_append"))
-_KV4_PROLOGUE = (1, *_lib.kv4_packer("b200kv_kv4_qk_norm_rope_append"))
-_KV4_GATHER = (2, *_lib.kv4_packer("b200kv_kv4_gather"))
-_KV4_DECODE = (3, *_lib.kv4_packer("b200kv_kv4_paged_decode"))
-_KV4_PREFILL = (4, *_lib.kv4_packer("b200kv_kv4_paged_prefill"))
-
-
-def _kv4_call(call: tuple, dev: int, *args) -> None:
-    """Launch on ``dev``'s current stream; ``args`` are all but the last two (status word and stream)."""
-    op, pack, n = call
-    words = pack(*args, _status_ptr(dev), _stream(dev))
-    if _current_device() == dev:
-        rc = _lib.lib().b200kv_kv4_call(op, words, n)
-    else:
-        with torch.cuda.device(dev):
-            rc = _lib.lib().b200kv_kv4_call(op, words, n)
-    if rc != 0:
-        _lib.check(rc)
-    if _DEBUG:
-        check_status(dev)
-
-
 def update_kv_buffer_kv4(KV_Values: torch.Tensor, Select_Index: torch.Tensor, KV4_Buffer: torch.Tensor) -> None:
     """:func:`update_kv_buffer` into a 4-bit pool: row ``i`` of ``KV_Values`` ``[num_tokens, 2*kv_heads,
     128]`` (fp16) is quantised in groups of 32 elements and written to slot ``Select_Index[i]``.
 
     A slot outside the pool is skipped and reported in the device status.  Two tokens of one call
     may name the same slot only with identical rows."""
-    dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
-    slots = _slots_arg(Select_Index, dev)
-    n = slots.shape[0]
-    k_ptr, stride = _rows_arg(KV_Values, "KV_Values", 2 * kvh, n, dev)
-    if n == 0:
-        return
     if _DEBUG:
-        _debug_check_append(KV_Values, slots, pages * KV4_PAGE_SIZE)
-    _kv4_call(_KV4_APPEND, dev, k_ptr, k_ptr + kvh * KV4_HEAD_DIM * 2, n, stride, stride, slots.data_ptr(), ptr, pages,
-              page_stride, kvh, KV4_HEAD_DIM)
+        _debug_check_append(KV_Values, Select_Index, KV4_Buffer.shape[0] * KV4_PAGE_SIZE)
+    _kv4.append(KV_Values, None, Select_Index, KV4_Buffer)
+    if _DEBUG:
+        check_status(KV4_Buffer.get_device())
 
 
 def update_kv_buffer_kv4_split(xk: torch.Tensor, xv: torch.Tensor, Select_Index: torch.Tensor,
                                KV4_Buffer: torch.Tensor) -> None:
     """:func:`update_kv_buffer_kv4` with K and V given separately (``[num_tokens, kv_heads, 128]`` each)."""
-    dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
-    slots = _slots_arg(Select_Index, dev)
-    n = slots.shape[0]
-    k_ptr, k_stride = _rows_arg(xk, "xk", kvh, n, dev)
-    v_ptr, v_stride = _rows_arg(xv, "xv", kvh, n, dev)
-    if n == 0:
-        return
+    if xv is None:
+        raise ValueError("xv must be float16 [num_tokens, kv_heads, 128]")
     if _DEBUG:
-        _debug_check_append(torch.cat([xk[:n], xv[:n]], dim=1), slots, pages * KV4_PAGE_SIZE)
-    _kv4_call(_KV4_APPEND, dev, k_ptr, v_ptr, n, k_stride, v_stride, slots.data_ptr(), ptr, pages, page_stride, kvh,
-              KV4_HEAD_DIM)
+        n = Select_Index.shape[0]
+        _debug_check_append(torch.cat([xk[:n], xv[:n]], dim=1), Select_Index, KV4_Buffer.shape[0] * KV4_PAGE_SIZE)
+    _kv4.append(xk, xv, Select_Index, KV4_Buffer)
+    if _DEBUG:
+        check_status(KV4_Buffer.get_device())
 
 
 def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_weight: Optional[torch.Tensor],
@@ -971,53 +890,15 @@ def fused_qk_norm_rope_append_kv4(xq: torch.Tensor, xkv: torch.Tensor, q_norm_we
     """:func:`fused_qk_norm_rope_append` into a 4-bit pool: QK-RMSNorm, rotary embedding, and the
     quantising append of K (normalised, rotated, rounded to fp16) and V in one launch.  Arguments and
     return value as there."""
-    dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
-    d = KV4_HEAD_DIM
-    if xq.dim() != 3 or xq.shape[1] == 0:
-        raise ValueError(f"xq must be float16 [n, q_heads, {d}]")
-    n, qh, _ = xq.shape
-    q_ptr, q_stride = _rows_arg(xq, "xq", qh, n, dev)
-    if out is None:
-        out, out_ptr, out_stride = xq, q_ptr, q_stride
-    else:
-        if out.shape != xq.shape:
-            raise ValueError("out must match xq")
-        out_ptr, out_stride = _rows_arg(out, "out", qh, n, dev)
-    row = 2 * kvh * d
-    if xkv.dim() == 3 and xkv.shape[1:] == (2 * kvh, d):
-        xkv = xkv.reshape(n, row) if xkv.shape[0] == n else xkv
-    kv_strides = xkv.stride()
-    if xkv.dtype is not torch.float16 or xkv.shape != (n, row) or kv_strides[1] != 1:
-        raise ValueError("xkv must be [n, 2*kv_heads*head_dim] float16, contiguous rows")
-    if xkv.get_device() != dev:
-        raise _off_device("xkv", xkv, dev)
+    if xkv.dim() == 3 and xkv.shape[2] == KV4_HEAD_DIM:
+        xkv = xkv.flatten(1)
     if cos.dim() != 2 or sin.dim() != 2:
         cos, sin = cos.reshape(-1, cos.shape[-1]), sin.reshape(-1, sin.shape[-1])
-    (rows, width), (cs_stride, cos_step), (sin_stride, sin_step) = cos.shape, cos.stride(), sin.stride()
-    if cos.dtype is not torch.float16 or sin.dtype is not torch.float16:
-        raise ValueError("cos and sin must be float16")
-    if rows != n or sin.shape != cos.shape or (width != d and width != d // 2) or cos_step != 1 or sin_step != 1 \
-            or (n > 1 and cs_stride != sin_stride):
-        raise ValueError("cos and sin must be one row of head_dim (or head_dim/2) per token with equal strides")
-    if cos.get_device() != dev or sin.get_device() != dev:
-        raise _off_device("cos and sin", cos if cos.get_device() != dev else sin, dev)
-    for w, name in ((q_norm_weight, "q_norm_weight"), (k_norm_weight, "k_norm_weight")):
-        if w is not None:
-            if w.dtype is not torch.float16 or w.shape != (d,) or not w.is_contiguous():
-                raise ValueError(f"{name} must be a contiguous float16 [head_dim] tensor or None")
-            if w.get_device() != dev:
-                raise _off_device(name, w, dev)
-    slots = _slots_arg(Select_Index, dev)
-    if slots.shape[0] != n:
-        raise ValueError("Select_Index must name one slot per token")
-    if n == 0:
-        return out
     if _DEBUG:
-        _debug_check_append(xkv, slots, pages * KV4_PAGE_SIZE)
-    _kv4_call(_KV4_PROLOGUE, dev, q_ptr, out_ptr, q_stride, out_stride, xkv.data_ptr(), kv_strides[0] if n > 1 else row,
-              0 if q_norm_weight is None else q_norm_weight.data_ptr(),
-              0 if k_norm_weight is None else k_norm_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(),
-              cs_stride if n > 1 else d, slots.data_ptr(), ptr, pages, page_stride, n, qh, kvh, d)
+        _debug_check_append(xkv, Select_Index, KV4_Buffer.shape[0] * KV4_PAGE_SIZE)
+    out = _kv4.prologue(xq, xkv, q_norm_weight, k_norm_weight, eps, cos, sin, Select_Index, KV4_Buffer, out)
+    if _DEBUG:
+        check_status(KV4_Buffer.get_device())
     return out
 
 
@@ -1025,19 +906,9 @@ def gather_kv_buffer_kv4(KV4_Buffer: torch.Tensor, Select_Index: torch.Tensor,
                          out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """The rows a 4-bit pool stands for: fp16 ``[n, 2*kv_heads, 128]``, row ``i`` from slot
     ``Select_Index[i]``.  A slot outside the pool gives zeros and is reported in the device status."""
-    dev, ptr, pages, page_stride, kvh = _kv4_pool(KV4_Buffer)
-    slots = _slots_arg(Select_Index, dev)
-    n, d = slots.shape[0], KV4_HEAD_DIM
-    if out is None:
-        out = torch.empty(n, 2 * kvh, d, dtype=torch.float16, device=slots.device)
-        out_ptr, out_stride = out.data_ptr(), 2 * kvh * d
-    else:
-        out_ptr, out_stride = _rows_arg(out, "out", 2 * kvh, n, dev)
-        if out.shape[0] != n:
-            raise ValueError(f"out must hold {n} rows")
-    if n == 0:
-        return out
-    _kv4_call(_KV4_GATHER, dev, ptr, pages, page_stride, slots.data_ptr(), n, out_ptr, out_stride, kvh, d)
+    out = _kv4.gather(KV4_Buffer, Select_Index, out)
+    if _DEBUG:
+        check_status(KV4_Buffer.get_device())
     return out
 
 
@@ -1057,44 +928,12 @@ def flash_decoding_kv4(
 ) -> torch.Tensor:
     """:func:`flash_decoding` over a 4-bit pool; the pool is passed whole instead of as a K and a V view.
     Every element counts as scale * (code - 8); a sequence of length 0 gives a zero row."""
-    dev, ptr, pages, page_stride, kv_heads = _kv4_pool(KV4_Buffer)
-    if q.dtype is not torch.float16 or q.dim() != 3:
-        raise ValueError(f"q must be float16 [batch, heads, {KV4_HEAD_DIM}], contiguous along head_dim")
-    batch, q_heads, d = q.shape
-    q_sb, q_sh, q_sd = q.stride()
-    if d != KV4_HEAD_DIM or q_sd != 1:
-        raise ValueError(f"q must be float16 [batch, heads, {KV4_HEAD_DIM}], contiguous along head_dim")
-    if q.get_device() != dev:
-        raise _off_device("q", q, dev)
-    tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols = _table_arg(b_req_tokens_table, table_kind, dev)
-    lens_ptr = _ints_arg(b_seq_len, "b_seq_len", batch, dev, True)
-    if b_req_idx is not None:
-        rows_ptr = _ints_arg(b_req_idx, "b_req_idx", batch, dev, False)
-    else:
-        rows_ptr = 0
-        if tbl_rows < batch:
-            raise ValueError("the table has fewer rows than the batch")
-    max_len = int(max_actual_seq_len)
-    if not 0 <= max_len <= tbl_cols * (page_size if kind == TABLE_BLOCK else 1):
-        raise ValueError("max_actual_seq_len exceeds the table width")
-    if out is None:
-        out = torch.empty_like(q) if q.is_contiguous() else torch.empty(batch, q_heads, d, dtype=torch.float16, device=q.device)
-        out_sb, out_sh = q_heads * d, d
-    else:
-        out_sb, out_sh, out_sd = out.stride() if out.dim() == 3 else (0, 0, 0)
-        if out.shape != q.shape or out.dtype is not torch.float16 or out_sd != 1:
-            raise ValueError("out must match q")
-        if out.get_device() != dev:
-            raise _off_device("out", out, dev)
-    if batch == 0:
-        return out
     if _DEBUG:
-        _debug_check_lengths(b_seq_len, max_len, b_req_idx, tbl_rows, "decode")
-    ws = kv4_workspace(dev, batch, 0, q_heads, kv_heads)
-    _kv4_call(_KV4_DECODE, dev, q.data_ptr(), q_sb, q_sh, ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows,
-              tbl_cols, rows_ptr, lens_ptr, b_seq_len.dtype is torch.int64, batch, q_heads, kv_heads, d, int(page_size),
-              float(qk_scale), max_len, ws.data_ptr(), ws.numel(), out.data_ptr(), out_sb, out_sh,
-              DECODE_SERIALIZED if metadata_fresh else 0)
+        _debug_check_lengths(b_seq_len, int(max_actual_seq_len), b_req_idx, b_req_tokens_table.shape[0], "decode")
+    out = _kv4.decode(q, KV4_Buffer, qk_scale, b_req_tokens_table, b_seq_len, int(max_actual_seq_len), b_req_idx, table_kind,
+                      page_size, out, metadata_fresh)
+    if _DEBUG:
+        check_status(KV4_Buffer.get_device())
     return out
 
 
@@ -1113,38 +952,16 @@ def paged_chunk_flash_attention_kv4(
     page_size: int = 16,
 ) -> torch.Tensor:
     """:func:`paged_chunk_flash_attention` over a 4-bit pool (passed whole); the chunk's own rows have been
-    appended to it.  ``sm_scale`` carries log2(e), as there.  Returns a tensor like ``q``."""
-    dev, ptr, pages, page_stride, kv_heads = _kv4_pool(KV4_Buffer)
-    if q.dtype is not torch.float16 or q.dim() != 3 or q.shape[2] != KV4_HEAD_DIM or q.stride(2) != 1:
-        raise ValueError(f"q must be float16 [tokens, heads, {KV4_HEAD_DIM}], contiguous along head_dim")
-    if q.get_device() != dev:
-        raise _off_device("q", q, dev)
-    tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols = _table_arg(req_token_table, table_kind, dev)
-    batch = q_seq_lens.shape[0] if q_seq_lens.dim() == 1 else -1
-    qlen_ptr = _ints_arg(q_seq_lens, "q_seq_lens", batch, dev, True)
-    ctx_ptr = _ints_arg(context_lens, "context_lens", batch, dev, True)
-    if context_lens.dtype is not q_seq_lens.dtype:
-        raise ValueError("context_lens and q_seq_lens must share dtype and shape")
-    ids_ptr = _ints_arg(req_ids, "req_ids", batch, dev, False)
-    start_ptr = _ints_arg(q_start_loc, "q_start_loc", batch, dev, False)
-    total_q, q_heads, d = q.shape
-    output = torch.empty_like(q) if q.is_contiguous() else torch.empty(total_q, q_heads, d, dtype=torch.float16, device=q.device)
-    if total_q == 0 or q_heads == 0 or batch == 0:
-        return output
+    appended to it.  ``sm_scale`` is positive and carries log2(e), as there.  Returns a tensor like ``q``."""
     if _DEBUG:
-        width = tbl_cols * (page_size if kind == TABLE_BLOCK else 1)
-        _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, tbl_rows, "paged prefill")
+        width = req_token_table.shape[1] * (page_size if table_kind == "block" else 1)
+        _debug_check_lengths(context_lens + q_seq_lens, width, req_ids, req_token_table.shape[0], "paged prefill")
         _debug_check_lengths(q_seq_lens, int(max_q_len), None, 0, "paged prefill chunk")   # longer ones are skipped
-    max_q_len = int(max_q_len)
-    # Scratch: chunks of few rows and heads are streamed like a decode step, and the keys of a few query tiles are cut
-    # into parts.  Beyond 128 rows only their number of 128-row tiles counts.
-    rows = max_q_len if max_q_len <= 128 else (max_q_len + 127) // 128 * 128
-    ws = kv4_workspace(dev, batch, rows, q_heads, kv_heads) if rows > 0 else None
-    _kv4_call(_KV4_PREFILL, dev, q.data_ptr(), q.stride(0) if total_q > 1 else q_heads * d, q.stride(1) if q_heads > 1 else d,
-              ptr, pages, page_stride, tbl_ptr, tbl_stride, kind, tbl_rows, tbl_cols, ids_ptr, start_ptr, ctx_ptr, qlen_ptr,
-              q_seq_lens.dtype is torch.int64, batch, total_q, max_q_len, q_heads, kv_heads, d, int(page_size), float(sm_scale),
-              output.data_ptr(), q_heads * d, d, 0 if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel())
-    return output
+    out = _kv4.prefill(q, KV4_Buffer, sm_scale, req_token_table, req_ids, q_start_loc, context_lens, q_seq_lens, int(max_q_len),
+                       table_kind, page_size)
+    if _DEBUG:
+        check_status(KV4_Buffer.get_device())
+    return out
 
 
 __all__ = [

@@ -4,6 +4,7 @@ inside a capture, many requests, the same slot twice, lengths that change under 
 
 Errors are counted as in test_gpu_kv4.py; where two calls do the same arithmetic they are held to equal bits."""
 
+import gc
 import math
 import os
 import subprocess
@@ -502,3 +503,83 @@ def test_chunks_of_many_columns_on_few_heads(lens, q_lens, qh, kvh):
     want, _, tol = c.want()
     _within(c.prefill("block"), want, tol)
     _within(c.prefill("token", torch.int32), want, tol)
+
+
+def test_every_argument_may_be_junk():
+    """Each argument of each operator replaced by objects of other kinds and tensors of other shapes: the call
+    raises, keeps no reference and launches nothing."""
+    c = Case(97, [20, 33], 4, 2, [1, 1])
+    q, pool, tbl, rows = c.q.to(DEV), c.pool.to(DEV), c.tables("block"), c.rows.to(DEV)
+    lens, one = torch.tensor(c.lens, device=DEV), torch.ones(2, dtype=torch.int64, device=DEV)
+    start = torch.tensor([0, 1], dtype=torch.int32, device=DEV)
+    kv, slots = _randn(98, (2, 4, 128)).to(DEV), torch.tensor([1, 2], dtype=torch.int32, device=DEV)
+    cs, w = torch.ones(2, 128, dtype=torch.float16, device=DEV), torch.ones(128, dtype=torch.float16, device=DEV)
+    tensors = [q, pool, tbl, rows, lens, one, start, kv, slots, cs, w]
+    before = [sys.getrefcount(t) for t in tensors]
+    calls = [
+        (kernels.update_kv_buffer_kv4, [kv, slots, pool], {}),
+        (kernels.update_kv_buffer_kv4_split, [kv[:, :2], kv[:, 2:], slots, pool], {}),
+        (kernels.fused_qk_norm_rope_append_kv4, [q, kv.flatten(1), w, w, 1e-6, cs, cs, slots, pool], {"out": torch.empty_like(q)}),
+        (kernels.gather_kv_buffer_kv4, [pool, slots], {"out": torch.empty_like(kv)}),
+        (kernels.flash_decoding_kv4, [q, pool, SCALE, tbl, lens, 33],
+         {"b_req_idx": rows, "table_kind": "block", "page_size": 16, "out": torch.empty_like(q)}),
+        (kernels.paged_chunk_flash_attention_kv4, [q, pool, SCALE, tbl, rows, start, lens - one, one, 1],
+         {"table_kind": "block", "page_size": 16}),
+    ]
+    junk = [7, "junk", [1], object(), torch.zeros(3, 3, 3, 3, device=DEV), torch.zeros(0, device=DEV), torch.zeros(2, 2),
+            torch.zeros(5, 128, dtype=torch.float16, device=DEV), torch.zeros((), device=DEV), torch.zeros(2, 4, 128, device=DEV)]
+    raised = pytest.raises
+    errors = (TypeError, ValueError, AttributeError, RuntimeError, IndexError)
+    for fn, args, kw in calls:
+        fn(*args, **kw)
+        # numbers, and what may be left out, are looked at below
+        for i, a in enumerate(args):
+            for j in junk:
+                if not isinstance(a, torch.Tensor) and isinstance(j, (int, torch.Tensor)):
+                    continue
+                with raised(errors):
+                    fn(*args[:i], j, *args[i + 1:], **kw)
+        for k, a in kw.items():
+            for j in junk:
+                if k == "page_size" and isinstance(j, (int, torch.Tensor)):
+                    continue
+                with raised(errors):
+                    fn(*args, **{**kw, k: j})
+    for bad in (1 << 40, -1, 1 << 70):
+        with pytest.raises((ValueError, OverflowError)):
+            kernels.flash_decoding_kv4(q, pool, SCALE, tbl, lens, 33, b_req_idx=rows, table_kind="block", page_size=bad)
+        with pytest.raises((ValueError, OverflowError)):
+            kernels.flash_decoding_kv4(q, pool, SCALE, tbl, lens, bad, b_req_idx=rows, table_kind="block")
+    del calls, args, kw, a, j
+    gc.collect()
+    assert [sys.getrefcount(t) for t in tensors] == before
+    torch.cuda.synchronize()
+    kernels.check_status(0)
+
+
+def test_tensors_of_a_device_that_is_not_current():
+    """Every other answer about the current device is another one: each call is made again with the tensors' own."""
+    c = Case(99, [40, 300], 4, 2, [1, 1])
+    want, tol, tol_p = c.want()
+    x = _randn(100, (2, 4, 128)).to(DEV)
+    slots = torch.tensor([int(s[3]) for s in c.slots], dtype=torch.int32, device=DEV)
+    cs = torch.ones(2, 128, dtype=torch.float16, device=DEV)
+    plain = [c.pool.to(DEV) for _ in (0, 1)]
+    kernels.update_kv_buffer_kv4(x, slots, plain[0])
+    q_plain = kernels.fused_qk_norm_rope_append_kv4(c.q.to(DEV), x.flatten(1), None, None, 1e-6, cs, cs, slots, plain[1])
+    asked = []
+    parts = kernels._kv4_parts()
+    parts["current_device"] = lambda: asked.append(0) or len(asked) % 2
+    kernels._kv4.setup(parts)
+    try:
+        _within(c.decode(), want, tol)
+        _within(c.prefill(), want, tol_p)
+        pools = [c.pool.to(DEV) for _ in (0, 1)]
+        kernels.update_kv_buffer_kv4(x, slots, pools[0])
+        q = kernels.fused_qk_norm_rope_append_kv4(c.q.to(DEV), x.flatten(1), None, None, 1e-6, cs, cs, slots, pools[1])
+        rows = kernels.gather_kv_buffer_kv4(pools[0], slots)
+    finally:
+        kernels._kv4.setup(kernels._kv4_parts())
+    assert len(asked) == 10
+    assert torch.equal(pools[0], plain[0]) and torch.equal(pools[1], plain[1]) and torch.equal(q, q_plain)
+    assert torch.equal(rows.cpu(), K4.rows_of(plain[0].cpu(), slots.cpu()).half())

@@ -157,28 +157,24 @@ def test_prefill_refuses_a_scale_that_is_not_positive(built_lib, scale, ws):
         0, None, None) == EINVAL
 
 
-def test_packed_calls_reach_the_same_checks(built_lib):
-    """Each operator called with packed words answers as the plain entry point; wrong operations, counts and words
-    out of an int's range are refused."""
-    from llama_lite_npu_b200 import _lib
+def test_native_calls_refuse_what_is_no_tensor(built_lib):
+    """Objects of any kind in place of the pool, and wrong numbers of arguments, raise."""
+    import numpy as np
 
-    pack, n = _lib.kv4_packer("b200kv_kv4_gather")
-    good = [A, 8, 2 * 4 * 1152, A, 4, A, 1024, 4, 128, 0, 0]
-    assert n == len(good) == len(_lib._SIGNATURES["b200kv_kv4_gather"][1])
-    for at, value, code in ((8, 64, EUNSUPPORTED), (4, 0, 0), (4, -1, EINVAL), (6, 1028, EALIGN), (3, 0, EINVAL),
-                            (7, 1 << 33, EINVAL), (7, -(1 << 33) + 4, EINVAL)):
-        bad = list(good)
-        bad[at] = value
-        assert built_lib.b200kv_kv4_call(2, pack(*bad), n) == code, (at, value)
-    for op in (-1, 5, 0):
-        assert built_lib.b200kv_kv4_call(op, pack(*good), n) == EINVAL
-    assert built_lib.b200kv_kv4_call(2, pack(*good), n - 1) == EINVAL
-    assert built_lib.b200kv_kv4_call(2, None, n) == EINVAL
-    # floats travel as doubles: an epsilon below zero is refused, and so is a scale of zero
-    pack, n = _lib.kv4_packer("b200kv_kv4_qk_norm_rope_append")
-    fused = [A, A, 1024, 1024, A, 1024, 0, 0, -1.0, A, A, 64, A, A, 8, 2 * 4 * 1152, 4, 8, 4, 128, 0, 0]
-    assert built_lib.b200kv_kv4_call(1, pack(*fused), n) == EINVAL
-    pack, n = _lib.kv4_packer("b200kv_kv4_paged_prefill")
-    chunk = [A, 1024, 128, A, 8, 2 * 4 * 1152, A, 10, 0, 2, 10, A, A, A, A, 0, 2, 8, 4, 8, 4, 128, 16, 0.0, A, 1024, 128,
-             0, 0, 0, 0]
-    assert built_lib.b200kv_kv4_call(4, pack(*chunk), n) == EINVAL
+    from llama_lite_npu_b200 import _kv4_native as native
+
+    pool = kernels.empty_kv4_buffer(2, 1, device="cpu")
+    with pytest.raises(ValueError):
+        kernels.gather_kv_buffer_kv4(pool, torch.zeros(1, dtype=torch.int32))       # connects the module
+    counts = {"append": 4, "prologue": 10, "gather": 3, "decode": 11, "prefill": 11}
+    for name, n in counts.items():
+        fn = getattr(native, name)
+        for wrong in (0, 1, n - 1, n + 1):
+            with pytest.raises(TypeError):
+                fn(*([pool] * wrong))
+        for junk in (None, 3, 2.5, "pool", [1, 2], (1, 2, 3), np.zeros((2, 2, 1152), dtype=np.uint8), object(), torch.Tensor):
+            with pytest.raises((TypeError, ValueError, AttributeError)):
+                fn(*([junk] * n))
+    for bad in (None, {}, {"float16": 1}):
+        with pytest.raises((TypeError, KeyError)):
+            native.setup(bad)
