@@ -78,7 +78,7 @@ def check_status(device_index: Optional[int] = None) -> None:
             ws = _workspace.get(device_index)
             if ws is not None:
                 ws[:DECODE_COUNTER_BYTES].zero_()
-            for (dev, _), ws in _kv4_workspace.items():
+            for (dev, _), ws in list(_kv4_workspace.items()):
                 if dev == device_index:
                     ws[:DECODE_COUNTER_BYTES].zero_()
             torch.cuda.synchronize(device_index)
@@ -927,7 +927,8 @@ def flash_decoding_kv4(
     metadata_fresh: bool = False,
 ) -> torch.Tensor:
     """:func:`flash_decoding` over a 4-bit pool; the pool is passed whole instead of as a K and a V view.
-    Every element counts as scale * (code - 8); a sequence of length 0 gives a zero row."""
+    Every element counts as scale * (code - 8); a sequence of length 0 gives a zero row.  ``metadata_fresh=True``
+    where lengths, rows or table come from the kernel launched immediately before, as there."""
     if _DEBUG:
         _debug_check_lengths(b_seq_len, int(max_actual_seq_len), b_req_idx, b_req_tokens_table.shape[0], "decode")
     out = _kv4.decode(q, KV4_Buffer, qk_scale, b_req_tokens_table, b_seq_len, int(max_actual_seq_len), b_req_idx, table_kind,
