@@ -152,22 +152,25 @@ static int read_slots(PyObject* t, int64_t dev, PyObject** keep, int64_t* n, uin
 }
 
 /* fp16 head rows [n or more, heads, 128], contiguous inside a token */
+static int check_rows(const Tensor* x, const char* name, int64_t heads, int64_t n, int64_t dev, int64_t* stride, uintptr_t* ptr) {
+  if (x->dtype != st.f16 || x->nd != 3 || x->shape[1] != heads || x->shape[2] != kDim || x->shape[0] < n) {
+    PyErr_Format(PyExc_ValueError, "%s must be float16 [%lld or more, %lld, 128]", name, (long long)n, (long long)heads);
+    return -1;
+  }
+  if (x->stride[2] != 1 || (x->stride[1] != kDim && heads > 1)) {
+    PyErr_Format(PyExc_ValueError, "%s must be contiguous inside a token", name);
+    return -1;
+  }
+  if (x->dev != dev) return off_device(name, x->t, dev);
+  *stride = n > 1 ? x->stride[0] : heads * kDim;
+  return address(x->t, ptr);
+}
 static int read_rows(PyObject* t, const char* name, int64_t heads, int64_t n, int64_t dev, int64_t* stride, uintptr_t* ptr,
                      int64_t* rows) {
   Tensor x;
   if (read_tensor(t, &x) != 0) return -1;
-  if (x.dtype != st.f16 || x.nd != 3 || x.shape[1] != heads || x.shape[2] != kDim || x.shape[0] < n) {
-    PyErr_Format(PyExc_ValueError, "%s must be float16 [%lld or more, %lld, 128]", name, (long long)n, (long long)heads);
-    return -1;
-  }
-  if (x.stride[2] != 1 || (x.stride[1] != kDim && heads > 1)) {
-    PyErr_Format(PyExc_ValueError, "%s must be contiguous inside a token", name);
-    return -1;
-  }
-  if (x.dev != dev) return off_device(name, t, dev);
-  *stride = n > 1 ? x.stride[0] : heads * kDim;
-  if (rows != NULL) *rows = x.shape[0];
-  return address(t, ptr);
+  if (rows != NULL) *rows = x.nd > 0 ? x.shape[0] : 0;
+  return check_rows(&x, name, heads, n, dev, stride, ptr);
 }
 
 typedef struct {
@@ -193,18 +196,20 @@ static int read_table(PyObject* t, PyObject* kind, int64_t dev, Table* b) {
 }
 
 /* a contiguous 1-D tensor of n int32 (or, with wide != NULL, int64) values */
-static int read_ints(PyObject* t, const char* name, int64_t n, int64_t dev, int* wide, uintptr_t* ptr) {
-  Tensor x;
-  if (read_tensor(t, &x) != 0) return -1;
-  const int is64 = wide != NULL && x.dtype == st.i64;
-  if ((x.dtype != st.i32 && !is64) || x.nd != 1 || x.shape[0] != n || (x.stride[0] != 1 && n > 1)) {
+static int check_ints(const Tensor* x, const char* name, int64_t n, int64_t dev, int* wide, uintptr_t* ptr) {
+  const int is64 = wide != NULL && x->dtype == st.i64;
+  if ((x->dtype != st.i32 && !is64) || x->nd != 1 || x->shape[0] != n || (x->stride[0] != 1 && n > 1)) {
     PyErr_Format(PyExc_ValueError, "%s must be a contiguous 1-D %s tensor of %lld values", name,
                  wide != NULL ? "int32 or int64" : "int32", (long long)n);
     return -1;
   }
-  if (x.dev != dev) return off_device(name, t, dev);
+  if (x->dev != dev) return off_device(name, x->t, dev);
   if (wide != NULL) *wide = is64;
-  return address(t, ptr);
+  return address(x->t, ptr);
+}
+static int read_ints(PyObject* t, const char* name, int64_t n, int64_t dev, int* wide, uintptr_t* ptr) {
+  Tensor x;
+  return read_tensor(t, &x) != 0 ? -1 : check_ints(&x, name, n, dev, wide, ptr);
 }
 
 /* ---- launching --------------------------------------------------------------------------------------- */
@@ -392,7 +397,7 @@ static PyObject* py_prologue(PyObject* self, PyObject* const* args, Py_ssize_t n
   const int64_t n = q.shape[0], q_heads = q.shape[1], row = 2 * pool.kv_heads * kDim;
   int64_t qs = 0, os = 0, rows = 0, n_slots = 0;
   uintptr_t qp = 0, op = 0, kvp = 0, cp = 0, sp = 0, qw = 0, kw = 0, slp = 0;
-  if (read_rows(args[0], "xq", q_heads, n, pool.dev, &qs, &qp, NULL) != 0) return NULL;
+  if (check_rows(&q, "xq", q_heads, n, pool.dev, &qs, &qp) != 0) return NULL;
   if (out == args[0]) {
     op = qp;
     os = qs;
@@ -580,7 +585,7 @@ static PyObject* py_prefill(PyObject* self, PyObject* const* args, Py_ssize_t na
   if (batch > INT32_MAX) return fail("q_seq_lens is too long"), NULL;
   int wide = 0, ctx_wide = 0;
   uintptr_t qlens = 0, ctx = 0, ids = 0, start = 0, qp = 0, op = 0, wp = 0;
-  if (read_ints(args[7], "q_seq_lens", batch, pool.dev, &wide, &qlens) != 0 ||
+  if (check_ints(&ql, "q_seq_lens", batch, pool.dev, &wide, &qlens) != 0 ||
       read_ints(args[6], "context_lens", batch, pool.dev, &ctx_wide, &ctx) != 0)
     return NULL;
   if (wide != ctx_wide) return fail("context_lens and q_seq_lens must share dtype and shape"), NULL;
