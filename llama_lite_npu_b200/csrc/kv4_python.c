@@ -7,7 +7,7 @@
  * outputs come from torch.empty, scratch and the status word from the Python module, and the entry points are
  * the C ABI of include/b200kv_kv4.h, whose addresses setup() is given.
  *
- * Host time per call, us, this / the same checks in Python with the launch through ctypes: decode 7.2 / 13.3, append
+ * Host time per call, us, this / the same checks in Python with the launch through ctypes: decode 6.8 / 13.3, append
  * 3.8 / 6.8, read-back 5.5 / 8.4; a launch takes 2.9 of them and a new output tensor 1.5.
  */
 #define PY_SSIZE_T_CLEAN
@@ -286,6 +286,16 @@ static int done(int rc) {
   Py_DECREF(r);
   return fail("a launch was refused");
 }
+/* Scratch of the last few eager shapes; the Python module owns the policy, and forget() drops what is held here. */
+typedef struct {
+  int64_t dev, batch, rows, q_heads, kv_heads, bytes;
+  uintptr_t stream, ptr;
+  PyObject* ws;       /* owned; NULL: the entry is free */
+} Scratch;
+enum { kHeld = 4 };
+static Scratch held[kHeld];
+static int held_next;
+
 /* scratch: its address and bytes, and a reference that keeps it until the launch is made (NULL for none) */
 static int read_scratch(int64_t dev, uintptr_t stream, int64_t batch, int64_t rows, int64_t q_heads, int64_t kv_heads,
                         PyObject** keep, uintptr_t* ptr, int64_t* bytes) {
@@ -294,6 +304,18 @@ static int read_scratch(int64_t dev, uintptr_t stream, int64_t batch, int64_t ro
   *ptr = 0;
   *bytes = 0;
   if (done(st.capture_id((void*)stream, &capture)) != 0) return -1;
+  if (capture == 0) {
+    for (int i = 0; i < kHeld; ++i) {
+      const Scratch* h = &held[i];
+      if (h->ws != NULL && h->dev == dev && h->stream == stream && h->batch == batch && h->rows == rows &&
+          h->q_heads == q_heads && h->kv_heads == kv_heads) {
+        *keep = Py_NewRef(h->ws);
+        *ptr = h->ptr;
+        *bytes = h->bytes;
+        return 0;
+      }
+    }
+  }
   PyObject* args = Py_BuildValue("(LKKLLLL)", (long long)dev, (unsigned long long)stream, (unsigned long long)capture,
                                  (long long)batch, (long long)rows, (long long)q_heads, (long long)kv_heads);
   if (args == NULL) return -1;
@@ -315,7 +337,18 @@ static int read_scratch(int64_t dev, uintptr_t stream, int64_t batch, int64_t ro
   }
   Py_DECREF(shape);
   *bytes = dims[0];
+  if (capture == 0) {
+    Scratch* h = &held[held_next];
+    PyObject* old = h->ws;
+    *h = (Scratch){dev, batch, rows, q_heads, kv_heads, *bytes, stream, *ptr, Py_NewRef(ws)};
+    held_next = (held_next + 1) % kHeld;
+    Py_XDECREF(old);
+  }
   return 0;
+}
+static PyObject* py_forget(PyObject* self, PyObject* none) {
+  for (int i = 0; i < kHeld; ++i) Py_CLEAR(held[i].ws);
+  Py_RETURN_NONE;
 }
 static int wanted(Py_ssize_t n, Py_ssize_t want) {
   if (n == want) return 0;
@@ -648,6 +681,7 @@ static PyObject* py_setup(PyObject* self, PyObject* with) {
 
 static PyMethodDef methods[] = {
     {"setup", py_setup, METH_O, NULL},
+    {"forget", py_forget, METH_NOARGS, NULL},
     {"append", (PyCFunction)(void (*)(void))py_append, METH_FASTCALL, NULL},
     {"prologue", (PyCFunction)(void (*)(void))py_prologue, METH_FASTCALL, NULL},
     {"gather", (PyCFunction)(void (*)(void))py_gather, METH_FASTCALL, NULL},

@@ -81,6 +81,8 @@ def check_status(device_index: Optional[int] = None) -> None:
             for (dev, _), ws in list(_kv4_workspace.items()):
                 if dev == device_index:
                     ws[:DECODE_COUNTER_BYTES].zero_()
+            if not isinstance(_kv4, _Kv4Native):
+                _kv4.forget()     # it may hold scratch that has been replaced since
             torch.cuda.synchronize(device_index)
         raise RuntimeError(f"b200kv device status {code}: {_lib.strerror(code)}")
 
@@ -795,7 +797,7 @@ class _Kv4Native:
 
 # The checks and launches of the 4-bit operators (csrc/kv4_python.c).  A call reads about thirty tensor attributes and
 # its kernel takes a few microseconds.  Host time per call, us, with the checks in Python and the launch through
-# ctypes / here: decode 13.3 / 7.2, append 6.8 / 3.8, read-back 8.4 / 5.5.
+# ctypes / here: decode 13.3 / 6.8, append 6.8 / 3.8, read-back 8.4 / 5.5.
 _kv4 = _Kv4Native()
 
 

@@ -583,3 +583,33 @@ def test_tensors_of_a_device_that_is_not_current():
     assert len(asked) == 10
     assert torch.equal(pools[0], plain[0]) and torch.equal(pools[1], plain[1]) and torch.equal(q, q_plain)
     assert torch.equal(rows.cpu(), K4.rows_of(plain[0].cpu(), slots.cpu()).half())
+
+
+def test_counters_are_cleared_after_a_wait_that_ran_out():
+    """A reported time-out clears the scratch of every shape that was in use, a larger shape's and the smaller one's."""
+    a, b = Case(131, [3000, 40], 8, 1), Case(132, [400] * 9, 16, 4)
+    want = [c.decode().clone() for c in (a, b, a)][1:]
+    for ws in kernels._kv4_workspace.values():
+        ws[: kernels.DECODE_COUNTER_BYTES] = 1
+    kernels.status_tensor(0).fill_(104)
+    with pytest.raises(RuntimeError, match="104"):
+        kernels.check_status(0)
+    assert not any(bool(ws[: kernels.DECODE_COUNTER_BYTES].any()) for ws in kernels._kv4_workspace.values())
+    for _ in range(2):
+        assert torch.equal(b.decode(), want[0]) and torch.equal(a.decode(), want[1])
+
+
+def test_many_shapes_on_many_streams():
+    """More shapes and streams than scratch is remembered for, in turn."""
+    cases = [Case(140 + i, [50 * i + 5, 700 - 90 * i], 4 * (1 + i % 3), 1 + i % 2) for i in range(7)]
+    want = [c.decode().clone() for c in cases]
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    torch.cuda.synchronize()
+    for r in range(3):
+        outs = []
+        for i, c in enumerate(cases):
+            with torch.cuda.stream(streams[(i + r) % 3]):
+                outs.append(c.decode())
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)
